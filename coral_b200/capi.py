@@ -14,6 +14,8 @@ import numpy as np
 from . import build as _build
 
 L2, IP = 0, 1
+F32, BF16, F16 = 0, 1, 2
+TOPK_MAX = 1024
 STATS_W = 8
 STAT_NAMES = ("status", "n_dist", "n_exp", "rounds", "hops", "n_scan", "max_cand", "n_spill")
 OK, ERR_ARG, ERR_STATE, ERR_CUDA, ERR_NOGPU, ERR_KERNEL, ERR_LIMIT, ERR_QUERY = range(8)
@@ -33,6 +35,8 @@ EXPORTS = (
     "coral_merge_shards_strided", "coral_comm_unique_id", "coral_comm_create", "coral_comm_create_all",
     "coral_comm_set_id_map", "coral_comm_destroy", "coral_comm_world", "coral_comm_rank", "coral_comm_last_error", "coral_query_slice",
     "coral_search_sharded",
+    "coral_fp8_code_pitch", "coral_fp8_scale_pitch", "coral_fp8_quantize", "coral_fp8_scores", "coral_adjust_scores",
+    "coral_topk_workspace", "coral_topk_scores", "coral_scores_check",
     "coral_map_ids", "coral_last_error", "coral_search_static", "coral_search_static_status",
 )
 
@@ -112,6 +116,17 @@ def load():
         "coral_comm_last_error": (C.c_char_p, [vp]),
         "coral_query_slice": (None, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
         "coral_search_sharded": (C.c_int, [vp, vp, i32p, f32p, C.c_int, C.c_int, C.c_int, i32p, f32p, vp]),
+        "coral_fp8_code_pitch": (C.c_int64, [C.c_int]),
+        "coral_fp8_scale_pitch": (C.c_int64, [C.c_int]),
+        "coral_fp8_quantize": (C.c_int, [vp, vp, C.c_int, C.c_int64, C.c_int, C.c_int64, vp, vp, vp]),
+        "coral_fp8_scores": (C.c_int, [vp, vp, vp, C.c_int, vp, vp, C.c_int64, C.c_int, C.c_float, vp, vp, C.c_int,
+                                       C.c_int64, vp]),
+        "coral_adjust_scores": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int64, C.c_int64, vp, C.c_int, vp, vp, vp, C.c_int,
+                                          vp, C.c_int64, vp, C.c_int64, vp]),
+        "coral_topk_workspace": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, i64p]),
+        "coral_topk_scores": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int32, vp, vp, vp,
+                                        C.c_int64, vp]),
+        "coral_scores_check": (C.c_int, [vp]),
         "coral_last_error": (C.c_char_p, [vp]),
         "coral_search_static": (C.c_int, [C.c_int, vp, f32p, i32p, C.c_int64, C.c_int, C.c_int, C.c_int, i32p, C.c_int,
                                           f32p, C.c_int, C.c_int, C.c_int, i32p, f32p]),
@@ -141,6 +156,23 @@ def _ptr(x, dtype):
         return C.c_void_p(x.data_ptr()), x
     a = np.ascontiguousarray(x, dtype=dtype)
     return C.c_void_p(a.ctypes.data), a
+
+
+_score_types = {}
+
+
+def _score_type(t, name: str) -> int:
+    if not _score_types:
+        import torch
+        _score_types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    code = _score_types.get(t.dtype)
+    if code is None:
+        raise CoralError(ERR_ARG, f"{name} must be float32, bfloat16 or float16")
+    return code
+
+
+def _refuse(name: str, what: str):
+    raise CoralError(ERR_ARG, f"{name} must be {what}")
 
 
 class Index:
@@ -438,3 +470,131 @@ class Index:
     def map_ids(self, d_ids, d_id_map, stream=None):
         self._check(self._lib.coral_map_ids(self._h, C.c_void_p(d_ids.data_ptr()), int(d_ids.numel()),
                                             C.c_void_p(d_id_map.data_ptr()), C.c_void_p(stream) if stream else None))
+
+    # ---- operators on score rows: CUDA tensors, enqueued on torch's current stream of the handle's device
+    def _stream(self):
+        """torch's default stream, whose handle is 0, is CUDA's legacy stream (1): in the C calls 0 stands
+        for the handle's own stream."""
+        import torch
+        return torch._C._cuda_getCurrentRawStream(self.device) or 1
+
+    def _on_device(self, name: str, t, dtypes, shape=None, contiguous=True):
+        """Checks of a tensor argument that the C call cannot make."""
+        if not (_is_torch(t) and t.is_cuda and t.device.index == self.device):
+            _refuse(name, f"a tensor of cuda:{self.device}")
+        if dtypes is not None and t.dtype not in dtypes:
+            _refuse(name, " or ".join(str(d) for d in dtypes))
+        if shape is not None and tuple(t.shape) != shape:
+            _refuse(name, f"of shape {list(shape)}")
+        if contiguous and not t.is_contiguous():
+            _refuse(name, "contiguous")
+        return t.data_ptr()
+
+    def _rows(self, name: str, t):
+        """(pointer, type, rows, columns, elements between rows) of a matrix whose rows are contiguous."""
+        p = self._on_device(name, t, None, contiguous=False)
+        if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+            _refuse(name, "a matrix with contiguous rows")
+        return p, _score_type(t, name), t.shape[0], t.shape[1], max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+    def fp8_quantize(self, x, out=None):
+        """Compresses the rows of a float matrix: (codes float8_e4m3fn [rows, code pitch], scales
+        float8_e8m0fnu [rows, scale pitch]); see coral_fp8_quantize.  `out` = such a pair to write to,
+        e.g. the rows of a larger base at which new ones start."""
+        import torch
+        p, kind, rows, dim, ld = self._rows("x", x)
+        cp, sp = self._lib.coral_fp8_code_pitch(dim), self._lib.coral_fp8_scale_pitch(dim)
+        if cp == 0:
+            _refuse("x", "1 to 65536 columns wide")
+        if out is None:
+            codes = torch.empty((rows, cp), dtype=torch.float8_e4m3fn, device=x.device)
+            scales = torch.empty((rows, sp), dtype=torch.float8_e8m0fnu, device=x.device)
+        else:
+            codes, scales = out
+        self._check(self._lib.coral_fp8_quantize(
+            self._h, p, kind, rows, dim, ld, self._on_device("codes", codes, (torch.float8_e4m3fn,), (rows, cp)),
+            self._on_device("scales", scales, (torch.float8_e8m0fnu,), (rows, sp)), self._stream()))
+        return codes, scales
+
+    def fp8_scores(self, queries, base, dim: int, alpha: float = 1.0, bias=None, dtype=None, out=None):
+        """alpha * <query, row> + bias[row] of compressed queries and base rows (pairs as fp8_quantize
+        returns them) of `dim` columns: [Q, n] in `dtype` (float32 unless given), or into `out`, whose
+        rows may be apart.  See coral_fp8_scores."""
+        import torch
+        cp, sp = self._lib.coral_fp8_code_pitch(dim), self._lib.coral_fp8_scale_pitch(dim)
+        if cp == 0:
+            raise CoralError(ERR_ARG, "dim must be in [1, 65536]")
+        Q, n = queries[0].shape[0], base[0].shape[0]
+        p = [self._on_device(f"{name} {part}", pair[i], (kind,), (rows, pitch))
+             for name, pair, rows in (("queries'", queries, Q), ("base's", base, n))
+             for i, part, kind, pitch in ((0, "codes", torch.float8_e4m3fn, cp), (1, "scales", torch.float8_e8m0fnu, sp))]
+        if out is None:
+            # rows start at multiples of 16 bytes whatever n: what follows loads and stores whole vectors
+            dtype = dtype or torch.float32
+            per = 16 // dtype.itemsize
+            out = torch.empty((Q, -(-n // per) * per), dtype=dtype, device=base[0].device)
+            if out.shape[1] != n:
+                out = out[:, :n]
+        elif dtype is not None and out.dtype != dtype:
+            _refuse("out", str(dtype))
+        po, kind, rows, cols, ld = self._rows("out", out)
+        if (rows, cols) != (Q, n):
+            _refuse("out", f"of shape {[Q, n]}")
+        pb = None if bias is None else self._on_device("bias", bias, (torch.float32,), (n,))
+        self._check(self._lib.coral_fp8_scores(self._h, p[0], p[1], Q, p[2], p[3], n, dim, alpha, pb, po, kind, ld,
+                                               self._stream()))
+        return out
+
+    def adjust_scores(self, scores, seen=None, penalties=None, bias_ids=None, bias=None, excluded=None, out=None):
+        """Rules on a matrix of scores (see coral_adjust_scores): seen int32 [Q, *] with -1 padding,
+        penalties float32 [Q, 3] (repetition, frequency, presence), bias_ids int32 and bias float32
+        [Q, *], excluded int32 words [Q or 1, (n + 31) // 32].  Writes `out` (a new matrix unless given;
+        `scores` itself works in place) and returns it."""
+        import torch
+        p, kind, Q, n, ld = self._rows("scores", scores)
+        if out is None:
+            out = torch.empty_strided((Q, n), (ld, 1), dtype=scores.dtype, device=scores.device)
+        po, kind_out, rows, cols, ld_out = self._rows("out", out)
+        if (rows, cols, kind_out) != (Q, n, kind):
+            _refuse("out", f"{scores.dtype} of shape {[Q, n]}")
+        ps = pp = pi = pb = pe = None
+        n_seen = n_bias = ld_ex = 0
+        if seen is not None:
+            n_seen = seen.shape[1] if _is_torch(seen) and seen.dim() == 2 else -1
+            ps = self._on_device("seen", seen, (torch.int32,), (Q, n_seen))
+            pp = self._on_device("penalties", penalties, (torch.float32,), (Q, 3))
+        elif penalties is not None:
+            _refuse("seen", "given with penalties")
+        if bias_ids is not None:
+            n_bias = bias_ids.shape[1] if _is_torch(bias_ids) and bias_ids.dim() == 2 else -1
+            pi = self._on_device("bias_ids", bias_ids, (torch.int32,), (Q, n_bias))
+            pb = self._on_device("bias", bias, (torch.float32,), (Q, n_bias))
+        elif bias is not None:
+            _refuse("bias_ids", "given with bias")
+        if excluded is not None:
+            words = (n + 31) // 32
+            one = _is_torch(excluded) and excluded.dim() == 2 and excluded.shape[0] == 1
+            pe = self._on_device("excluded", excluded, (torch.int32,), (1 if one else Q, words))
+            ld_ex = 0 if one else words
+        self._check(self._lib.coral_adjust_scores(self._h, p, kind, Q, n, ld, ps, n_seen, pp, pi, pb, n_bias, pe, ld_ex, po,
+                                                  ld_out, self._stream()))
+        return out
+
+    def topk_scores(self, scores, k: int, id_base: int = 0):
+        """(ids int32 [Q, k], scores float32 [Q, k]) of the k largest of every row, best first, equal
+        scores by the lower column; see coral_topk_scores."""
+        import torch
+        p, kind, Q, n, ld = self._rows("scores", scores)
+        need = C.c_int64(0)
+        self._check(self._lib.coral_topk_workspace(self._h, Q, n, k, C.byref(need)))
+        ids = torch.empty((Q, k), dtype=torch.int32, device=scores.device)
+        best = torch.empty((Q, k), dtype=torch.float32, device=scores.device)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=scores.device) if need.value else None
+        self._check(self._lib.coral_topk_scores(self._h, p, kind, Q, n, ld, k, id_base, ids.data_ptr(), best.data_ptr(),
+                                                ws.data_ptr() if ws is not None else None, need.value,
+                                                self._stream()))
+        return ids, best
+
+    def scores_check(self):
+        """Raises when a bounded wait of an earlier fp8_scores ran out (call after synchronising)."""
+        self._check(self._lib.coral_scores_check(self._h))

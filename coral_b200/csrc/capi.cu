@@ -17,6 +17,7 @@
 #include "dense_topk.cuh"
 #include "plan.cuh"
 #include "schedule.cuh"
+#include "scores.cuh"
 #include "search_kernel.cuh"
 #include "start_select.cuh"
 
@@ -110,6 +111,7 @@ struct coral_index {
     unsigned long long* d_ctrl = nullptr;  // [0] q_counter(int) | err(int), [1] hops_total
     unsigned long long* h_ctrl = nullptr;  // pinned mirror
     int64_t* d_hits = nullptr;
+    int* h_scores_err = nullptr;           // pinned, written by the device when a bounded wait runs out
     std::map<int, std::pair<SearchPlan, int>> plans;  // L -> (plan, CTAs per SM)
 
     // graph build (NAP + CE): distances of the stored edges, degrees, claim words, batch scratch
@@ -389,6 +391,8 @@ int coral_index_create(coral_index_t** out, int device, int64_t n, int dim, int 
     if (e == cudaSuccess) e = cudaMalloc(&h->d_ctrl, kCtrlWords * sizeof(unsigned long long));
     if (e == cudaSuccess) e = cudaMallocHost(&h->h_ctrl, kCtrlWords * sizeof(unsigned long long));
     if (e == cudaSuccess) e = cudaMalloc(&h->d_hits, sizeof(int64_t));
+    if (e == cudaSuccess) e = cudaMallocHost(&h->h_scores_err, sizeof(int));
+    if (e == cudaSuccess) *h->h_scores_err = 0;
     if (e != cudaSuccess) {
         cudaGetLastError();
         std::string msg = std::string("handle set-up: ") + cudaGetErrorString(e);
@@ -419,6 +423,7 @@ int coral_index_destroy(coral_index_t* h) {
     cudaFree(h->d_claim);
     cudaFree(h->d_nap_scratch);
     if (h->h_ctrl) cudaFreeHost(h->h_ctrl);
+    if (h->h_scores_err) cudaFreeHost(h->h_scores_err);
     if (h->ev_t0) cudaEventDestroy(h->ev_t0);
     if (h->ev_k0) cudaEventDestroy(h->ev_k0);
     if (h->ev_k1) cudaEventDestroy(h->ev_k1);
@@ -1462,6 +1467,211 @@ int coral_map_ids(coral_index_t* h, int32_t* d_ids, int64_t count, const int32_t
     map_ids_kernel<<<blocks, 256, 0, st>>>(d_ids, count, d_id_map);
     h->launches += 1;
     CK(cudaGetLastError());
+    return CORAL_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// The device made current for one call, the caller's put back at its end.
+struct DeviceScope {
+    int before = -1;
+    bool ok = false;
+    explicit DeviceScope(int device) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        ok = before == device || cudaSetDevice(device) == cudaSuccess;
+        if (before == device) before = -1;
+        if (!ok) cudaGetLastError();
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// Whether the kernels of the handle's GPU may use p, `align` bytes aligned.
+bool usable(const coral_index* h, const void* p, size_t align) {
+    cudaPointerAttributes at;
+    if ((uintptr_t)p % align != 0) return false;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == h->device);
+}
+
+bool score_type(int type) { return type == CORAL_F32 || type == CORAL_BF16 || type == CORAL_F16; }
+size_t score_align(int type) { return (size_t)coral::type_bytes(type); }
+
+// Whether elements of two arrays of Q rows x n columns can share memory (pointers differ).
+bool rows_overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int size, int64_t Q, int64_t n) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    const uintptr_t ea = pa + (uintptr_t)(((Q - 1) * lda + n) * size), eb = pb + (uintptr_t)(((Q - 1) * ldb + n) * size);
+    if (ea <= pb || eb <= pa) return false;
+    if (lda != ldb) return true;
+    // columns of the same rows, side by side
+    const uintptr_t row = (uintptr_t)(lda * size), gap = (pb > pa ? pb - pa : pa - pb) % row;
+    return gap < (uintptr_t)(n * size) || row - gap < (uintptr_t)(n * size);
+}
+
+#define ARG(cond, text)                                             \
+    do {                                                            \
+        if (!(cond)) return fail(h, CORAL_ERR_ARG, text);           \
+    } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int64_t coral_fp8_code_pitch(int dim) { return dim < 1 || dim > coral::kFp8MaxDim ? 0 : coral::fp8_code_pitch(dim); }
+int64_t coral_fp8_scale_pitch(int dim) { return dim < 1 || dim > coral::kFp8MaxDim ? 0 : coral::fp8_scale_pitch(dim); }
+
+int coral_fp8_quantize(coral_index_t* h, const void* d_x, int type, int64_t rows, int dim, int64_t ld, uint8_t* d_codes,
+                       uint8_t* d_scales, void* stream) {
+    ARG(h, "null handle");
+    ARG(score_type(type), "type must be CORAL_F32, CORAL_BF16 or CORAL_F16");
+    ARG(dim >= 1 && dim <= coral::kFp8MaxDim, "dim must be in [1, 65536]");
+    ARG(rows >= 0 && rows <= 0x7fffffffll, "rows must be in [0, 2^31)");
+    ARG(ld >= dim && ld < (1ll << 31), "ld must be in [dim, 2^31)");
+    if (rows == 0) return CORAL_OK;
+    ARG(d_x && d_codes && d_scales, "null argument");
+    DeviceScope scope(h->device);
+    if (!scope.ok) return fail(h, CORAL_ERR_CUDA, "cudaSetDevice failed");
+    ARG(usable(h, d_x, score_align(type)) && usable(h, d_codes, 16) && usable(h, d_scales, 4),
+        "arrays must be aligned device memory of the handle's GPU");
+    CK(coral::launch_fp8_quantize(d_x, type, rows, dim, ld, d_codes, d_scales, h->sm_count,
+                                  stream ? (cudaStream_t)stream : h->stream));
+    h->launches += 1;
+    return CORAL_OK;
+}
+
+int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* d_q_scales, int Q, const uint8_t* d_codes,
+                     const uint8_t* d_scales, int64_t n, int dim, float alpha, const float* d_bias, void* d_out, int type,
+                     int64_t ld, void* stream) {
+    ARG(h, "null handle");
+    ARG(score_type(type), "type must be CORAL_F32, CORAL_BF16 or CORAL_F16");
+    ARG(dim >= 1 && dim <= coral::kFp8MaxDim, "dim must be in [1, 65536]");
+    ARG(Q >= 0 && n >= 0 && n <= 0x7fffffffll, "Q and n must be in [0, 2^31)");
+    ARG(ld >= n && ld < (1ll << 31), "ld must be in [n, 2^31)");
+    if (Q == 0 || n == 0) return CORAL_OK;
+    ARG(d_q_codes && d_q_scales && d_codes && d_scales && d_out, "null argument");
+    DeviceScope scope(h->device);
+    if (!scope.ok) return fail(h, CORAL_ERR_CUDA, "cudaSetDevice failed");
+    ARG(usable(h, d_q_codes, 16) && usable(h, d_q_scales, 4) && usable(h, d_codes, 16) && usable(h, d_scales, 4) &&
+            (!d_bias || usable(h, d_bias, 4)) && usable(h, d_out, score_align(type)),
+        "arrays must be aligned device memory of the handle's GPU");
+    coral::Fp8ScoresArgs a{};
+    a.q_codes = d_q_codes;
+    a.q_scales = d_q_scales;
+    a.codes = d_codes;
+    a.scales = d_scales;
+    a.Q = Q;
+    a.n = (int)n;
+    a.dim = dim;
+    a.alpha = alpha;
+    a.bias = d_bias;
+    a.out = d_out;
+    a.type = type;
+    a.ld = ld;
+    a.err = h->h_scores_err;
+    CK(coral::launch_fp8_scores(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
+    h->launches += 1;
+    return CORAL_OK;
+}
+
+int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q, int64_t n, int64_t ld,
+                        const int32_t* d_seen, int n_seen, const float* d_penalties, const int32_t* d_bias_ids,
+                        const float* d_bias, int n_bias, const uint32_t* d_excluded, int64_t ld_excluded, void* d_out,
+                        int64_t ld_out, void* stream) {
+    ARG(h, "null handle");
+    ARG(score_type(type), "type must be CORAL_F32, CORAL_BF16 or CORAL_F16");
+    ARG(Q >= 0 && n >= 0 && n <= 0x7fffffffll, "Q and n must be in [0, 2^31)");
+    ARG(ld >= n && ld < (1ll << 31) && ld_out >= n && ld_out < (1ll << 31), "ld and ld_out must be in [n, 2^31)");
+    ARG(n_seen >= 0 && n_bias >= 0, "negative list length");
+    if (n_bias > coral::kRulesMaxBias) return fail(h, CORAL_ERR_LIMIT, "n_bias must not exceed 1024");
+    if ((n + 8191) / 8192 * Q > 0x7fffffffll) return fail(h, CORAL_ERR_LIMIT, "too many score rows for one call");
+    if (Q == 0 || n == 0) return CORAL_OK;
+    ARG(d_scores && d_out && (n_seen == 0 || (d_seen && d_penalties)) && (n_bias == 0 || (d_bias_ids && d_bias)),
+        "null argument");
+    ARG(!d_excluded || ld_excluded == 0 || ld_excluded >= (n + 31) / 32, "ld_excluded must be 0 or at least (n + 31) / 32");
+    DeviceScope scope(h->device);
+    if (!scope.ok) return fail(h, CORAL_ERR_CUDA, "cudaSetDevice failed");
+    ARG(usable(h, d_scores, score_align(type)) && usable(h, d_out, score_align(type)) &&
+            (n_seen == 0 || (usable(h, d_seen, 4) && usable(h, d_penalties, 4))) &&
+            (n_bias == 0 || (usable(h, d_bias_ids, 4) && usable(h, d_bias, 4))) &&
+            (!d_excluded || usable(h, d_excluded, 4)),
+        "arrays must be aligned device memory of the handle's GPU");
+    if (d_out == d_scores)
+        ARG(ld == ld_out || Q == 1, "in place, ld_out must be ld");
+    else
+        ARG(!rows_overlap(d_scores, ld, d_out, ld_out, coral::type_bytes(type), Q, n), "d_out overlaps d_scores");
+    coral::RulesArgs a{};
+    a.in = d_scores;
+    a.out = d_out;
+    a.type = type;
+    a.Q = Q;
+    a.n = n;
+    a.ld = ld;
+    a.ld_out = ld_out;
+    a.seen = d_seen;
+    a.n_seen = n_seen;
+    a.penalties = d_penalties;
+    a.bias_ids = d_bias_ids;
+    a.bias = d_bias;
+    a.n_bias = n_bias;
+    a.excluded = d_excluded;
+    a.ld_excluded = ld_excluded;
+    CK(coral::launch_score_rules(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
+    h->launches += 1;
+    return CORAL_OK;
+}
+
+int coral_topk_workspace(coral_index_t* h, int Q, int64_t n, int k, int64_t* bytes_out) {
+    ARG(h && bytes_out, "null argument");
+    ARG(Q >= 0 && n >= 0 && n <= 0x7fffffffll && k >= 1, "Q and n must be in [0, 2^31) and k positive");
+    if (k > coral::kTopkMax) return fail(h, CORAL_ERR_LIMIT, "k must not exceed 1024");
+    *bytes_out = coral::topk_workspace_bytes(Q, n, k, h->sm_count);
+    return CORAL_OK;
+}
+
+int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, int64_t n, int64_t ld, int k,
+                      int32_t id_base, int32_t* d_ids_out, float* d_scores_out, void* d_workspace,
+                      int64_t workspace_bytes, void* stream) {
+    int64_t need = 0;
+    if (int rc = coral_topk_workspace(h, Q, n, k, &need)) return rc;
+    ARG(score_type(type), "type must be CORAL_F32, CORAL_BF16 or CORAL_F16");
+    ARG(ld >= n && ld < (1ll << 31), "ld must be in [n, 2^31)");
+    ARG(id_base >= 0 && id_base + n <= 0x7fffffffll, "id_base must be in [0, 2^31 - n)");
+    if (Q == 0) return CORAL_OK;
+    ARG((n == 0 || d_scores) && d_ids_out && d_scores_out && (need == 0 || d_workspace), "null argument");
+    if (workspace_bytes < need) return fail(h, CORAL_ERR_LIMIT, "workspace smaller than coral_topk_workspace");
+    DeviceScope scope(h->device);
+    if (!scope.ok) return fail(h, CORAL_ERR_CUDA, "cudaSetDevice failed");
+    ARG((n == 0 || usable(h, d_scores, score_align(type))) && usable(h, d_ids_out, 4) && usable(h, d_scores_out, 4) &&
+            (need == 0 || usable(h, d_workspace, 8)),
+        "arrays must be aligned device memory of the handle's GPU");
+    coral::TopkArgs a{};
+    a.in = d_scores;
+    a.type = type;
+    a.Q = Q;
+    a.n = n;
+    a.ld = ld;
+    a.k = k;
+    a.id_base = id_base;
+    a.ids_out = d_ids_out;
+    a.scores_out = d_scores_out;
+    a.ws = static_cast<uint64_t*>(d_workspace);
+    int launches = 0;
+    CK(coral::launch_topk(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream, &launches));
+    h->launches += launches;
+    return CORAL_OK;
+}
+
+int coral_scores_check(coral_index_t* h) {
+    ARG(h, "null handle");
+    const int err = *static_cast<volatile int*>(h->h_scores_err);
+    *h->h_scores_err = 0;
+    if (err) return fail(h, CORAL_ERR_KERNEL, "a bounded wait in the score kernel ran out; its scores are invalid");
     return CORAL_OK;
 }
 

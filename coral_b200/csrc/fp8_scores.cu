@@ -1,0 +1,505 @@
+// Rows in 8-bit floating point, and dense scores of such rows on the tcgen05 tensor cores.
+//
+// A row keeps its columns as e4m3 codes with one power-of-two scale (e8m0: a byte, 2^(byte - 127))
+// for each block of 128 columns: x ~ code * 2^e, e the least integer with max|x| <= 448 * 2^e.  A
+// power of two costs nothing against a free scale: the codes are floating point, so their relative
+// rounding (half a step, 2^-4) does not depend on where in the range a block sits, and scaling by
+// 2^e is exact.  It is also the scale the tensor cores apply themselves
+// (tcgen05.mma kind::mxf8f6f4.block_scale), so the accumulator needs no correction between blocks.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "scores.cuh"
+
+namespace coral {
+
+namespace {
+
+// ------------------------------------------------------------------------------- compression
+
+// Order of |v|.  What is not finite counts as nothing, and its code is NaN (e4m3 has no infinity): it
+// shows in every score of its row and costs the rest of its block no precision.
+__device__ __forceinline__ uint32_t abs_bits(float v) {
+    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+__device__ __forceinline__ float scaled(float v, float f) {
+    return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v * f : __uint_as_float(0x7fffffffu);
+}
+
+// Least e in [-127, 127] with amax <= 448 * 2^e, 448 = 1.75 * 2^8, from the bits of amax: the
+// exponent less 8, one more when the mantissa is above 1.75.  A subnormal or zero amax ends at -127.
+__device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+    const int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -127 ? -127 : e;
+}
+
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float wide(T v);
+template <>
+__device__ __forceinline__ float wide<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float wide<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float wide<__half>(__half v) { return __half2float(v); }
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantBlocks = 4;   // blocks of 128 columns a warp has in flight
+
+// One warp takes kQuantBlocks consecutive blocks, lane l the columns 4 l .. 4 l + 3 of each: a block
+// of fp32 is one coalesced 512-byte read, and its maximum one warp reduction over the magnitudes'
+// bits.  Bound by memory.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kQuantThreads)
+fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, uint8_t* __restrict__ codes,
+                    uint8_t* __restrict__ scales) {
+    const int lane = threadIdx.x & 31;
+    const int per_row = (dim + kFp8Block - 1) / kFp8Block;
+    const int code_pitch = (dim + 15) / 16 * 16, scale_pitch = (dim + 511) / 512 * 4;
+    const int64_t total = rows * per_row;
+    const int64_t first = ((int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5)) * kQuantBlocks;
+    if (first >= total) return;
+    int64_t row = total <= 0x7fffffff ? (int64_t)((uint32_t)first / (uint32_t)per_row) : first / per_row;
+    int b = (int)(first - row * per_row);
+    float v[kQuantBlocks][4];
+    int64_t r[kQuantBlocks];
+    int bb[kQuantBlocks];
+#pragma unroll
+    for (int u = 0; u < kQuantBlocks; ++u) {
+        r[u] = row;
+        bb[u] = b;
+        const int c = b * kFp8Block + lane * 4;
+        const T* p = x + row * ld + c;
+        if (first + u < total) {
+            if (VEC && c + 4 <= dim) {
+                if (sizeof(T) == 4) {
+                    *reinterpret_cast<float4*>(v[u]) = __ldcs(reinterpret_cast<const float4*>(p));
+                } else {
+                    alignas(8) T t[4];
+                    *reinterpret_cast<uint2*>(t) = __ldcs(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[u][i] = wide<T>(t[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[u][i] = c + i < dim ? wide<T>(p[i]) : 0.f;
+            }
+        }
+        if (++b == per_row) {
+            b = 0;
+            ++row;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kQuantBlocks; ++u) {
+        if (first + u >= total) break;
+        uint32_t m = max(max(abs_bits(v[u][0]), abs_bits(v[u][1])), max(abs_bits(v[u][2]), abs_bits(v[u][3])));
+        m = __reduce_max_sync(0xffffffffu, m);
+        const int e = scale_exponent(m);
+        const float f = __uint_as_float((uint32_t)(127 - e) << 23);     // 2^-e: e in [-127, 120], 2^-e never subnormal
+        const int c = bb[u] * kFp8Block + lane * 4;
+        if (c < code_pitch)
+            *reinterpret_cast<uint32_t*>(codes + r[u] * code_pitch + c) =
+                pack_e4m3(scaled(v[u][0], f), scaled(v[u][1], f), scaled(v[u][2], f), scaled(v[u][3], f));
+        uint8_t* s = scales + r[u] * scale_pitch + bb[u];
+        if (lane == 0) *s = (uint8_t)(e + 127);
+        // the last block's warp zeroes the scales that pad the row to a multiple of four
+        if (lane > 0 && bb[u] == per_row - 1 && bb[u] + lane < scale_pitch) s[lane] = 0;
+    }
+}
+
+template <typename T>
+cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t* codes, uint8_t* scales,
+                       cudaStream_t stream) {
+    const int64_t total = rows * ((dim + kFp8Block - 1) / kFp8Block);
+    const int per_cta = kQuantThreads / 32 * kQuantBlocks;
+    const int64_t ctas = (total + per_cta - 1) / per_cta;
+    const bool vec = ((uintptr_t)x | (uintptr_t)(ld * sizeof(T))) % (4 * sizeof(T)) == 0;
+    auto kernel = vec ? fp8_quantize_kernel<T, true> : fp8_quantize_kernel<T, false>;
+    kernel<<<(unsigned)ctas, kQuantThreads, 0, stream>>>(static_cast<const T*>(x), rows, dim, ld, codes, scales);
+    return cudaGetLastError();
+}
+
+// ----------------------------------------------------------------------------------- product
+//
+// out[q][j] = alpha * sum_b 2^(eq_b + ej_b) * (codes of q, codes of j)_b + bias[j], accumulated in
+// fp32 in tensor memory.  One persistent CTA of 8 warps per SM, tiles of 128 queries x 256 rows:
+//   warp 0     one lane issues the tiles' TMA loads (128-byte swizzle, 128 columns a stage);
+//   warp 1     one lane issues, per stage, three tcgen05.cp (the stage's scales to tensor memory)
+//              and four tcgen05.mma (M = 128, N = 256, K = 32);
+//   warp 2     brings the stage's scales to shared memory in the layout tcgen05.cp takes;
+//   warps 4-7  read the finished accumulator, apply alpha and bias, and store.
+// A scale word of four bytes covers 512 columns; an instruction's K = 32 lies inside one block, so
+// all four instructions of a stage name the same byte of the word (the scale ids of the instruction
+// descriptor), byte (k-block mod 4).
+//
+// Tensor memory: two accumulators of 256 columns that share 64 (0-255 and 192-447) and, from 448,
+// one slot of 16 columns of scales per stage.  The epilogue reads the shared columns first and then
+// lets the next tile's products start.
+
+constexpr int kTileM = 128, kTileN = 256, kTileK = 128;
+constexpr int kStages = 4;
+constexpr int kABytes = kTileM * kTileK, kBBytes = kTileN * kTileK;
+constexpr int kScaleBytes = (kTileM + kTileN) * 4;
+constexpr int kAccStep = 192, kShared = 64, kTmemScales = 448;
+constexpr int kOffScales = kStages * (kABytes + kBBytes);
+constexpr int kOffStage = kOffScales + kStages * kScaleBytes;       // epilogue staging
+constexpr int kStagePitch = 33;
+constexpr int kOffBars = kOffStage + 4 * 32 * kStagePitch * 4;
+constexpr int kSmemBytes = kOffBars + 256 + 1024;
+constexpr int kThreads = 256;
+constexpr long long kWaitClocks = 4000000000ll;                     // ~2 s
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t mbar_try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+        : "memory");
+    return ok;
+}
+// Bounded wait: gives up when the clock limit runs out or another role of the CTA gave up.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (uint32_t spins = 1;; ++spins) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((spins & 15u) == 0u) {
+            if (*abort_flag) return false;
+            if (clock64() - t0 > kWaitClocks) {
+                *abort_flag = 1;
+                atomicExch_system(err, 1);
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+        : "memory");
+}
+// Shared-memory matrix descriptor, K-major rows of 128 bytes with the 128-byte swizzle: 8-row groups
+// 1024 bytes apart, descriptor version 1, layout type 2.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// The same for 32 unswizzled rows of 16 bytes (scales): 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t desc_rows16(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
+}
+// Instruction descriptor of kind::mxf8f6f4: e4m3 x e4m3 (type 0), both K-major, e8m0 scales (bit 23),
+// N / 8 from bit 17, M / 128 from bit 27; the scale ids (A from bit 29, B from bit 4) are or-ed in.
+constexpr uint32_t kInstrDesc = (1u << 23) | ((uint32_t)(kTileN >> 3) << 17) | ((uint32_t)(kTileM >> 7) << 27);
+
+__device__ __forceinline__ void umma_mxf8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                          uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+        : "memory");
+}
+// 32 rows of 16 bytes to 4 columns of tensor memory, the same in each of the four lane groups.
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const Fp8ScoresArgs a, const int tiles_m, const int64_t tiles) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);   // [kStages] codes and scales landed
+    uint64_t* empty = full + kStages;                                // [kStages] the products that read the stage are done
+    uint64_t* tfull = empty + kStages;                               // accumulator complete
+    uint64_t* tfree = tfull + 1;                                     // the columns the next tile shares are drained
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int k_blocks = (a.dim + kTileK - 1) / kTileK;
+    const int scale_pitch = (a.dim + 511) / 512 * 4;
+
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 2);        // the TMA lane and the scale warp
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(tfull, 1);
+        mbar_init(tfree, 4);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t par = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                const int m0 = (int)(t % tiles_m) * kTileM, n0 = (int)(t / tiles_m) * kTileN;
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
+                    unsigned char* st = smem + s * (kABytes + kBBytes);
+                    mbar_expect_tx(&full[s], kABytes + kBBytes);
+                    tma_load_2d(st, &map_a, kb * kTileK, m0, &full[s]);
+                    tma_load_2d(st + kABytes, &map_b, kb * kTileK, n0, &full[s]);
+                    if (++s == kStages) {
+                        s = 0;
+                        par ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t par = 0, i = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
+                if (i > 0 && !mbar_wait(tfree, (i - 1) & 1u, abort_flag, a.err)) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + (i & 1u) * kAccStep;
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    if (!(ok = mbar_wait(&full[s], par, abort_flag, a.err))) break;
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + s * (kABytes + kBBytes)), sb = sa + kABytes;
+                    const uint32_t sc = smem_u32(smem + kOffScales + s * kScaleBytes);
+                    const uint32_t ta = tmem + kTmemScales + s * 16, tb = ta + 8;
+                    scales_to_tmem(ta, desc_rows16(sc));
+                    scales_to_tmem(tb, desc_rows16(sc + 512));
+                    scales_to_tmem(tb + 4, desc_rows16(sc + 1024));
+                    const uint32_t id = (uint32_t)(kb & 3);
+                    const uint32_t idesc = kInstrDesc | id << 29 | id << 4;
+#pragma unroll
+                    for (int j = 0; j < kTileK / 32; ++j)
+                        umma_mxf8(acc, desc_sw128(sa + j * 32), desc_sw128(sb + j * 32), idesc, ta, tb,
+                                  (kb | j) != 0 ? 1u : 0u);
+                    umma_commit(&empty[s]);
+                    if (++s == kStages) {
+                        s = 0;
+                        par ^= 1u;
+                    }
+                }
+                if (ok) umma_commit(tfull);
+            }
+        }
+    } else if (warp == 2) {
+        // Scales: lane l keeps the words of rows l, l + 32, ... of both tiles for four k-blocks.
+        int s = 0;
+        uint32_t par = 0;
+        bool ok = true;
+        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            const int64_t m0 = (t % tiles_m) * kTileM, n0 = (t / tiles_m) * kTileN;
+            uint32_t w[12];
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                if ((kb & 3) == 0) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int64_t r = m0 + g * 32 + lane;
+                        w[g] = r < a.Q ? *reinterpret_cast<const uint32_t*>(a.q_scales + r * scale_pitch + kb) : 0u;
+                    }
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const int64_t r = n0 + g * 32 + lane;
+                        w[4 + g] = r < a.n ? *reinterpret_cast<const uint32_t*>(a.scales + r * scale_pitch + kb) : 0u;
+                    }
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err));
+                if (!ok) break;
+                uint4* dst = reinterpret_cast<uint4*>(smem + kOffScales + s * kScaleBytes) + lane;
+                dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                dst[32] = make_uint4(w[4], w[5], w[6], w[7]);
+                dst[64] = make_uint4(w[8], w[9], w[10], w[11]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
+                if (++s == kStages) {
+                    s = 0;
+                    par ^= 1u;
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        const int g = warp & 3;                          // the 32 lanes of tensor memory this warp reads
+        float* stage = reinterpret_cast<float*>(smem + kOffStage) + g * 32 * kStagePitch;
+        uint32_t i = 0;
+        for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+            const int64_t m0 = (t % tiles_m) * kTileM + g * 32, n0 = (t / tiles_m) * kTileN;
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1u, abort_flag, a.err))) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16) + (i & 1u) * kAccStep;
+            // the accumulator's shared columns first: its last 64 or its first 64
+            const int start = (i & 1u) ? 0 : kTileN - kShared;
+            for (int c = 0; c < kTileN; c += 32) {
+                const int col = (start + c) & (kTileN - 1);
+                uint32_t r[32];
+                tmem_ld32(acc + (uint32_t)col, r);
+                tmem_ld_wait();
+                if (c + 32 == kShared) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tfree);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) stage[lane * kStagePitch + j] = __uint_as_float(r[j]);
+                __syncwarp();
+                const int64_t n = n0 + col + lane;
+                if (n < a.n) {
+                    const float b = a.bias ? a.bias[n] : 0.f;
+                    T* out = static_cast<T*>(a.out) + m0 * a.ld + n;
+                    const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);
+                    for (int j = 0; j < rows; ++j)
+                        out[j * a.ld] = narrow<T>(fmaf(a.alpha, stage[j * kStagePitch + lane], b));
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        // a wait ran out: give copies and products in flight time to land (bounded)
+        const long long t_end = clock64() + 20000000ll;
+        while (clock64() < t_end) {
+        }
+        __syncthreads();
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static std::mutex mu;
+    static EncodeTiledFn fn = nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &res) != cudaSuccess ||
+            res != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        fn = reinterpret_cast<EncodeTiledFn>(p);
+    }
+    return fn;
+}
+
+// Codes as a 2-D tensor (column, row); columns >= dim and rows past the end read zeros.
+bool codes_map(CUtensorMap* map, const uint8_t* codes, int64_t rows, int dim, int box_rows) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t gdim[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
+    const cuuint64_t gstride[1] = {(cuuint64_t)fp8_code_pitch(dim)};
+    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), gdim, gstride, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(fp8_scores_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    alignas(64) CUtensorMap map_a, map_b;
+    if (!codes_map(&map_a, a.q_codes, a.Q, a.dim, kTileM) || !codes_map(&map_b, a.codes, a.n, a.dim, kTileN))
+        return cudaErrorInvalidValue;
+    const int tiles_m = (a.Q + kTileM - 1) / kTileM;
+    const int64_t tiles = (int64_t)tiles_m * ((a.n + kTileN - 1) / kTileN);
+    const int grid = (int)(tiles < sm_count ? tiles : sm_count);
+    fp8_scores_kernel<T><<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, a, tiles_m, tiles);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_quantize(const void* x, int type, int64_t rows, int dim, int64_t ld, uint8_t* codes,
+                                uint8_t* scales, int, cudaStream_t stream) {
+    if (type == kTypeF32) return quantize_t<float>(x, rows, dim, ld, codes, scales, stream);
+    if (type == kTypeBf16) return quantize_t<__nv_bfloat16>(x, rows, dim, ld, codes, scales, stream);
+    return quantize_t<__half>(x, rows, dim, ld, codes, scales, stream);
+}
+
+cudaError_t launch_fp8_scores(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) {
+    if (a.type == kTypeF32) return scores_t<float>(a, sm_count, stream);
+    if (a.type == kTypeBf16) return scores_t<__nv_bfloat16>(a, sm_count, stream);
+    return scores_t<__half>(a, sm_count, stream);
+}
+
+}  // namespace coral

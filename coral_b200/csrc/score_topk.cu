@@ -1,0 +1,272 @@
+// The k best of every row of scores: ids and scores, best first, equal scores by the lower id.
+//
+// Keys: ord(score) in the high word (ord is monotone), the complement of the column in the low one,
+// so keys are unique and a larger key is better.  -inf (an excluded row) and NaN never become a key;
+// a row with fewer than k keys ends in padding (id -1).
+//
+// A CTA streams one slice of one row: every tile's scores are compared with the slice's threshold,
+// the k-th best score seen so far, and what beats it is appended to a buffer in shared memory that
+// always has room for one more tile.  Columns arrive in ascending order, so a score equal to the
+// threshold has a higher id than the k keys it would have to beat and loses.  When the buffer could
+// overflow, a radix selection (8-bit digits, from the top) cuts it to its k best and tightens the
+// threshold.  Rows are cut into slices while there are fewer rows than CTAs to keep busy; the k best
+// of each slice then meet in a second launch, which selects among keys in the same way.
+#include <math_constants.h>
+
+#include "scores.cuh"
+
+namespace coral {
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kTile = 8192;                 // scores per step of a CTA
+constexpr int kCap = kTile + kTopkMax;      // keys held in shared memory
+
+struct Shared {
+    uint64_t keys[kCap];
+    uint32_t hist[256];
+    int cnt;
+    int digit, above;     // the selection's current digit, keys above it
+    float thr;
+};
+
+template <typename T>
+__device__ __forceinline__ float score_of(T v);
+template <>
+__device__ __forceinline__ float score_of<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float score_of<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float score_of<__half>(__half v) { return __half2float(v); }
+
+__device__ __forceinline__ uint64_t key_of(float s, uint32_t col) {
+    const uint32_t u = __float_as_uint(s + 0.f);      // one zero
+    return (uint64_t)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << 32 | (uint32_t)~col;
+}
+__device__ __forceinline__ float score_of_key(uint64_t k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+
+// Cuts sh.keys[0..cnt) to its k largest (any order); all threads call it, cnt > k, keys distinct.
+// Leaves the k-th largest's score in sh.thr and k in sh.cnt.
+__device__ void select_k(Shared& sh, int k) {
+    const int tid = threadIdx.x, cnt = sh.cnt;
+    uint64_t prefix = 0;          // digits of the k-th largest key found so far
+    int want = k;                 // it is the want-th largest of the keys that share them
+    int shift = 56;
+    for (;; shift -= 8) {
+        if (tid < 256) sh.hist[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < cnt; i += kThreads) {
+            const uint64_t key = sh.keys[i];
+            if (shift == 56 || (key >> (shift + 8)) == prefix) atomicAdd(&sh.hist[(key >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        if (tid < 32) {           // lane l: digits 255 - 8 l .. 248 - 8 l, from the top
+            uint32_t c[8], s = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += c[i] = sh.hist[255 - 8 * tid - i];
+            uint32_t before = s;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
+                if (tid >= o) before += x;
+            }
+            before -= s;          // keys with a digit above this lane's
+            if (before < (uint32_t)want && before + s >= (uint32_t)want) {
+                int i = 0;
+#pragma unroll
+                for (int j = 0; j < 7; ++j)
+                    if (i == j && before + c[j] < (uint32_t)want) {
+                        before += c[j];
+                        i = j + 1;
+                    }
+                sh.digit = 255 - 8 * tid - i;
+                sh.above = (int)before;
+            }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | (uint64_t)sh.digit;
+        want -= sh.above;
+        const bool whole = sh.hist[sh.digit] == (uint32_t)want;   // the digit's keys are all wanted
+        __syncthreads();
+        if (whole || shift == 0) break;
+    }
+    // keys whose leading digits are >= prefix are exactly the k largest
+    constexpr int kPer = (kCap + kThreads - 1) / kThreads;
+    uint64_t mine[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mine[i] = i * kThreads + tid < cnt ? sh.keys[i * kThreads + tid] : 0;
+    if (tid == 0) {
+        sh.cnt = 0;
+        sh.thr = CUDART_INF_F;
+    }
+    __syncthreads();
+    uint32_t least = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (mine[i] != 0 && (mine[i] >> shift) >= prefix) {
+            sh.keys[atomicAdd(&sh.cnt, 1)] = mine[i];
+            least = min(least, (uint32_t)(mine[i] >> 32));
+        }
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (tid < 256) sh.hist[tid] = 0xffffffffu;
+    __syncthreads();
+    if ((tid & 31) == 0) sh.hist[tid >> 5] = least;
+    __syncthreads();
+    if (tid < 32) {
+        least = __reduce_min_sync(0xffffffffu, sh.hist[tid]);
+        if (tid == 0) sh.thr = score_of_key((uint64_t)least << 32);
+    }
+    __syncthreads();
+}
+
+// Writes the row's result from sh.keys[0..cnt), cnt <= k: bitonic sort, descending.
+__device__ void finish_row(Shared& sh, int q, const TopkArgs& a) {
+    const int tid = threadIdx.x, cnt = sh.cnt;
+    int n2 = 32;
+    while (n2 < cnt) n2 <<= 1;
+    for (int i = cnt + tid; i < n2; i += kThreads) sh.keys[i] = 0;
+    __syncthreads();
+    for (int w = 2; w <= n2; w <<= 1)
+        for (int j = w >> 1; j > 0; j >>= 1) {
+            for (int i = tid; i < n2; i += kThreads) {
+                const int p = i ^ j;
+                if (p > i) {
+                    const uint64_t x = sh.keys[i], y = sh.keys[p];
+                    if ((x < y) == ((i & w) == 0)) {
+                        sh.keys[i] = y;
+                        sh.keys[p] = x;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    for (int i = tid; i < a.k; i += kThreads) {
+        const bool there = i < cnt;
+        const uint64_t key = there ? sh.keys[i] : 0;
+        a.ids_out[(size_t)q * a.k + i] = there ? (int32_t)~(uint32_t)key + a.id_base : -1;
+        a.scores_out[(size_t)q * a.k + i] = there ? score_of_key(key) : -3.402823466e+38f;
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared& sh = *reinterpret_cast<Shared*>(smem);
+    const int tid = threadIdx.x;
+    const int q = blockIdx.x / splits, part = blockIdx.x % splits;
+    const int64_t c0 = part * slice;
+    const int64_t c1 = c0 + slice < a.n ? c0 + slice : a.n;
+    const T* row = static_cast<const T*>(a.in) + (size_t)q * a.ld;
+    if (tid == 0) {
+        sh.cnt = 0;
+        sh.thr = -CUDART_INF_F;
+    }
+    __syncthreads();
+    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    constexpr int U = kTile / (kThreads * V);
+    for (int64_t t0 = c0; t0 < c1; t0 += kTile) {
+        const float thr = sh.thr;
+        alignas(16) T v[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t j = t0 + (u * kThreads + tid) * V;
+            if (VEC && j + V <= c1) {
+                *reinterpret_cast<uint4*>(v[u]) = *reinterpret_cast<const uint4*>(row + j);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (j + i < c1) v[u][i] = row[j + i];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t j = t0 + (u * kThreads + tid) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float s = score_of<T>(v[u][i]);
+                if (j + i < c1 && s > thr) sh.keys[atomicAdd(&sh.cnt, 1)] = key_of(s, (uint32_t)(j + i));
+            }
+        }
+        __syncthreads();
+        const int cnt = sh.cnt;
+        // a full buffer must be cut; the first cut gives the first threshold
+        if (cnt > a.k && (cnt > kCap - kTile || thr == -CUDART_INF_F)) select_k(sh, a.k);
+        else __syncthreads();
+    }
+    if (sh.cnt > a.k) select_k(sh, a.k);
+    __syncthreads();
+    if (splits == 1) {
+        finish_row(sh, q, a);
+    } else {
+        uint64_t* mine = a.ws + ((size_t)q * splits + part) * a.k;
+        for (int i = tid; i < a.k; i += kThreads) mine[i] = i < sh.cnt ? sh.keys[i] : 0;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) topk_join_kernel(const TopkArgs a, const int splits) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared& sh = *reinterpret_cast<Shared*>(smem);
+    const int tid = threadIdx.x, q = blockIdx.x;
+    const int total = splits * a.k;
+    const uint64_t* keys = a.ws + (size_t)q * total;
+    if (tid == 0) sh.cnt = 0;
+    __syncthreads();
+    for (int t0 = 0; t0 < total; t0 += kTile) {
+        for (int i = t0 + tid; i < min(total, t0 + kTile); i += kThreads) {
+            const uint64_t key = keys[i];
+            if (key != 0) sh.keys[atomicAdd(&sh.cnt, 1)] = key;
+        }
+        __syncthreads();
+        const int cnt = sh.cnt;
+        __syncthreads();
+        if (cnt > a.k) select_k(sh, a.k);
+    }
+    finish_row(sh, q, a);
+}
+
+int topk_splits(int Q, int64_t n, int k, int sm_count) {
+    const int64_t want = Q > 0 ? (int64_t)sm_count * 3 / Q : 1;
+    const int64_t least = k > 512 ? 32 * (int64_t)k : 16384;     // a slice is worth its own selection
+    int64_t s = n / least;
+    if (s > want) s = want;
+    return s < 1 ? 1 : (int)s;
+}
+
+template <typename T>
+cudaError_t launch_topk_t(const TopkArgs& a, int splits, cudaStream_t stream) {
+    const bool vec = ((uintptr_t)a.in | (uintptr_t)(a.ld * sizeof(T))) % 16 == 0;
+    auto kernel = vec ? topk_scan_kernel<T, true> : topk_scan_kernel<T, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+    if (e != cudaSuccess) return e;
+    // slices start at multiples of 8 scores, so 16-byte loads stay aligned
+    const int64_t slice = ((a.n + splits - 1) / splits + 7) / 8 * 8;
+    kernel<<<(unsigned)((int64_t)a.Q * splits), kThreads, sizeof(Shared), stream>>>(a, splits, slice);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+int64_t topk_workspace_bytes(int Q, int64_t n, int k, int sm_count) {
+    const int s = topk_splits(Q, n, k, sm_count);
+    return s == 1 ? 0 : (int64_t)Q * s * k * 8;
+}
+
+cudaError_t launch_topk(const TopkArgs& a, int sm_count, cudaStream_t stream, int* launches) {
+    const int splits = topk_splits(a.Q, a.n, a.k, sm_count);
+    cudaError_t e = a.type == kTypeF32    ? launch_topk_t<float>(a, splits, stream)
+                    : a.type == kTypeBf16 ? launch_topk_t<__nv_bfloat16>(a, splits, stream)
+                                          : launch_topk_t<__half>(a, splits, stream);
+    *launches = 1;
+    if (e != cudaSuccess || splits == 1) return e;
+    e = cudaFuncSetAttribute(topk_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+    if (e != cudaSuccess) return e;
+    topk_join_kernel<<<a.Q, kThreads, sizeof(Shared), stream>>>(a, splits);
+    *launches = 2;
+    return cudaGetLastError();
+}
+
+}  // namespace coral

@@ -394,6 +394,74 @@ int coral_search_static(int device, void* stream, const float* d_vecs, const int
  * `device`; -1 for a device index out of range.  No counterpart in the reference. */
 int coral_search_static_status(int device);
 
+/* ---- operators on score rows (no counterpart in the reference, which scores one graph neighbour at
+ * a time in fp32) ----
+ *
+ * A dense pass over a compressed base under per-query rules: rows are compressed once
+ * (coral_fp8_quantize), a batch of queries at its arrival, coral_fp8_scores forms every score on the
+ * tensor cores, coral_adjust_scores applies the rules and coral_topk_scores chooses.  Chunks or
+ * shards of the base meet in coral_merge_shards (id_base makes ids global).
+ *
+ * All five take device pointers of the handle's GPU (checked; CORAL_ERR_ARG else), need no vectors in
+ * the handle, keep no state between calls, enqueue on `stream` (NULL = the handle's stream) without
+ * synchronising and leave the caller's current device as it was.  They allocate nothing, so they can
+ * be captured into a graph; a workspace belongs to one call at a time.  Empty sizes are allowed and
+ * launch nothing (coral_topk_scores still writes its padding). */
+
+/* element types */
+#define CORAL_F32 0
+#define CORAL_BF16 1
+#define CORAL_F16 2
+
+/* Layout of compressed rows: codes e4m3, row r at r * coral_fp8_code_pitch(dim) bytes (dim rounded up
+ * to 16); scales e8m0, the scale of columns [128 b, 128 b + 128) of row r at byte
+ * r * coral_fp8_scale_pitch(dim) + b (a multiple of 4 that holds all blocks); padding bytes are zero.
+ * value = e4m3(code) * 2^(scale - 127).  0 for dim outside [1, 65536]. */
+int64_t coral_fp8_code_pitch(int dim);
+int64_t coral_fp8_scale_pitch(int dim);
+
+/* Compresses `rows` rows of `dim` values of `type`, `ld` >= dim elements apart.  A block's exponent is
+ * the least e in [-127, 127] with max|x| <= 448 * 2^e; values are rounded to nearest even.  NaN and
+ * infinities do not count in the maximum and become NaN codes (e4m3 has no infinity).  d_codes:
+ * 16-byte aligned, d_scales: 4-byte aligned. */
+int coral_fp8_quantize(coral_index_t* h, const void* d_x, int type, int64_t rows, int dim, int64_t ld,
+                       uint8_t* d_codes, uint8_t* d_scales, void* stream);
+
+/* d_out[q * ld + j] = alpha * <query q, row j> + d_bias[j] (d_bias may be NULL) in `type`, for Q query
+ * rows and n base rows of the layout above, accumulated in fp32 and rounded once.  Squared distance:
+ * alpha = 2 (or 1) and d_bias = -|row|^2 (or half of it) order as -|q - row|^2.  Code pointers are
+ * 16-byte aligned, scale pointers 4-byte; n < 2^31.  A NaN code makes its row's scores NaN. */
+int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* d_q_scales, int Q,
+                     const uint8_t* d_codes, const uint8_t* d_scales, int64_t n, int dim, float alpha,
+                     const float* d_bias, void* d_out, int type, int64_t ld, void* stream);
+
+/* Rules on Q score rows of n columns, in fp32, rounded once.  With c = how often j stands in row q of
+ * d_seen ([Q][n_seen], entries outside [0, n) are padding) and (rho, phi, pi) = d_penalties[q]
+ * ([Q][3], rho > 0):  c > 0: s = (s > 0 ? s / rho : s * rho) - phi * c - pi.  Then s += every
+ * d_bias[q][i] with d_bias_ids[q][i] = j, in list order ([Q][n_bias], n_bias <= 1024, ids outside
+ * [0, n) are padding).  Then s = -inf where bit j % 32 of word j / 32 of row q of d_excluded is set
+ * (the bitset of coral_index_set_deleted; rows ld_excluded words apart, 0 = one row for all).  Each
+ * list may be absent (NULL and n_seen / n_bias 0; d_penalties goes with d_seen).  d_out may be
+ * d_scores with the same ld; any other overlap is refused. */
+int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q, int64_t n, int64_t ld,
+                        const int32_t* d_seen, int n_seen, const float* d_penalties, const int32_t* d_bias_ids,
+                        const float* d_bias, int n_bias, const uint32_t* d_excluded, int64_t ld_excluded,
+                        void* d_out, int64_t ld_out, void* stream);
+
+/* The k (<= 1024) largest of every score row, best first, equal scores by the lower column:
+ * d_ids_out[q][i] = column + id_base and d_scores_out[q][i] (fp32, exact).  -inf and NaN are never
+ * chosen; a row that runs out ends in id -1, score -3.402823466e+38 (what coral_search pads with for
+ * CORAL_IP).  id_base >= 0, id_base + n <= 2^31 - 1.  d_workspace: coral_topk_workspace bytes (may be
+ * 0), 8-byte aligned. */
+int coral_topk_workspace(coral_index_t* h, int Q, int64_t n, int k, int64_t* bytes_out);
+int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, int64_t n, int64_t ld, int k,
+                      int32_t id_base, int32_t* d_ids_out, float* d_scores_out, void* d_workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* After the stream has been synchronised: CORAL_ERR_KERNEL if a bounded wait of coral_fp8_scores ran
+ * out since the last check (its scores are invalid), else CORAL_OK. */
+int coral_scores_check(coral_index_t* h);
+
 /* Last error text of the handle (or of handle creation when h is NULL). */
 const char* coral_last_error(coral_index_t* h);
 
