@@ -4,13 +4,16 @@
 // so keys are unique and a larger key is better.  -inf (an excluded row) and NaN never become a key;
 // a row with fewer than k keys ends in padding (id -1).
 //
-// A CTA streams one slice of one row: every tile's scores are compared with the slice's threshold,
-// the k-th best score seen so far, and what beats it is appended to a buffer in shared memory that
-// always has room for one more tile.  Columns arrive in ascending order, so a score equal to the
-// threshold has a higher id than the k keys it would have to beat and loses.  When the buffer could
-// overflow, a radix selection (8-bit digits, from the top) cuts it to its k best and tightens the
-// threshold.  Rows are cut into slices while there are fewer rows than CTAs to keep busy; the k best
-// of each slice then meet in a second launch, which selects among keys in the same way.
+// A CTA streams one slice of one row, a tile of scores in registers at a time (the next tile's loads
+// are in flight meanwhile).  What reaches the slice's threshold is appended to a buffer in shared
+// memory that always has room for one more tile.  The first threshold comes from the first tile
+// itself: the k-th largest of its vectors' maxima, rounded down to 16 bits, is a lower bound of the
+// k-th best score and lets little more than k scores pass.  When the buffer could overflow, a radix
+// selection (8-bit digits, from the top) cuts it to its k best and the threshold becomes the value
+// just above the k-th: columns arrive in ascending order, so a score equal to the k-th has a higher
+// id than the k keys it would have to beat and loses.  Rows are cut into slices while there are fewer
+// rows than CTAs to keep busy; the k best of each slice then meet in a second launch, which selects
+// among keys in the same way.
 #include <math_constants.h>
 
 #include "scores.cuh"
@@ -28,7 +31,7 @@ struct Shared {
     uint32_t hist[256];
     int cnt;
     int digit, above;     // the selection's current digit, keys above it
-    float thr;
+    float least;          // scores below it cannot be among the k best
 };
 
 template <typename T>
@@ -40,17 +43,53 @@ __device__ __forceinline__ float score_of<__nv_bfloat16>(__nv_bfloat16 v) { retu
 template <>
 __device__ __forceinline__ float score_of<__half>(__half v) { return __half2float(v); }
 
-__device__ __forceinline__ uint64_t key_of(float s, uint32_t col) {
+__device__ __forceinline__ uint32_t ord_of(float s) {
     const uint32_t u = __float_as_uint(s + 0.f);      // one zero
-    return (uint64_t)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << 32 | (uint32_t)~col;
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float score_of_key(uint64_t k) {
-    const uint32_t o = (uint32_t)(k >> 32);
-    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+__device__ __forceinline__ float of_ord(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
+__device__ __forceinline__ float score_of_key(uint64_t k) { return of_ord((uint32_t)(k >> 32)); }
+
+__device__ __forceinline__ uint64_t key_of(float s, uint32_t col) { return (uint64_t)ord_of(s) << 32 | (uint32_t)~col; }
+
+// One step of a radix selection: warp 0 finds, from the histogram of a digit, the digit that holds
+// the want-th largest key (sh.digit) and how many keys lie above it (sh.above).
+__device__ __forceinline__ void pick_digit(Shared& sh, int want) {
+    const int lane = threadIdx.x;     // lane l: digits 255 - 8 l .. 248 - 8 l, from the top
+    uint32_t c[8], s = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += c[i] = sh.hist[255 - 8 * lane - i];
+    uint32_t before = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+    }
+    before -= s;          // keys with a digit above this lane's
+    if (before < (uint32_t)want && before + s >= (uint32_t)want) {
+        int i = 0;
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+            if (i == j && before + c[j] < (uint32_t)want) {
+                before += c[j];
+                i = j + 1;
+            }
+        sh.digit = 255 - 8 * lane - i;
+        sh.above = (int)before;
+    }
 }
 
+template <typename T>
+__device__ __forceinline__ T lowest_of();      // -inf
+template <>
+__device__ __forceinline__ float lowest_of<float>() { return -CUDART_INF_F; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 lowest_of<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+template <>
+__device__ __forceinline__ __half lowest_of<__half>() { return __ushort_as_half(0xfc00); }
+
 // Cuts sh.keys[0..cnt) to its k largest (any order); all threads call it, cnt > k, keys distinct.
-// Leaves the k-th largest's score in sh.thr and k in sh.cnt.
+// Leaves k in sh.cnt and, in sh.least, the value just above the k-th largest's score.
 __device__ void select_k(Shared& sh, int k) {
     const int tid = threadIdx.x, cnt = sh.cnt;
     uint64_t prefix = 0;          // digits of the k-th largest key found so far
@@ -64,29 +103,7 @@ __device__ void select_k(Shared& sh, int k) {
             if (shift == 56 || (key >> (shift + 8)) == prefix) atomicAdd(&sh.hist[(key >> shift) & 255], 1u);
         }
         __syncthreads();
-        if (tid < 32) {           // lane l: digits 255 - 8 l .. 248 - 8 l, from the top
-            uint32_t c[8], s = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s += c[i] = sh.hist[255 - 8 * tid - i];
-            uint32_t before = s;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
-                if (tid >= o) before += x;
-            }
-            before -= s;          // keys with a digit above this lane's
-            if (before < (uint32_t)want && before + s >= (uint32_t)want) {
-                int i = 0;
-#pragma unroll
-                for (int j = 0; j < 7; ++j)
-                    if (i == j && before + c[j] < (uint32_t)want) {
-                        before += c[j];
-                        i = j + 1;
-                    }
-                sh.digit = 255 - 8 * tid - i;
-                sh.above = (int)before;
-            }
-        }
+        if (tid < 32) pick_digit(sh, want);
         __syncthreads();
         prefix = prefix << 8 | (uint64_t)sh.digit;
         want -= sh.above;
@@ -99,10 +116,7 @@ __device__ void select_k(Shared& sh, int k) {
     uint64_t mine[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) mine[i] = i * kThreads + tid < cnt ? sh.keys[i * kThreads + tid] : 0;
-    if (tid == 0) {
-        sh.cnt = 0;
-        sh.thr = CUDART_INF_F;
-    }
+    if (tid == 0) sh.cnt = 0;
     __syncthreads();
     uint32_t least = 0xffffffffu;
 #pragma unroll
@@ -118,7 +132,7 @@ __device__ void select_k(Shared& sh, int k) {
     __syncthreads();
     if (tid < 32) {
         least = __reduce_min_sync(0xffffffffu, sh.hist[tid]);
-        if (tid == 0) sh.thr = score_of_key((uint64_t)least << 32);
+        if (tid == 0) sh.least = of_ord(least + 1u);      // above +inf: NaN, which nothing reaches
     }
     __syncthreads();
 }
@@ -152,8 +166,74 @@ __device__ void finish_row(Shared& sh, int q, const TopkArgs& a) {
     }
 }
 
+// One tile in registers: U vectors of V scores a thread, vector u at column t0 + (u * kThreads + tid) * V.
+// What lies past the slice's end reads -inf.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice) {
+struct Tile {
+    static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    static constexpr int U = kTile / (kThreads * V);
+    alignas(16) T v[U][V];
+
+    __device__ __forceinline__ void load(const T* row, int64_t t0, int64_t c1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t j = t0 + (u * kThreads + threadIdx.x) * V;
+            if (VEC && j + V <= c1) {
+                *reinterpret_cast<uint4*>(v[u]) = *reinterpret_cast<const uint4*>(row + j);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[u][i] = j + i < c1 ? row[j + i] : lowest_of<T>();
+            }
+        }
+    }
+    __device__ __forceinline__ float best(int u) const {     // NaN counts as nothing
+        float m = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = fmaxf(m, score_of<T>(v[u][i]));
+        return m;
+    }
+};
+
+// A lower bound of the k-th best score of the slice from its first tile (all of it inside the slice):
+// the k-th largest of the tile's maxima -- of threads, or of vectors where there are too few threads --
+// with the low 16 bits of its order cleared.  Two 8-bit digits of a radix selection.
+template <typename T, bool VEC>
+__device__ void first_threshold(Shared& sh, const Tile<T, VEC>& t, int k) {
+    constexpr int U = Tile<T, VEC>::U;
+    const int tid = threadIdx.x;
+    uint32_t o[U], top = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        o[u] = ord_of(t.best(u)) >> 16;
+        top = max(top, o[u]);
+    }
+    const bool by_thread = k <= kThreads / 2;
+    int want = k;
+    uint32_t prefix = 0;
+    for (int shift = 8; shift >= 0; shift -= 8) {
+        if (tid < 256) sh.hist[tid] = 0;
+        __syncthreads();
+        if (by_thread) {
+            if (shift == 8 || top >> 8 == prefix) atomicAdd(&sh.hist[(top >> shift) & 255], 1u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (shift == 8 || o[u] >> 8 == prefix) atomicAdd(&sh.hist[(o[u] >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        if (tid < 32) pick_digit(sh, want);
+        __syncthreads();
+        prefix = prefix << 8 | (uint32_t)sh.digit;
+        want -= sh.above;
+        __syncthreads();
+    }
+    // never below the lowest finite score: -inf is not chosen
+    if (tid == 0) sh.least = prefix <= ord_of(-3.402823466e+38f) >> 16 ? -3.402823466e+38f : of_ord(prefix << 16);
+    __syncthreads();
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem);
     const int tid = threadIdx.x;
@@ -161,41 +241,33 @@ __global__ void __launch_bounds__(kThreads) topk_scan_kernel(const TopkArgs a, c
     const int64_t c0 = part * slice;
     const int64_t c1 = c0 + slice < a.n ? c0 + slice : a.n;
     const T* row = static_cast<const T*>(a.in) + (size_t)q * a.ld;
+    using Scores = Tile<T, VEC>;
+    Scores cur, next;
+    if (c0 < c1) cur.load(row, c0, c1);
     if (tid == 0) {
         sh.cnt = 0;
-        sh.thr = -CUDART_INF_F;
+        sh.least = -3.402823466e+38f;
     }
     __syncthreads();
-    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-    constexpr int U = kTile / (kThreads * V);
     for (int64_t t0 = c0; t0 < c1; t0 += kTile) {
-        const float thr = sh.thr;
-        alignas(16) T v[U][V];
+        if (t0 + kTile < c1) next.load(row, t0 + kTile, c1);
+        if (t0 == c0 && c1 - c0 >= kTile) first_threshold(sh, cur, a.k);
+        const float least = sh.least;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t j = t0 + (u * kThreads + tid) * V;
-            if (VEC && j + V <= c1) {
-                *reinterpret_cast<uint4*>(v[u]) = *reinterpret_cast<const uint4*>(row + j);
-            } else {
+        for (int u = 0; u < Scores::U; ++u)
+            if (cur.best(u) >= least) {
+                const int64_t j = t0 + (u * kThreads + tid) * Scores::V;
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (j + i < c1) v[u][i] = row[j + i];
+                for (int i = 0; i < Scores::V; ++i) {
+                    const float s = score_of<T>(cur.v[u][i]);
+                    if (s >= least) sh.keys[atomicAdd(&sh.cnt, 1)] = key_of(s, (uint32_t)(j + i));
+                }
             }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t j = t0 + (u * kThreads + tid) * V;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float s = score_of<T>(v[u][i]);
-                if (j + i < c1 && s > thr) sh.keys[atomicAdd(&sh.cnt, 1)] = key_of(s, (uint32_t)(j + i));
-            }
-        }
         __syncthreads();
         const int cnt = sh.cnt;
-        // a full buffer must be cut; the first cut gives the first threshold
-        if (cnt > a.k && (cnt > kCap - kTile || thr == -CUDART_INF_F)) select_k(sh, a.k);
+        if (cnt > kCap - kTile && cnt > a.k) select_k(sh, a.k);     // no room for another tile
         else __syncthreads();
+        cur = next;
     }
     if (sh.cnt > a.k) select_k(sh, a.k);
     __syncthreads();
