@@ -1589,7 +1589,7 @@ int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q,
     ARG(ld >= n && ld < (1ll << 31) && ld_out >= n && ld_out < (1ll << 31), "ld and ld_out must be in [n, 2^31)");
     ARG(n_seen >= 0 && n_bias >= 0, "negative list length");
     if (n_bias > coral::kRulesMaxBias) return fail(h, CORAL_ERR_LIMIT, "n_bias must not exceed 1024");
-    if ((n + 8191) / 8192 * Q > 0x7fffffffll) return fail(h, CORAL_ERR_LIMIT, "too many score rows for one call");
+    if ((n + 4095) / 4096 * Q > 0x7fffffffll) return fail(h, CORAL_ERR_LIMIT, "too many score rows for one call");
     if (Q == 0 || n == 0) return CORAL_OK;
     ARG(d_scores && d_out && (n_seen == 0 || (d_seen && d_penalties)) && (n_bias == 0 || (d_bias_ids && d_bias)),
         "null argument");

@@ -5,10 +5,12 @@
 //     excluded: s <- -inf
 // in fp32, rounded once to the output's type.
 //
-// A CTA owns kCols columns of one row.  It turns the row's two id lists into tables over its own
-// columns in shared memory (integer counts, so the order of the atomics does not show; a bias is
-// summed by the thread that holds the id's first entry), then streams its columns with 16-byte
-// accesses.  No table in global memory, nothing to clear between calls, no second launch.
+// A CTA owns kCols columns of one row.  Its own scores and mask words are requested first and stay in
+// flight while it turns the row's two id lists into tables over its columns in shared memory: counts
+// by integer atomics (their order does not show), biases by one warp in list order.  Then it applies
+// the rules and stores.  No table in global memory, nothing to clear between calls, one launch.  The
+// history is read once per CTA, from L2: wider columns would read it less often but leave fewer CTAs
+// an SM, and latency, not that traffic, is what a CTA waits for.
 #include <math_constants.h>
 
 #include "scores.cuh"
@@ -18,7 +20,7 @@ namespace coral {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCols = 8192;
+constexpr int kCols = 4096;
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -39,52 +41,84 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a, const int chunks) {
-    extern __shared__ unsigned char smem[];
+    extern __shared__ __align__(16) unsigned char smem[];
     const int q = blockIdx.x / chunks;
     const int64_t c0 = (int64_t)(blockIdx.x % chunks) * kCols;
     const int cols = (int)(a.n - c0 < kCols ? a.n - c0 : kCols);
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31;
     const bool has_seen = a.n_seen > 0, has_bias = a.n_bias > 0;
     uint32_t* count = reinterpret_cast<uint32_t*>(smem);
     float* bias = reinterpret_cast<float*>(smem) + (has_seen ? kCols : 0);
-    float rho = 1.f, phi = 0.f, pi = 0.f;
-    if (has_seen) {
-        rho = a.penalties[(size_t)q * 3];
-        phi = a.penalties[(size_t)q * 3 + 1];
-        pi = a.penalties[(size_t)q * 3 + 2];
-        for (int i = tid; i < kCols; i += kThreads) count[i] = 0u;
-    }
-    if (has_bias)
-        for (int i = tid; i < kCols; i += kThreads) bias[i] = 0.f;
-    if (has_seen || has_bias) __syncthreads();
-    if (has_seen) {
-        const int32_t* seen = a.seen + (size_t)q * a.n_seen;
-        for (int i = tid; i < a.n_seen; i += kThreads) {
-            const int64_t j = (int64_t)seen[i] - c0;
-            if (j >= 0 && j < cols) atomicAdd(&count[j], 1u);
-        }
-    }
-    if (has_bias) {
-        const int32_t* ids = a.bias_ids + (size_t)q * a.n_bias;
-        const float* vals = a.bias + (size_t)q * a.n_bias;
-        for (int i = tid; i < a.n_bias; i += kThreads) {
-            const int32_t id = ids[i];
-            const int64_t j = (int64_t)id - c0;
-            if (j < 0 || j >= cols) continue;
-            bool first = true;
-            for (int p = 0; p < i && first; ++p) first = ids[p] != id;
-            if (!first) continue;
-            float s = vals[i];
-            for (int p = i + 1; p < a.n_bias; ++p)
-                if (ids[p] == id) s += vals[p];
-            bias[j] = s;
-        }
-    }
-    if (has_seen || has_bias) __syncthreads();
 
+    // the thread's scores: U vectors of V, vector u at column (u * kThreads + tid) * V
+    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    constexpr int U = kCols / (kThreads * V);
+    constexpr uint32_t kAll = (1u << V) - 1u;
     const T* in = static_cast<const T*>(a.in) + (size_t)q * a.ld + c0;
     T* out = static_cast<T*>(a.out) + (size_t)q * a.ld_out + c0;
     const uint32_t* ex = a.excluded ? a.excluded + (size_t)q * a.ld_excluded + c0 / 32 : nullptr;
+    alignas(16) T v[U][V];
+    uint32_t m[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = (u * kThreads + tid) * V;
+        m[u] = ex && j < cols ? ex[j >> 5] >> (j & 31) & kAll : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = (u * kThreads + tid) * V;
+        if (m[u] != kAll) {      // what is excluded altogether is not read
+            if (VEC && j + V <= cols) {
+                *reinterpret_cast<uint4*>(v[u]) = *reinterpret_cast<const uint4*>(in + j);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (j + i < cols) v[u][i] = in[j + i];
+            }
+        }
+    }
+
+    float rho = 1.f, phi = 0.f, pi = 0.f;
+    if (has_seen || has_bias) {
+        if (has_seen) {
+            rho = a.penalties[(size_t)q * 3];
+            phi = a.penalties[(size_t)q * 3 + 1];
+            pi = a.penalties[(size_t)q * 3 + 2];
+        }
+        const int words = kCols * ((has_seen ? 1 : 0) + (has_bias ? 1 : 0));
+        for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        if (has_seen) {
+            const int32_t* seen = a.seen + (size_t)q * a.n_seen;
+#pragma unroll 4
+            for (int i = tid; i < a.n_seen; i += kThreads) {
+                const int64_t j = (int64_t)seen[i] - c0;
+                if (j >= 0 && j < cols) atomicAdd(&count[j], 1u);
+            }
+        }
+        if (has_bias && tid < 32) {
+            const int32_t* ids = a.bias_ids + (size_t)q * a.n_bias;
+            const float* vals = a.bias + (size_t)q * a.n_bias;
+            for (int i0 = 0; i0 < a.n_bias; i0 += 32) {
+                const int i = i0 + lane;
+                const int64_t j = i < a.n_bias ? (int64_t)ids[i] - c0 : -1;
+                const bool mine = j >= 0 && j < cols;
+                const float val = mine ? vals[i] : 0.f;
+                // entries of one id: its first lane sums them, in list order, onto what earlier ones left
+                const uint32_t same = __match_any_sync(0xffffffffu, mine ? (int)j : -1 - lane);
+                const bool leads = mine && (same & ((1u << lane) - 1u)) == 0u;
+                float s = leads ? bias[j] : 0.f;
+                for (uint32_t p = 0; p < 32; ++p) {
+                    const float x = __shfl_sync(0xffffffffu, val, p);
+                    if (same >> p & 1u) s += x;
+                }
+                if (leads) bias[j] = s;
+                __syncwarp();
+            }
+        }
+        __syncthreads();
+    }
+
     auto rule = [&](float s, int j, bool out_of) {
         if (has_seen) {
             const uint32_t c = count[j];
@@ -93,26 +127,25 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
                 s = s - phi * (float)c - pi;
             }
         }
-        if (has_bias) s += bias[j];
+        if (has_bias) {
+            const float b = bias[j];
+            if (b != 0.f) s += b;
+        }
         return from_f32<T>(out_of ? -CUDART_INF_F : s);
     };
-    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-    int j0 = tid * V;
-    if (VEC) {
-        for (; j0 + V <= cols; j0 += kThreads * V) {
-            const uint32_t m = ex ? (ex[j0 >> 5] >> (j0 & 31)) & ((1u << V) - 1u) : 0u;
-            alignas(16) T v[V];
-            // a fully excluded vector is not read
-            if (m != (1u << V) - 1u) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(in + j0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = rule(to_f32<T>(v[i]), j0 + i, (m >> i) & 1u);
-            *reinterpret_cast<uint4*>(out + j0) = *reinterpret_cast<uint4*>(v);
+    for (int u = 0; u < U; ++u) {
+        const int j = (u * kThreads + tid) * V;
+        if (VEC && j + V <= cols) {
+            alignas(16) T w[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = rule(to_f32<T>(v[u][i]), j + i, m[u] >> i & 1u);
+            *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<uint4*>(w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (j + i < cols) out[j + i] = rule(to_f32<T>(v[u][i]), j + i, m[u] >> i & 1u);
         }
-        j0 = cols / V * V + tid;    // the ragged end, element by element
-    }
-    for (; j0 < cols; j0 += kThreads) {
-        const bool m = ex && ((ex[j0 >> 5] >> (j0 & 31)) & 1u);
-        out[j0] = rule(m ? 0.f : to_f32<T>(in[j0]), j0, m);
     }
 }
 
@@ -123,10 +156,6 @@ cudaError_t launch_rules(const RulesArgs& a, cudaStream_t stream) {
     const bool vec = ((uintptr_t)a.in | (uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T)) |
                       (uintptr_t)(a.ld_out * sizeof(T))) % 16 == 0;
     auto kernel = vec ? score_rules_kernel<T, true> : score_rules_kernel<T, false>;
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
     kernel<<<(unsigned)(chunks * a.Q), kThreads, smem, stream>>>(a, (int)chunks);
     return cudaGetLastError();
 }
