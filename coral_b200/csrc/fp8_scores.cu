@@ -55,68 +55,88 @@ __device__ __forceinline__ float wide<__nv_bfloat16>(__nv_bfloat16 v) { return _
 template <>
 __device__ __forceinline__ float wide<__half>(__half v) { return __half2float(v); }
 
+#ifndef QSTEPS
+#define QSTEPS 4
+#endif
 constexpr int kQuantThreads = 256;
-constexpr int kQuantBlocks = 4;   // blocks of 128 columns a warp has in flight
+constexpr int kQuantSteps = QSTEPS;    // 16-byte loads a lane has in flight
 
-// One warp takes kQuantBlocks consecutive blocks, lane l the columns 4 l .. 4 l + 3 of each: a block
-// of fp32 is one coalesced 512-byte read, and its maximum one warp reduction over the magnitudes'
-// bits.  Bound by memory.
+// A block of 128 columns belongs to G lanes that hold 16 bytes each (32 lanes of fp32, 16 of the 16-bit
+// types): one coalesced read, and its maximum one reduction over the magnitudes' bits.  A warp takes
+// kQuantSteps * 32 / G consecutive blocks and writes their scales together.  Bound by memory.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads)
 fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, uint8_t* __restrict__ codes,
                     uint8_t* __restrict__ scales) {
-    const int lane = threadIdx.x & 31;
+    constexpr int E = 16 / (int)sizeof(T), G = kFp8Block / E, P = 32 / G, N = kQuantSteps * P;
+    const int lane = threadIdx.x & 31, in_block = lane % G, g = lane / G;
+    const uint32_t members = G == 32 ? 0xffffffffu : 0xffffu << (g * G);
     const int per_row = (dim + kFp8Block - 1) / kFp8Block;
     const int code_pitch = (dim + 15) / 16 * 16, scale_pitch = (dim + 511) / 512 * 4;
     const int64_t total = rows * per_row;
-    const int64_t first = ((int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5)) * kQuantBlocks;
+    const int64_t first = ((int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5)) * N;
     if (first >= total) return;
-    int64_t row = total <= 0x7fffffff ? (int64_t)((uint32_t)first / (uint32_t)per_row) : first / per_row;
-    int b = (int)(first - row * per_row);
-    float v[kQuantBlocks][4];
-    int64_t r[kQuantBlocks];
-    int bb[kQuantBlocks];
+    const int64_t row0 = total <= 0x7fffffff ? (int64_t)((uint32_t)first / (uint32_t)per_row) : first / per_row;
+    const int b0 = (int)(first - row0 * per_row);
+    auto place = [&](int i, int64_t& row, int& b) {      // block first + i
+        row = row0;
+        b = b0 + i;
+        if (b >= per_row) {
+            const int over = b / per_row;
+            row += over;
+            b -= over * per_row;
+        }
+    };
+    alignas(16) T v[kQuantSteps][E];
+    int64_t row[kQuantSteps];
+    int b[kQuantSteps];
 #pragma unroll
-    for (int u = 0; u < kQuantBlocks; ++u) {
-        r[u] = row;
-        bb[u] = b;
-        const int c = b * kFp8Block + lane * 4;
-        const T* p = x + row * ld + c;
-        if (first + u < total) {
-            if (VEC && c + 4 <= dim) {
-                if (sizeof(T) == 4) {
-                    *reinterpret_cast<float4*>(v[u]) = __ldcs(reinterpret_cast<const float4*>(p));
-                } else {
-                    alignas(8) T t[4];
-                    *reinterpret_cast<uint2*>(t) = __ldcs(reinterpret_cast<const uint2*>(p));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[u][i] = wide<T>(t[i]);
-                }
+    for (int u = 0; u < kQuantSteps; ++u) {
+        place(u * P + g, row[u], b[u]);
+        const int c = b[u] * kFp8Block + in_block * E;
+        const T* p = x + row[u] * ld + c;
+        if (first + u * P + g < total) {
+            if (VEC && c + E <= dim) {
+                *reinterpret_cast<uint4*>(v[u]) = __ldcs(reinterpret_cast<const uint4*>(p));
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[u][i] = c + i < dim ? wide<T>(p[i]) : 0.f;
+                for (int i = 0; i < E; ++i) v[u][i] = c + i < dim ? p[i] : T(0.f);
             }
         }
-        if (++b == per_row) {
-            b = 0;
-            ++row;
-        }
     }
+    int mine = 0;      // the exponent of block first + lane
 #pragma unroll
-    for (int u = 0; u < kQuantBlocks; ++u) {
-        if (first + u >= total) break;
-        uint32_t m = max(max(abs_bits(v[u][0]), abs_bits(v[u][1])), max(abs_bits(v[u][2]), abs_bits(v[u][3])));
-        m = __reduce_max_sync(0xffffffffu, m);
+    for (int u = 0; u < kQuantSteps; ++u) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) m = max(m, abs_bits(wide<T>(v[u][i])));
+        m = __reduce_max_sync(members, m);
         const int e = scale_exponent(m);
         const float f = __uint_as_float((uint32_t)(127 - e) << 23);     // 2^-e: e in [-127, 120], 2^-e never subnormal
-        const int c = bb[u] * kFp8Block + lane * 4;
-        if (c < code_pitch)
-            *reinterpret_cast<uint32_t*>(codes + r[u] * code_pitch + c) =
-                pack_e4m3(scaled(v[u][0], f), scaled(v[u][1], f), scaled(v[u][2], f), scaled(v[u][3], f));
-        uint8_t* s = scales + r[u] * scale_pitch + bb[u];
-        if (lane == 0) *s = (uint8_t)(e + 127);
-        // the last block's warp zeroes the scales that pad the row to a multiple of four
-        if (lane > 0 && bb[u] == per_row - 1 && bb[u] + lane < scale_pitch) s[lane] = 0;
+        const int got = P == 1 ? e : __shfl_sync(0xffffffffu, e, lane % P * G);
+        if (lane / P == u) mine = got;
+        const int c = b[u] * kFp8Block + in_block * E;
+        if (first + u * P + g < total && c < code_pitch) {
+            uint32_t w[E / 4];
+#pragma unroll
+            for (int i = 0; i < E; i += 4)
+                w[i / 4] = pack_e4m3(scaled(wide<T>(v[u][i]), f), scaled(wide<T>(v[u][i + 1]), f),
+                                     scaled(wide<T>(v[u][i + 2]), f), scaled(wide<T>(v[u][i + 3]), f));
+            uint8_t* out = codes + row[u] * code_pitch + c;
+            if (E == 4)
+                *reinterpret_cast<uint32_t*>(out) = w[0];
+            else
+                *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[E / 4 - 1]);
+        }
+    }
+    if (lane < N && first + lane < total) {
+        int64_t r;
+        int bl;
+        place(lane, r, bl);
+        uint8_t* s = scales + r * scale_pitch + bl;
+        *s = (uint8_t)(mine + 127);
+        if (bl == per_row - 1)      // the scales that pad the row to a multiple of four
+            for (int i = 1; bl + i < scale_pitch; ++i) s[i] = 0;
     }
 }
 
@@ -124,9 +144,9 @@ template <typename T>
 cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t* codes, uint8_t* scales,
                        cudaStream_t stream) {
     const int64_t total = rows * ((dim + kFp8Block - 1) / kFp8Block);
-    const int per_cta = kQuantThreads / 32 * kQuantBlocks;
+    const int per_cta = kQuantThreads / 32 * kQuantSteps * (int)(sizeof(float) / sizeof(T));
     const int64_t ctas = (total + per_cta - 1) / per_cta;
-    const bool vec = ((uintptr_t)x | (uintptr_t)(ld * sizeof(T))) % (4 * sizeof(T)) == 0;
+    const bool vec = ((uintptr_t)x | (uintptr_t)(ld * sizeof(T))) % 16 == 0;
     auto kernel = vec ? fp8_quantize_kernel<T, true> : fp8_quantize_kernel<T, false>;
     kernel<<<(unsigned)ctas, kQuantThreads, 0, stream>>>(static_cast<const T*>(x), rows, dim, ld, codes, scales);
     return cudaGetLastError();
@@ -139,8 +159,11 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 //   warp 0     one lane issues the tiles' TMA loads (128-byte swizzle, 128 columns a stage);
 //   warp 1     one lane issues, per stage, three tcgen05.cp (the stage's scales to tensor memory)
 //              and four tcgen05.mma (M = 128, N = 256, K = 32);
-//   warp 2     brings the stage's scales to shared memory in the layout tcgen05.cp takes;
-//   warps 4-7  read the finished accumulator, apply alpha and bias, and store.
+//   warp 2     brings the stage's scales to shared memory in the layout tcgen05.cp takes, the words of
+//              the next four stages in flight;
+//   warps 4-7  read the finished accumulator, apply alpha and bias, and store: 64-byte pieces of 32
+//              rows through shared memory (64-byte swizzle) and TMA, two pieces in flight a warp, or,
+//              where the output's rows do not start at 16-byte boundaries, by coalesced plain stores.
 // A scale word of four bytes covers 512 columns; an instruction's K = 32 lies inside one block, so
 // all four instructions of a stage name the same byte of the word (the scale ids of the instruction
 // descriptor), byte (k-block mod 4).
@@ -155,9 +178,10 @@ constexpr int kABytes = kTileM * kTileK, kBBytes = kTileN * kTileK;
 constexpr int kScaleBytes = (kTileM + kTileN) * 4;
 constexpr int kAccStep = 192, kShared = 64, kTmemScales = 448;
 constexpr int kOffScales = kStages * (kABytes + kBBytes);
-constexpr int kOffStage = kOffScales + kStages * kScaleBytes;       // epilogue staging
-constexpr int kStagePitch = 33;
-constexpr int kOffBars = kOffStage + 4 * 32 * kStagePitch * 4;
+constexpr int kOffOut = kOffScales + kStages * kScaleBytes;         // 4 KB of output staging a warp
+constexpr int kOffBias = kOffOut + 4 * 4096;                        // the tile's biases, one copy a warp
+constexpr int kOffBars = kOffBias + 4 * kTileN * 4;
+static_assert(kOffOut % 1024 == 0, "swizzled staging");
 constexpr int kSmemBytes = kOffBars + 256 + 1024;
 constexpr int kThreads = 256;
 constexpr long long kWaitClocks = 4000000000ll;                     // ~2 s
@@ -205,6 +229,12 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
         ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar))
         : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, const void* src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0),
+                 "r"(c1), "r"(smem_u32(src))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 // Shared-memory matrix descriptor, K-major rows of 128 bytes with the 128-byte swizzle: 8-row groups
 // 1024 bytes apart, descriptor version 1, layout type 2.
@@ -262,9 +292,25 @@ template <>
 __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
 template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<float>(float lo, float) { return __float_as_uint(lo); }
+
+template <typename T, bool TMA_OUT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                  const Fp8ScoresArgs a, const int tiles_m, const int64_t tiles) {
+                  const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const int tiles_m,
+                  const int64_t tiles) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);   // [kStages] codes and scales landed
@@ -337,8 +383,8 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     scales_to_tmem(tb + 4, desc_rows16(sc + 1024));
                     const uint32_t id = (uint32_t)(kb & 3);
                     const uint32_t idesc = kInstrDesc | id << 29 | id << 4;
-#pragma unroll
-                    for (int j = 0; j < kTileK / 32; ++j)
+                    const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
+                    for (int j = 0; j < slices; ++j)
                         umma_mxf8(acc, desc_sw128(sa + j * 32), desc_sw128(sb + j * 32), idesc, ta, tb,
                                   (kb | j) != 0 ? 1u : 0u);
                     umma_commit(&empty[s]);
@@ -351,76 +397,134 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     } else if (warp == 2) {
-        // Scales: lane l keeps the words of rows l, l + 32, ... of both tiles for four k-blocks.
+        // Lane l keeps the scale words of rows l, l + 32, ... of both tiles for four k-blocks.
         int s = 0;
         uint32_t par = 0;
         bool ok = true;
-        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        uint32_t next[12];
+        auto fetch = [&](int64_t t, int kb) {
             const int64_t m0 = (t % tiles_m) * kTileM, n0 = (t / tiles_m) * kTileN;
-            uint32_t w[12];
-            for (int kb = 0; kb < k_blocks; ++kb) {
-                if ((kb & 3) == 0) {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int64_t r = m0 + g * 32 + lane;
-                        w[g] = r < a.Q ? *reinterpret_cast<const uint32_t*>(a.q_scales + r * scale_pitch + kb) : 0u;
-                    }
+            for (int g = 0; g < 4; ++g) {
+                const int64_t r = m0 + g * 32 + lane;
+                next[g] = r < a.Q ? *reinterpret_cast<const uint32_t*>(a.q_scales + r * scale_pitch + kb) : 0u;
+            }
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const int64_t r = n0 + g * 32 + lane;
-                        w[4 + g] = r < a.n ? *reinterpret_cast<const uint32_t*>(a.scales + r * scale_pitch + kb) : 0u;
+            for (int g = 0; g < 8; ++g) {
+                const int64_t r = n0 + g * 32 + lane;
+                next[4 + g] = r < a.n ? *reinterpret_cast<const uint32_t*>(a.scales + r * scale_pitch + kb) : 0u;
+            }
+        };
+        if (blockIdx.x < tiles) fetch(blockIdx.x, 0);
+        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int kb0 = 0; kb0 < k_blocks && ok; kb0 += 4) {
+                uint32_t w[12];
+#pragma unroll
+                for (int i = 0; i < 12; ++i) w[i] = next[i];
+                if (kb0 + 4 < k_blocks)
+                    fetch(t, kb0 + 4);
+                else if (t + gridDim.x < tiles)
+                    fetch(t + gridDim.x, 0);
+                for (int kb = kb0; kb < min(kb0 + 4, k_blocks); ++kb) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err));
+                    if (!ok) break;
+                    uint4* dst = reinterpret_cast<uint4*>(smem + kOffScales + s * kScaleBytes) + lane;
+                    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                    dst[32] = make_uint4(w[4], w[5], w[6], w[7]);
+                    dst[64] = make_uint4(w[8], w[9], w[10], w[11]);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[s]);
+                    if (++s == kStages) {
+                        s = 0;
+                        par ^= 1u;
                     }
-                }
-                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err));
-                if (!ok) break;
-                uint4* dst = reinterpret_cast<uint4*>(smem + kOffScales + s * kScaleBytes) + lane;
-                dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                dst[32] = make_uint4(w[4], w[5], w[6], w[7]);
-                dst[64] = make_uint4(w[8], w[9], w[10], w[11]);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[s]);
-                if (++s == kStages) {
-                    s = 0;
-                    par ^= 1u;
                 }
             }
         }
     } else if (warp >= 4) {
         const int g = warp & 3;                          // the 32 lanes of tensor memory this warp reads
-        float* stage = reinterpret_cast<float*>(smem + kOffStage) + g * 32 * kStagePitch;
-        uint32_t i = 0;
+        unsigned char* stage = smem + kOffOut + g * 4096;
+        float* sbias = reinterpret_cast<float*>(smem + kOffBias) + g * kTileN;
+        uint32_t i = 0, piece = 0;
         for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
             const int64_t m0 = (t % tiles_m) * kTileM + g * 32, n0 = (t / tiles_m) * kTileN;
+            if (a.bias) {
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < kTileN; j += 32) sbias[j + lane] = n0 + j + lane < a.n ? a.bias[n0 + j + lane] : 0.f;
+                __syncwarp();
+            }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1u, abort_flag, a.err))) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16) + (i & 1u) * kAccStep;
             // the accumulator's shared columns first: its last 64 or its first 64
             const int start = (i & 1u) ? 0 : kTileN - kShared;
+#pragma unroll 1
             for (int c = 0; c < kTileN; c += 32) {
                 const int col = (start + c) & (kTileN - 1);
+                const bool used = m0 < a.Q && n0 + col < a.n;
                 uint32_t r[32];
-                tmem_ld32(acc + (uint32_t)col, r);
-                tmem_ld_wait();
+                if (used) {
+                    tmem_ld32(acc + (uint32_t)col, r);
+                    tmem_ld_wait();
+                }
                 if (c + 32 == kShared) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(tfree);
                 }
-                __syncwarp();
+                if (!used) continue;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) stage[lane * kStagePitch + j] = __uint_as_float(r[j]);
-                __syncwarp();
-                const int64_t n = n0 + col + lane;
-                if (n < a.n) {
-                    const float b = a.bias ? a.bias[n] : 0.f;
-                    T* out = static_cast<T*>(a.out) + m0 * a.ld + n;
-                    const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);
-                    for (int j = 0; j < rows; ++j)
-                        out[j * a.ld] = narrow<T>(fmaf(a.alpha, stage[j * kStagePitch + lane], b));
+                for (int j = 0; j < 32; j += 4) {
+                    float4 b = a.bias ? *reinterpret_cast<const float4*>(sbias + col + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    r[j] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j]), b.x));
+                    r[j + 1] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j + 1]), b.y));
+                    r[j + 2] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j + 2]), b.z));
+                    r[j + 3] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j + 3]), b.w));
+                }
+                if (TMA_OUT) {
+                    constexpr int W = 64 / (int)sizeof(T);      // columns of a piece
+#pragma unroll
+                    for (int p = 0; p < 32; p += W) {
+                        if (n0 + col + p >= a.n) break;
+                        unsigned char* buf = stage + (piece++ & 1u) * 2048;
+                        // all but the latest piece have left shared memory
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            uint4 x;
+                            if (sizeof(T) == 4)
+                                x = make_uint4(r[p + 4 * u], r[p + 4 * u + 1], r[p + 4 * u + 2], r[p + 4 * u + 3]);
+                            else
+                                x = make_uint4(pack2<T>(__uint_as_float(r[(8 * u) & 31]), __uint_as_float(r[(8 * u + 1) & 31])),
+                                               pack2<T>(__uint_as_float(r[(8 * u + 2) & 31]), __uint_as_float(r[(8 * u + 3) & 31])),
+                                               pack2<T>(__uint_as_float(r[(8 * u + 4) & 31]), __uint_as_float(r[(8 * u + 5) & 31])),
+                                               pack2<T>(__uint_as_float(r[(8 * u + 6) & 31]), __uint_as_float(r[(8 * u + 7) & 31])));
+                            *reinterpret_cast<uint4*>(buf + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = x;
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) tma_store_2d(&map_out, (int)(n0 + col + p), (int)m0, buf);
+                    }
+                } else {
+                    float* tile = reinterpret_cast<float*>(stage);      // column j of row l at l * 32 + (j ^ l)
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = __uint_as_float(r[j]);
+                    __syncwarp();
+                    if (n0 + col + lane < a.n) {
+                        T* out = static_cast<T*>(a.out) + m0 * a.ld + n0 + col + lane;
+                        const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);
+#pragma unroll 4
+                        for (int j = 0; j < rows; ++j) out[j * a.ld] = narrow<T>(tile[j * 32 + (lane ^ j)]);
+                    }
                 }
             }
         }
+        if (TMA_OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
 
     tc_fence_before();
@@ -460,30 +564,44 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// Codes as a 2-D tensor (column, row); columns >= dim and rows past the end read zeros.
-bool codes_map(CUtensorMap* map, const uint8_t* codes, int64_t rows, int dim, int box_rows) {
+// A matrix as a 2-D tensor (column, row).  Loads outside it read zeros, stores outside it are dropped.
+bool matrix_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows, int64_t cols, int64_t row_bytes,
+                int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
     EncodeTiledFn enc = encode_fn();
     if (!enc) return false;
-    const cuuint64_t gdim[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
-    const cuuint64_t gstride[1] = {(cuuint64_t)fp8_code_pitch(dim)};
-    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows};
+    const cuuint64_t gdim[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t gstride[1] = {(cuuint64_t)row_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), gdim, gstride, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return enc(map, type, 2, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T>
 cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(fp8_scores_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (e != cudaSuccess) return e;
-    alignas(64) CUtensorMap map_a, map_b;
-    if (!codes_map(&map_a, a.q_codes, a.Q, a.dim, kTileM) || !codes_map(&map_b, a.codes, a.n, a.dim, kTileN))
+    const CUtensorMapDataType type = a.type == kTypeF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : a.type == kTypeBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    // tensor stores need rows that start at 16-byte boundaries
+    const bool tma = ((uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T))) % 16 == 0;
+    alignas(64) CUtensorMap map_a, map_b, map_out;
+    if (!matrix_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q_codes, a.Q, a.dim, fp8_code_pitch(a.dim), kTileK, kTileM,
+                    CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !matrix_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.n, a.dim, fp8_code_pitch(a.dim), kTileK, kTileN,
+                    CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
+    if (!tma)
+        map_out = map_a;      // not used
+    else if (!matrix_map(&map_out, type, a.out, a.Q, a.n, a.ld * (int64_t)sizeof(T), 64 / (int)sizeof(T), 32,
+                         CU_TENSOR_MAP_SWIZZLE_64B))
+        return cudaErrorInvalidValue;
+    auto kernel = tma ? fp8_scores_kernel<T, true> : fp8_scores_kernel<T, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
     const int tiles_m = (a.Q + kTileM - 1) / kTileM;
     const int64_t tiles = (int64_t)tiles_m * ((a.n + kTileN - 1) / kTileN);
     const int grid = (int)(tiles < sm_count ? tiles : sm_count);
-    fp8_scores_kernel<T><<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, a, tiles_m, tiles);
+    kernel<<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, map_out, a, tiles_m, tiles);
     return cudaGetLastError();
 }
 
