@@ -15,7 +15,7 @@ from . import build as _build
 
 L2, IP = 0, 1
 F32, BF16, F16 = 0, 1, 2
-TOPK_MAX = 1024
+FP8_MAX_DIM = 65536
 STATS_W = 8
 STAT_NAMES = ("status", "n_dist", "n_exp", "rounds", "hops", "n_scan", "max_cand", "n_spill")
 OK, ERR_ARG, ERR_STATE, ERR_CUDA, ERR_NOGPU, ERR_KERNEL, ERR_LIMIT, ERR_QUERY = range(8)
@@ -158,17 +158,18 @@ def _ptr(x, dtype):
     return C.c_void_p(a.ctypes.data), a
 
 
+_torch = None
 _score_types = {}
 
 
-def _score_type(t, name: str) -> int:
-    if not _score_types:
+def _use_torch():
+    """torch, imported when the first operator on score rows runs (the rest of the binding takes numpy)."""
+    global _torch
+    if _torch is None:
         import torch
         _score_types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
-    code = _score_types.get(t.dtype)
-    if code is None:
-        raise CoralError(ERR_ARG, f"{name} must be float32, bfloat16 or float16")
-    return code
+        _torch = torch
+    return _torch
 
 
 def _refuse(name: str, what: str):
@@ -475,74 +476,77 @@ class Index:
     def _stream(self):
         """torch's default stream, whose handle is 0, is CUDA's legacy stream (1): in the C calls 0 stands
         for the handle's own stream."""
-        import torch
-        return torch._C._cuda_getCurrentRawStream(self.device) or 1
+        return _torch._C._cuda_getCurrentRawStream(self.device) or 1
 
-    def _on_device(self, name: str, t, dtypes, shape=None, contiguous=True):
-        """Checks of a tensor argument that the C call cannot make."""
-        if not (_is_torch(t) and t.is_cuda and t.device.index == self.device):
-            _refuse(name, f"a tensor of cuda:{self.device}")
-        if dtypes is not None and t.dtype not in dtypes:
-            _refuse(name, " or ".join(str(d) for d in dtypes))
-        if shape is not None and tuple(t.shape) != shape:
-            _refuse(name, f"of shape {list(shape)}")
-        if contiguous and not t.is_contiguous():
-            _refuse(name, "contiguous")
-        return t.data_ptr()
+    def _at(self, name: str, t, dtype, shape):
+        """The address of a contiguous tensor of this type and shape on the handle's GPU."""
+        try:
+            if t.get_device() == self.device and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+                return t.data_ptr()
+        except AttributeError:
+            pass
+        _refuse(name, f"a contiguous {dtype} tensor of shape {list(shape)} on cuda:{self.device}")
 
     def _rows(self, name: str, t):
-        """(pointer, type, rows, columns, elements between rows) of a matrix whose rows are contiguous."""
-        p = self._on_device(name, t, None, contiguous=False)
-        if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-            _refuse(name, "a matrix with contiguous rows")
-        return p, _score_type(t, name), t.shape[0], t.shape[1], max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+        """(address, type, rows, columns, elements between rows) of a matrix whose rows are contiguous."""
+        try:
+            kind = _score_types.get(t.dtype)
+            if kind is not None and t.get_device() == self.device:
+                rows, cols = t.shape
+                ld, step = t.stride()
+                if rows <= 1:
+                    ld = cols
+                if (step == 1 or cols <= 1) and ld >= cols and not (rows | cols) >> 31:
+                    return t.data_ptr(), kind, rows, cols, ld
+        except (AttributeError, ValueError):
+            pass
+        _refuse(name, f"a float32, bfloat16 or float16 matrix with contiguous rows on cuda:{self.device}")
 
     def fp8_quantize(self, x, out=None):
         """Compresses the rows of a float matrix: (codes float8_e4m3fn [rows, code pitch], scales
         float8_e8m0fnu [rows, scale pitch]); see coral_fp8_quantize.  `out` = such a pair to write to,
         e.g. the rows of a larger base at which new ones start."""
-        import torch
+        torch = _torch or _use_torch()
         p, kind, rows, dim, ld = self._rows("x", x)
-        cp, sp = self._lib.coral_fp8_code_pitch(dim), self._lib.coral_fp8_scale_pitch(dim)
-        if cp == 0:
-            _refuse("x", "1 to 65536 columns wide")
+        if not 1 <= dim <= FP8_MAX_DIM:
+            _refuse("x", f"1 to {FP8_MAX_DIM} columns wide")
+        codes, scales = (rows, (dim + 15) // 16 * 16), (rows, (dim + 511) // 512 * 4)
         if out is None:
-            codes = torch.empty((rows, cp), dtype=torch.float8_e4m3fn, device=x.device)
-            scales = torch.empty((rows, sp), dtype=torch.float8_e8m0fnu, device=x.device)
+            out = (x.new_empty(codes, dtype=torch.float8_e4m3fn), x.new_empty(scales, dtype=torch.float8_e8m0fnu))
+            pc, ps = out[0].data_ptr(), out[1].data_ptr()
         else:
-            codes, scales = out
-        self._check(self._lib.coral_fp8_quantize(
-            self._h, p, kind, rows, dim, ld, self._on_device("codes", codes, (torch.float8_e4m3fn,), (rows, cp)),
-            self._on_device("scales", scales, (torch.float8_e8m0fnu,), (rows, sp)), self._stream()))
-        return codes, scales
+            pc = self._at("codes", out[0], torch.float8_e4m3fn, codes)
+            ps = self._at("scales", out[1], torch.float8_e8m0fnu, scales)
+        self._check(self._lib.coral_fp8_quantize(self._h, p, kind, rows, dim, ld, pc, ps, self._stream()))
+        return out
 
     def fp8_scores(self, queries, base, dim: int, alpha: float = 1.0, bias=None, dtype=None, out=None):
         """alpha * <query, row> + bias[row] of compressed queries and base rows (pairs as fp8_quantize
         returns them) of `dim` columns: [Q, n] in `dtype` (float32 unless given), or into `out`, whose
         rows may be apart.  See coral_fp8_scores."""
-        import torch
-        cp, sp = self._lib.coral_fp8_code_pitch(dim), self._lib.coral_fp8_scale_pitch(dim)
-        if cp == 0:
-            raise CoralError(ERR_ARG, "dim must be in [1, 65536]")
+        torch = _torch or _use_torch()
+        if not 1 <= dim <= FP8_MAX_DIM:
+            raise CoralError(ERR_ARG, f"dim must be in [1, {FP8_MAX_DIM}]")
+        cp, sp = (dim + 15) // 16 * 16, (dim + 511) // 512 * 4
         Q, n = queries[0].shape[0], base[0].shape[0]
-        p = [self._on_device(f"{name} {part}", pair[i], (kind,), (rows, pitch))
-             for name, pair, rows in (("queries'", queries, Q), ("base's", base, n))
-             for i, part, kind, pitch in ((0, "codes", torch.float8_e4m3fn, cp), (1, "scales", torch.float8_e8m0fnu, sp))]
+        pq = self._at("the queries' codes", queries[0], torch.float8_e4m3fn, (Q, cp))
+        sq = self._at("the queries' scales", queries[1], torch.float8_e8m0fnu, (Q, sp))
+        pr = self._at("the base's codes", base[0], torch.float8_e4m3fn, (n, cp))
+        sr = self._at("the base's scales", base[1], torch.float8_e8m0fnu, (n, sp))
+        pb = None if bias is None else self._at("bias", bias, torch.float32, (n,))
         if out is None:
             # rows start at multiples of 16 bytes whatever n: what follows loads and stores whole vectors
             dtype = dtype or torch.float32
             per = 16 // dtype.itemsize
-            out = torch.empty((Q, -(-n // per) * per), dtype=dtype, device=base[0].device)
+            out = base[0].new_empty((Q, (n + per - 1) // per * per), dtype=dtype)
             if out.shape[1] != n:
                 out = out[:, :n]
-        elif dtype is not None and out.dtype != dtype:
+        elif dtype is not None and out.dtype is not dtype:
             _refuse("out", str(dtype))
         po, kind, rows, cols, ld = self._rows("out", out)
-        if (rows, cols) != (Q, n):
+        if rows != Q or cols != n:
             _refuse("out", f"of shape {[Q, n]}")
-        pb = None if bias is None else self._on_device("bias", bias, (torch.float32,), (n,))
-        self._check(self._lib.coral_fp8_scores(self._h, p[0], p[1], Q, p[2], p[3], n, dim, alpha, pb, po, kind, ld,
-                                               self._stream()))
+        self._check(self._lib.coral_fp8_scores(self._h, pq, sq, Q, pr, sr, n, dim, alpha, pb, po, kind, ld, self._stream()))
         return out
 
     def adjust_scores(self, scores, seen=None, penalties=None, bias_ids=None, bias=None, excluded=None, out=None):
@@ -550,31 +554,35 @@ class Index:
         penalties float32 [Q, 3] (repetition, frequency, presence), bias_ids int32 and bias float32
         [Q, *], excluded int32 words [Q or 1, (n + 31) // 32].  Writes `out` (a new matrix unless given;
         `scores` itself works in place) and returns it."""
-        import torch
+        torch = _torch or _use_torch()
         p, kind, Q, n, ld = self._rows("scores", scores)
         if out is None:
             out = torch.empty_strided((Q, n), (ld, 1), dtype=scores.dtype, device=scores.device)
-        po, kind_out, rows, cols, ld_out = self._rows("out", out)
-        if (rows, cols, kind_out) != (Q, n, kind):
-            _refuse("out", f"{scores.dtype} of shape {[Q, n]}")
+            po, ld_out = out.data_ptr(), ld
+        else:
+            po, kind_out, rows, cols, ld_out = self._rows("out", out)
+            if rows != Q or cols != n or kind_out != kind:
+                _refuse("out", f"{scores.dtype} of shape {[Q, n]}")
         ps = pp = pi = pb = pe = None
         n_seen = n_bias = ld_ex = 0
         if seen is not None:
-            n_seen = seen.shape[1] if _is_torch(seen) and seen.dim() == 2 else -1
-            ps = self._on_device("seen", seen, (torch.int32,), (Q, n_seen))
-            pp = self._on_device("penalties", penalties, (torch.float32,), (Q, 3))
+            n_seen = seen.shape[-1] if _is_torch(seen) and seen.dim() else 0
+            ps = self._at("seen", seen, torch.int32, (Q, n_seen))
+            pp = self._at("penalties", penalties, torch.float32, (Q, 3))
         elif penalties is not None:
             _refuse("seen", "given with penalties")
+        if n_seen >> 31:
+            _refuse("seen", "narrower than 2^31")
         if bias_ids is not None:
-            n_bias = bias_ids.shape[1] if _is_torch(bias_ids) and bias_ids.dim() == 2 else -1
-            pi = self._on_device("bias_ids", bias_ids, (torch.int32,), (Q, n_bias))
-            pb = self._on_device("bias", bias, (torch.float32,), (Q, n_bias))
+            n_bias = bias_ids.shape[-1] if _is_torch(bias_ids) and bias_ids.dim() else 0
+            pi = self._at("bias_ids", bias_ids, torch.int32, (Q, n_bias))
+            pb = self._at("bias", bias, torch.float32, (Q, n_bias))
         elif bias is not None:
             _refuse("bias_ids", "given with bias")
         if excluded is not None:
             words = (n + 31) // 32
             one = _is_torch(excluded) and excluded.dim() == 2 and excluded.shape[0] == 1
-            pe = self._on_device("excluded", excluded, (torch.int32,), (1 if one else Q, words))
+            pe = self._at("excluded", excluded, torch.int32, (1 if one else Q, words))
             ld_ex = 0 if one else words
         self._check(self._lib.coral_adjust_scores(self._h, p, kind, Q, n, ld, ps, n_seen, pp, pi, pb, n_bias, pe, ld_ex, po,
                                                   ld_out, self._stream()))
@@ -583,16 +591,18 @@ class Index:
     def topk_scores(self, scores, k: int, id_base: int = 0):
         """(ids int32 [Q, k], scores float32 [Q, k]) of the k largest of every row, best first, equal
         scores by the lower column; see coral_topk_scores."""
-        import torch
+        torch = _torch or _use_torch()
         p, kind, Q, n, ld = self._rows("scores", scores)
+        if not (0 <= k < 2 ** 31 and 0 <= id_base <= 2 ** 31 - 1 - n):      # what a C int cannot hold
+            raise CoralError(ERR_ARG, "k must be in [1, 1024] and id_base in [0, 2^31 - n)")
         need = C.c_int64(0)
         self._check(self._lib.coral_topk_workspace(self._h, Q, n, k, C.byref(need)))
-        ids = torch.empty((Q, k), dtype=torch.int32, device=scores.device)
-        best = torch.empty((Q, k), dtype=torch.float32, device=scores.device)
-        ws = torch.empty(need.value, dtype=torch.uint8, device=scores.device) if need.value else None
+        size = need.value
+        ids = scores.new_empty((Q, k), dtype=torch.int32)
+        best = scores.new_empty((Q, k), dtype=torch.float32)
+        ws = scores.new_empty((size,), dtype=torch.uint8) if size else None
         self._check(self._lib.coral_topk_scores(self._h, p, kind, Q, n, ld, k, id_base, ids.data_ptr(), best.data_ptr(),
-                                                ws.data_ptr() if ws is not None else None, need.value,
-                                                self._stream()))
+                                                ws.data_ptr() if size else None, size, self._stream()))
         return ids, best
 
     def scores_check(self):

@@ -18,16 +18,6 @@ namespace {
 
 // ------------------------------------------------------------------------------- compression
 
-// Order of |v|.  What is not finite counts as nothing, and its code is NaN (e4m3 has no infinity): it
-// shows in every score of its row and costs the rest of its block no precision.
-__device__ __forceinline__ uint32_t abs_bits(float v) {
-    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;
-}
-__device__ __forceinline__ float scaled(float v, float f) {
-    return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v * f : __uint_as_float(0x7fffffffu);
-}
-
 // Least e in [-127, 127] with amax <= 448 * 2^e, 448 = 1.75 * 2^8, from the bits of amax: the
 // exponent less 8, one more when the mantissa is above 1.75.  A subnormal or zero amax ends at -127.
 __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
@@ -55,19 +45,36 @@ __device__ __forceinline__ float wide<__nv_bfloat16>(__nv_bfloat16 v) { return _
 template <>
 __device__ __forceinline__ float wide<__half>(__half v) { return __half2float(v); }
 
-#ifndef QSTEPS
-#define QSTEPS 4
-#endif
 constexpr int kQuantThreads = 256;
-constexpr int kQuantSteps = QSTEPS;    // 16-byte loads a lane has in flight
+constexpr int kQuantSteps = 4;    // 16-byte loads a lane has in flight
+
+// The largest magnitude of 16 bytes, as the bits of an fp32: magnitudes order as their bits do.
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max(uint4 v);
+template <>
+__device__ __forceinline__ uint32_t abs_max<float>(uint4 v) {
+    return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+}
+__device__ __forceinline__ uint32_t abs_max_halves(uint4 v) {
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+}
+template <>
+__device__ __forceinline__ uint32_t abs_max<__nv_bfloat16>(uint4 v) { return abs_max_halves(v) << 16; }
+template <>
+__device__ __forceinline__ uint32_t abs_max<__half>(uint4 v) {
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)abs_max_halves(v))));
+}
 
 // A block of 128 columns belongs to G lanes that hold 16 bytes each (32 lanes of fp32, 16 of the 16-bit
 // types): one coalesced read, and its maximum one reduction over the magnitudes' bits.  A warp takes
-// kQuantSteps * 32 / G consecutive blocks and writes their scales together.  Bound by memory.
+// kQuantSteps * 32 / G consecutive blocks and writes their scales together.  Bound by memory, and close
+// behind it by instructions: what is not finite (a maximum of an infinity's bits or more) is dealt with
+// in a branch of its own.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads)
 fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, uint8_t* __restrict__ codes,
-                    uint8_t* __restrict__ scales) {
+                    uint8_t* __restrict__ scales, uint32_t inv_per_row) {
     constexpr int E = 16 / (int)sizeof(T), G = kFp8Block / E, P = 32 / G, N = kQuantSteps * P;
     const int lane = threadIdx.x & 31, in_block = lane % G, g = lane / G;
     const uint32_t members = G == 32 ? 0xffffffffu : 0xffffu << (g * G);
@@ -78,16 +85,17 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
     if (first >= total) return;
     const int64_t row0 = total <= 0x7fffffff ? (int64_t)((uint32_t)first / (uint32_t)per_row) : first / per_row;
     const int b0 = (int)(first - row0 * per_row);
-    auto place = [&](int i, int64_t& row, int& b) {      // block first + i
-        row = row0;
+    auto place = [&](int i, int64_t& row, int& b) {      // block first + i, i < N
         b = b0 + i;
-        if (b >= per_row) {
-            const int over = b / per_row;
-            row += over;
-            b -= over * per_row;
-        }
+        const int over = per_row >= N ? (b >= per_row ? 1 : 0) : (int)((uint32_t)b * inv_per_row >> 16);
+        row = row0 + over;
+        b -= over * per_row;
     };
-    alignas(16) T v[kQuantSteps][E];
+    union Piece {
+        uint4 raw;
+        T v[E];
+        __device__ Piece() {}
+    } in[kQuantSteps];
     int64_t row[kQuantSteps];
     int b[kQuantSteps];
 #pragma unroll
@@ -95,22 +103,38 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
         place(u * P + g, row[u], b[u]);
         const int c = b[u] * kFp8Block + in_block * E;
         const T* p = x + row[u] * ld + c;
+        in[u].raw = make_uint4(0u, 0u, 0u, 0u);
         if (first + u * P + g < total) {
             if (VEC && c + E <= dim) {
-                *reinterpret_cast<uint4*>(v[u]) = __ldcs(reinterpret_cast<const uint4*>(p));
+                in[u].raw = __ldcs(reinterpret_cast<const uint4*>(p));
             } else {
 #pragma unroll
-                for (int i = 0; i < E; ++i) v[u][i] = c + i < dim ? p[i] : T(0.f);
+                for (int i = 0; i < E; ++i)
+                    if (c + i < dim) in[u].v[i] = p[i];
             }
         }
     }
     int mine = 0;      // the exponent of block first + lane
 #pragma unroll
     for (int u = 0; u < kQuantSteps; ++u) {
-        uint32_t m = 0;
+        uint32_t m = __reduce_max_sync(members, abs_max<T>(in[u].raw));
+        float v[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) m = max(m, abs_bits(wide<T>(v[u][i])));
-        m = __reduce_max_sync(members, m);
+        for (int i = 0; i < E; ++i) v[i] = wide<T>(in[u].v[i]);
+        if (m >= 0x7f800000u) {
+            // What is not finite counts as nothing, and its code is NaN (e4m3 has no infinity): it shows
+            // in every score of its row and costs the rest of its block no precision.
+            m = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+                if (a < 0x7f800000u)
+                    m = max(m, a);
+                else
+                    v[i] = __uint_as_float(0x7fffffffu);
+            }
+            m = __reduce_max_sync(members, m);
+        }
         const int e = scale_exponent(m);
         const float f = __uint_as_float((uint32_t)(127 - e) << 23);     // 2^-e: e in [-127, 120], 2^-e never subnormal
         const int got = P == 1 ? e : __shfl_sync(0xffffffffu, e, lane % P * G);
@@ -119,9 +143,7 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
         if (first + u * P + g < total && c < code_pitch) {
             uint32_t w[E / 4];
 #pragma unroll
-            for (int i = 0; i < E; i += 4)
-                w[i / 4] = pack_e4m3(scaled(wide<T>(v[u][i]), f), scaled(wide<T>(v[u][i + 1]), f),
-                                     scaled(wide<T>(v[u][i + 2]), f), scaled(wide<T>(v[u][i + 3]), f));
+            for (int i = 0; i < E; i += 4) w[i / 4] = pack_e4m3(v[i] * f, v[i + 1] * f, v[i + 2] * f, v[i + 3] * f);
             uint8_t* out = codes + row[u] * code_pitch + c;
             if (E == 4)
                 *reinterpret_cast<uint32_t*>(out) = w[0];
@@ -148,7 +170,8 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
     const int64_t ctas = (total + per_cta - 1) / per_cta;
     const bool vec = ((uintptr_t)x | (uintptr_t)(ld * sizeof(T))) % 16 == 0;
     auto kernel = vec ? fp8_quantize_kernel<T, true> : fp8_quantize_kernel<T, false>;
-    kernel<<<(unsigned)ctas, kQuantThreads, 0, stream>>>(static_cast<const T*>(x), rows, dim, ld, codes, scales);
+    kernel<<<(unsigned)ctas, kQuantThreads, 0, stream>>>(static_cast<const T*>(x), rows, dim, ld, codes, scales,
+                                                    65536u / (uint32_t)((dim + kFp8Block - 1) / kFp8Block) + 1u);
     return cudaGetLastError();
 }
 

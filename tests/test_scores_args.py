@@ -13,7 +13,7 @@ def test_row_layout():
         cp, sp = lib.coral_fp8_code_pitch(dim), lib.coral_fp8_scale_pitch(dim)
         assert cp % 16 == 0 and dim <= cp < dim + 16
         assert sp % 4 == 0 and sp >= -(-dim // 128) and (sp - 4) * 128 < dim
-    for dim in (0, -1, 65537):
+    for dim in (0, -1, capi.FP8_MAX_DIM + 1):
         assert lib.coral_fp8_code_pitch(dim) == 0 and lib.coral_fp8_scale_pitch(dim) == 0
 
 
