@@ -178,15 +178,16 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // ----------------------------------------------------------------------------------- product
 //
 // out[q][j] = alpha * sum_b 2^(eq_b + ej_b) * (codes of q, codes of j)_b + bias[j], accumulated in
-// fp32 in tensor memory.  One persistent CTA of 8 warps per SM, tiles of 128 queries x 256 rows:
+// fp32 in tensor memory.  One persistent CTA of 12 warps per SM, tiles of 128 queries x 256 rows:
 //   warp 0     one lane issues the tiles' TMA loads (128-byte swizzle, 128 columns a stage);
 //   warp 1     one lane issues, per stage, three tcgen05.cp (the stage's scales to tensor memory)
 //              and four tcgen05.mma (M = 128, N = 256, K = 32);
 //   warp 2     brings the stage's scales to shared memory in the layout tcgen05.cp takes, the words of
 //              the next four stages in flight;
-//   warps 4-7  read the finished accumulator, apply alpha and bias, and store: 64-byte pieces of 32
-//              rows through shared memory (64-byte swizzle) and TMA, two pieces in flight a warp, or,
-//              where the output's rows do not start at 16-byte boundaries, by coalesced plain stores.
+//   warps 4-11 read the finished accumulator (two warps to a quarter of its rows, turn by turn),
+//              apply alpha and bias, and store: pieces of 32 rows x 128 bytes through shared memory
+//              (128-byte swizzle) and TMA, two in flight a warp, or, where the output's rows do not
+//              start at 16-byte boundaries, by coalesced plain stores.
 // A scale word of four bytes covers 512 columns; an instruction's K = 32 lies inside one block, so
 // all four instructions of a stage name the same byte of the word (the scale ids of the instruction
 // descriptor), byte (k-block mod 4).
@@ -196,17 +197,20 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // lets the next tile's products start.
 
 constexpr int kTileM = 128, kTileN = 256, kTileK = 128;
-constexpr int kStages = 4;
+#ifndef NSTAGES
+#define NSTAGES 3
+#endif
+constexpr int kStages = NSTAGES;
 constexpr int kABytes = kTileM * kTileK, kBBytes = kTileN * kTileK;
 constexpr int kScaleBytes = (kTileM + kTileN) * 4;
 constexpr int kAccStep = 192, kShared = 64, kTmemScales = 448;
 constexpr int kOffScales = kStages * (kABytes + kBBytes);
-constexpr int kOffOut = kOffScales + kStages * kScaleBytes;         // 4 KB of output staging a warp
-constexpr int kOffBias = kOffOut + 4 * 4096;                        // the tile's biases, one copy a warp
-constexpr int kOffBars = kOffBias + 4 * kTileN * 4;
-static_assert(kOffOut % 1024 == 0, "swizzled staging");
+constexpr int kEpiWarps = 8, kOutBufs = 2;
+constexpr int kOffOut = (kOffScales + kStages * kScaleBytes + 1023) / 1024 * 1024;
+constexpr int kOffBias = kOffOut + kEpiWarps * kOutBufs * 4096;     // each warp the biases of its columns
+constexpr int kOffBars = kOffBias + kEpiWarps * (kTileN / 2) * 4;
 constexpr int kSmemBytes = kOffBars + 256 + 1024;
-constexpr int kThreads = 256;
+constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr long long kWaitClocks = 4000000000ll;                     // ~2 s
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -352,7 +356,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             mbar_init(&empty[s], 1);
         }
         mbar_init(tfull, 1);
-        mbar_init(tfree, 4);
+        mbar_init(tfree, kEpiWarps);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -466,82 +470,93 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     } else if (warp >= 4) {
-        const int g = warp & 3;                          // the 32 lanes of tensor memory this warp reads
-        unsigned char* stage = smem + kOffOut + g * 4096;
-        float* sbias = reinterpret_cast<float*>(smem + kOffBias) + g * kTileN;
-        uint32_t i = 0, piece = 0;
+        const int g = warp & 3, half = (warp - 4) >> 2;      // 32 lanes of tensor memory; which of their two warps
+        constexpr int W = 128 / (int)sizeof(T);              // columns of a piece
+        constexpr int kPieces = kTileN / W;
+        unsigned char* stage = smem + kOffOut + (warp - 4) * kOutBufs * 4096;
+        float* sbias = reinterpret_cast<float*>(smem + kOffBias) + (warp - 4) * (kTileN / 2);
+        uint32_t i = 0, sent = 0;
         for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
             const int64_t m0 = (t % tiles_m) * kTileM + g * 32, n0 = (t / tiles_m) * kTileN;
+            // pieces in turn from the accumulator's shared columns on: its last 64 or its first 64
+            const int start = (i & 1u) ? 0 : kTileN - kShared;
+            const auto col_of = [&](int p) { return (start + p * W) & (kTileN - 1); };
             if (a.bias) {
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < kTileN; j += 32) sbias[j + lane] = n0 + j + lane < a.n ? a.bias[n0 + j + lane] : 0.f;
+                for (int p = 0; p < kPieces / 2; ++p)
+#pragma unroll
+                    for (int j = 0; j < W; j += 32) {
+                        const int64_t n = n0 + col_of(2 * p + half) + j + lane;
+                        sbias[p * W + j + lane] = n < a.n ? a.bias[n] : 0.f;
+                    }
                 __syncwarp();
             }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1u, abort_flag, a.err))) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16) + (i & 1u) * kAccStep;
-            // the accumulator's shared columns first: its last 64 or its first 64
-            const int start = (i & 1u) ? 0 : kTileN - kShared;
 #pragma unroll 1
-            for (int c = 0; c < kTileN; c += 32) {
-                const int col = (start + c) & (kTileN - 1);
+            for (int p = 0; p < kPieces / 2; ++p) {
+                const int col = col_of(2 * p + half);
                 const bool used = m0 < a.Q && n0 + col < a.n;
-                uint32_t r[32];
+                uint32_t r[W / 32][32];
                 if (used) {
-                    tmem_ld32(acc + (uint32_t)col, r);
+#pragma unroll
+                    for (int w = 0; w < W / 32; ++w) tmem_ld32(acc + (uint32_t)(col + w * 32), r[w]);
                     tmem_ld_wait();
                 }
-                if (c + 32 == kShared) {
+                if (p == 0) {      // the shared columns are the first pieces of the two warps
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(tfree);
                 }
                 if (!used) continue;
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    float4 b = a.bias ? *reinterpret_cast<const float4*>(sbias + col + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    r[j] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j]), b.x));
-                    r[j + 1] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j + 1]), b.y));
-                    r[j + 2] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j + 2]), b.z));
-                    r[j + 3] = __float_as_uint(fmaf(a.alpha, __uint_as_float(r[j + 3]), b.w));
+                for (int j = 0; j < W; j += 4) {
+                    const float4 b = a.bias ? *reinterpret_cast<const float4*>(sbias + p * W + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    uint32_t* x = &r[j / 32][j % 32];
+                    x[0] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[0]), b.x));
+                    x[1] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[1]), b.y));
+                    x[2] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[2]), b.z));
+                    x[3] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[3]), b.w));
                 }
                 if (TMA_OUT) {
-                    constexpr int W = 64 / (int)sizeof(T);      // columns of a piece
+                    unsigned char* buf = stage + (sent++ % kOutBufs) * 4096;
+                    // the piece that used this buffer has left shared memory
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kOutBufs - 1) : "memory");
+                    __syncwarp();
 #pragma unroll
-                    for (int p = 0; p < 32; p += W) {
-                        if (n0 + col + p >= a.n) break;
-                        unsigned char* buf = stage + (piece++ & 1u) * 2048;
-                        // all but the latest piece have left shared memory
-                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                        __syncwarp();
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            uint4 x;
-                            if (sizeof(T) == 4)
-                                x = make_uint4(r[p + 4 * u], r[p + 4 * u + 1], r[p + 4 * u + 2], r[p + 4 * u + 3]);
-                            else
-                                x = make_uint4(pack2<T>(__uint_as_float(r[(8 * u) & 31]), __uint_as_float(r[(8 * u + 1) & 31])),
-                                               pack2<T>(__uint_as_float(r[(8 * u + 2) & 31]), __uint_as_float(r[(8 * u + 3) & 31])),
-                                               pack2<T>(__uint_as_float(r[(8 * u + 4) & 31]), __uint_as_float(r[(8 * u + 5) & 31])),
-                                               pack2<T>(__uint_as_float(r[(8 * u + 6) & 31]), __uint_as_float(r[(8 * u + 7) & 31])));
-                            *reinterpret_cast<uint4*>(buf + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = x;
+                    for (int u = 0; u < 8; ++u) {
+                        uint4 x;
+                        if (sizeof(T) == 4) {
+                            x = make_uint4(r[0][4 * u], r[0][4 * u + 1], r[0][4 * u + 2], r[0][4 * u + 3]);
+                        } else {
+                            const uint32_t* y = &r[(W / 32 - 1) * u / 4][8 * u % 32];
+                            x = make_uint4(pack2<T>(__uint_as_float(y[0]), __uint_as_float(y[1])),
+                                           pack2<T>(__uint_as_float(y[2]), __uint_as_float(y[3])),
+                                           pack2<T>(__uint_as_float(y[4]), __uint_as_float(y[5])),
+                                           pack2<T>(__uint_as_float(y[6]), __uint_as_float(y[7])));
                         }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) tma_store_2d(&map_out, (int)(n0 + col + p), (int)m0, buf);
+                        *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = x;
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tma_store_2d(&map_out, (int)(n0 + col), (int)m0, buf);
                 } else {
                     float* tile = reinterpret_cast<float*>(stage);      // column j of row l at l * 32 + (j ^ l)
-                    __syncwarp();
+                    const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = __uint_as_float(r[j]);
-                    __syncwarp();
-                    if (n0 + col + lane < a.n) {
-                        T* out = static_cast<T*>(a.out) + m0 * a.ld + n0 + col + lane;
-                        const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);
+                    for (int w = 0; w < W / 32; ++w) {
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = __uint_as_float(r[w][j]);
+                        __syncwarp();
+                        const int64_t n = n0 + col + w * 32 + lane;
+                        if (n < a.n) {
+                            T* out = static_cast<T*>(a.out) + m0 * a.ld + n;
 #pragma unroll 4
-                        for (int j = 0; j < rows; ++j) out[j * a.ld] = narrow<T>(tile[j * 32 + (lane ^ j)]);
+                            for (int j = 0; j < rows; ++j) out[j * a.ld] = narrow<T>(tile[j * 32 + (lane ^ j)]);
+                        }
                     }
                 }
             }
@@ -615,8 +630,8 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
         return cudaErrorInvalidValue;
     if (!tma)
         map_out = map_a;      // not used
-    else if (!matrix_map(&map_out, type, a.out, a.Q, a.n, a.ld * (int64_t)sizeof(T), 64 / (int)sizeof(T), 32,
-                         CU_TENSOR_MAP_SWIZZLE_64B))
+    else if (!matrix_map(&map_out, type, a.out, a.Q, a.n, a.ld * (int64_t)sizeof(T), 128 / (int)sizeof(T), 32,
+                         CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     auto kernel = tma ? fp8_scores_kernel<T, true> : fp8_scores_kernel<T, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
