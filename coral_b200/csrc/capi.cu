@@ -1553,6 +1553,8 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     ARG(dim >= 1 && dim <= coral::kFp8MaxDim, "dim must be in [1, 65536]");
     ARG(Q >= 0 && n >= 0 && n <= 0x7fffffffll, "Q and n must be in [0, 2^31)");
     ARG(ld >= n && ld < (1ll << 31), "ld must be in [n, 2^31)");
+    if (((int64_t)Q + 127) / 128 * ((n + 255) / 256) > 0x7fffffffll / 2)
+        return fail(h, CORAL_ERR_LIMIT, "too many scores for one call");
     if (Q == 0 || n == 0) return CORAL_OK;
     ARG(d_q_codes && d_q_scales && d_codes && d_scales && d_out, "null argument");
     DeviceScope scope(h->device);

@@ -180,10 +180,11 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // out[q][j] = alpha * sum_b 2^(eq_b + ej_b) * (codes of q, codes of j)_b + bias[j], accumulated in
 // fp32 in tensor memory.  One persistent CTA of 12 warps per SM, tiles of 128 queries x 256 rows:
 //   warp 0     one lane issues the tiles' TMA loads (128-byte swizzle, 128 columns a stage);
-//   warp 1     one lane issues, per stage, three tcgen05.cp (the stage's scales to tensor memory)
-//              and four tcgen05.mma (M = 128, N = 256, K = 32);
-//   warp 2     brings the stage's scales to shared memory in the layout tcgen05.cp takes, the words of
-//              the next four stages in flight;
+//   warp 1     one lane issues, per stage, four tcgen05.mma (M = 128, N = 256, K = 32) and, per four
+//              stages, three tcgen05.cp (their scales to tensor memory);
+//   warp 2     brings scales to a shared-memory ring of their own in the layout tcgen05.cp takes, with
+//              asynchronous 4-byte copies, six groups of four stages ahead: with rows of one or two
+//              stages the latency of a scale would otherwise be the time of a tile;
 //   warps 4-11 read the finished accumulator (two warps to a quarter of its rows, turn by turn),
 //              apply alpha and bias, and store: pieces of 32 rows x 128 bytes through shared memory
 //              (128-byte swizzle) and TMA, two in flight a warp, or, where the output's rows do not
@@ -193,24 +194,27 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // descriptor), byte (k-block mod 4).
 //
 // Tensor memory: two accumulators of 256 columns that share 64 (0-255 and 192-447) and, from 448,
-// one slot of 16 columns of scales per stage.  The epilogue reads the shared columns first and then
+// four slots of 16 columns of scales.  A slot is written again four groups, so at least four stages,
+// later; that stage's codes have landed, so the products of the stage kStages before it are done, and
+// with them the slot's old ones.  The epilogue reads the shared columns first and then
 // lets the next tile's products start.
 
 constexpr int kTileM = 128, kTileN = 256, kTileK = 128;
-#ifndef NSTAGES
-#define NSTAGES 3
-#endif
-constexpr int kStages = NSTAGES;
+constexpr int kStages = 3;
 constexpr int kABytes = kTileM * kTileK, kBBytes = kTileN * kTileK;
 constexpr int kScaleBytes = (kTileM + kTileN) * 4;
 constexpr int kAccStep = 192, kShared = 64, kTmemScales = 448;
 constexpr int kOffScales = kStages * (kABytes + kBBytes);
 constexpr int kEpiWarps = 8, kOutBufs = 2;
-constexpr int kOffOut = (kOffScales + kStages * kScaleBytes + 1023) / 1024 * 1024;
+constexpr int kScaleSlots = 8, kScalesAhead = 6;                    // groups in the ring, and in flight
+static_assert(kStages <= 4, "scale slots in tensor memory");
+constexpr int kOffOut = kOffScales + kScaleSlots * kScaleBytes;
+static_assert(kOffOut % 1024 == 0, "swizzled staging");
 constexpr int kOffBias = kOffOut + kEpiWarps * kOutBufs * 4096;     // each warp the biases of its columns
 constexpr int kOffBars = kOffBias + kEpiWarps * (kTileN / 2) * 4;
 constexpr int kSmemBytes = kOffBars + 256 + 1024;
 constexpr int kThreads = 128 + 32 * kEpiWarps;
+constexpr int64_t kChunkBytes = 32ll << 20;      // base bytes per chunk of tiles: a quarter of L2
 constexpr long long kWaitClocks = 4000000000ll;                     // ~2 s
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -228,10 +232,10 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint64_t* bar, uint32_t parity
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+        : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
     return ok;
 }
@@ -257,11 +261,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
         ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar))
         : "memory");
 }
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, const void* src) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0),
-                 "r"(c1), "r"(smem_u32(src))
-                 : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+// Issued by the leader lane of a converged warp.  Written once and not read here: the output leaves L2
+// to the base.
+__device__ __forceinline__ void tma_store_2d(uint32_t leads, const CUtensorMap* map, int c0, int c1, const void* src,
+                                             uint64_t policy) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%1, %2}], [%3], %4;\n\t"
+        "@q cp.async.bulk.commit_group;\n\t}" ::"l"(map), "r"(c0), "r"(c1), "r"(smem_u32(src)), "l"(policy), "r"(leads)
+        : "memory");
 }
 // Shared-memory matrix descriptor, K-major rows of 128 bytes with the 128-byte swizzle: 8-row groups
 // 1024 bytes apart, descriptor version 1, layout type 2.
@@ -276,22 +285,43 @@ __device__ __forceinline__ uint64_t desc_rows16(uint32_t addr) {
 // N / 8 from bit 17, M / 128 from bit 27; the scale ids (A from bit 29, B from bit 4) are or-ed in.
 constexpr uint32_t kInstrDesc = (1u << 23) | ((uint32_t)(kTileN >> 3) << 17) | ((uint32_t)(kTileM >> 7) << 27);
 
-__device__ __forceinline__ void umma_mxf8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                          uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
+// The issuing warp runs converged, with every operand the same in all lanes (so that operands stay in
+// uniform registers: moving them there from one diverged lane costs more than the product lasts), and
+// its leader lane issues.
+__device__ __forceinline__ uint32_t elect_leader() {
+    uint32_t leads;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(leads));
+    return leads;
+}
+__device__ __forceinline__ void umma_mxf8(uint32_t leads, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                          uint32_t idesc, uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+        "setp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate), "r"(leads)
         : "memory");
 }
 // 32 rows of 16 bytes to 4 columns of tensor memory, the same in each of the four lane groups.
-__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void scales_to_tmem(uint32_t leads, uint32_t taddr, uint64_t desc) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(leads)
+        : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void umma_commit(uint32_t leads, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(leads)
+        : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -333,27 +363,48 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 template <>
 __device__ __forceinline__ uint32_t pack2<float>(float lo, float) { return __float_as_uint(lo); }
 
+// The order of the tiles: the base in chunks of `chunk_n` row tiles that stay in L2, per chunk all query
+// tiles, per query tile the chunk's row tiles.  Neighbouring CTAs then write neighbouring pieces of the
+// same output rows, which DRAM takes faster than the same bytes scattered over many rows.
+struct TileOrder {
+    uint32_t tiles, tiles_m, tiles_n, chunk_n;
+    __device__ __forceinline__ void at(uint32_t t, int64_t& m0, int64_t& n0) const {
+        const uint32_t c = t / (chunk_n * tiles_m), left = tiles_n - c * chunk_n;
+        const uint32_t width = left < chunk_n ? left : chunk_n, in_chunk = t - c * chunk_n * tiles_m;
+        const uint32_t m = in_chunk / width;
+        m0 = (int64_t)m * kTileM;
+        n0 = (int64_t)(c * chunk_n + in_chunk - m * width) * kTileN;
+    }
+};
+
 template <typename T, bool TMA_OUT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                  const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const int tiles_m,
-                  const int64_t tiles) {
+                  const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const TileOrder order,
+                  const int a_rows) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);   // [kStages] codes and scales landed
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);   // [kStages] codes landed
     uint64_t* empty = full + kStages;                                // [kStages] the products that read the stage are done
-    uint64_t* tfull = empty + kStages;                               // accumulator complete
+    uint64_t* sfull = empty + kStages;                               // [kScaleSlots] a group's scales landed
+    uint64_t* sempty = sfull + kScaleSlots;                          // [kScaleSlots] and are no longer needed
+    uint64_t* tfull = sempty + kScaleSlots;                          // accumulator complete
     uint64_t* tfree = tfull + 1;                                     // the columns the next tile shares are drained
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // known to be uniform
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
     const int scale_pitch = (a.dim + 511) / 512 * 4;
 
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(&full[s], 2);        // the TMA lane and the scale warp
+            mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kScaleSlots; ++s) {
+            mbar_init(&sfull[s], 1);
+            mbar_init(&sempty[s], 1);
         }
         mbar_init(tfull, 1);
         mbar_init(tfree, kEpiWarps);
@@ -375,14 +426,15 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             int s = 0;
             uint32_t par = 0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                const int m0 = (int)(t % tiles_m) * kTileM, n0 = (int)(t / tiles_m) * kTileN;
+            for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x) {
+                int64_t m0, n0;
+                order.at(t, m0, n0);
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
                     unsigned char* st = smem + s * (kABytes + kBBytes);
-                    mbar_expect_tx(&full[s], kABytes + kBBytes);
-                    tma_load_2d(st, &map_a, kb * kTileK, m0, &full[s]);
-                    tma_load_2d(st + kABytes, &map_b, kb * kTileK, n0, &full[s]);
+                    mbar_expect_tx(&full[s], a_rows * kTileK + kBBytes);
+                    tma_load_2d(st, &map_a, kb * kTileK, (int)m0, &full[s]);
+                    tma_load_2d(st + kABytes, &map_b, kb * kTileK, (int)n0, &full[s]);
                     if (++s == kStages) {
                         s = 0;
                         par ^= 1u;
@@ -391,177 +443,192 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t par = 0, i = 0;
-            bool ok = true;
-            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
-                if (i > 0 && !mbar_wait(tfree, (i - 1) & 1u, abort_flag, a.err)) break;
-                tc_fence_after();
-                const uint32_t acc = tmem + (i & 1u) * kAccStep;
-                for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!(ok = mbar_wait(&full[s], par, abort_flag, a.err))) break;
-                    tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * (kABytes + kBBytes)), sb = sa + kABytes;
-                    const uint32_t sc = smem_u32(smem + kOffScales + s * kScaleBytes);
-                    const uint32_t ta = tmem + kTmemScales + s * 16, tb = ta + 8;
-                    scales_to_tmem(ta, desc_rows16(sc));
-                    scales_to_tmem(tb, desc_rows16(sc + 512));
-                    scales_to_tmem(tb + 4, desc_rows16(sc + 1024));
-                    const uint32_t id = (uint32_t)(kb & 3);
-                    const uint32_t idesc = kInstrDesc | id << 29 | id << 4;
-                    const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
-                    for (int j = 0; j < slices; ++j)
-                        umma_mxf8(acc, desc_sw128(sa + j * 32), desc_sw128(sb + j * 32), idesc, ta, tb,
-                                  (kb | j) != 0 ? 1u : 0u);
-                    umma_commit(&empty[s]);
-                    if (++s == kStages) {
-                        s = 0;
-                        par ^= 1u;
-                    }
+        const uint32_t leads = elect_leader();
+        const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + kOffScales);
+        uint32_t s = 0, par = 0, i = 0, group = 0;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x, ++i) {
+            if (i > 0 && !__all_sync(0xffffffffu, mbar_wait(tfree, (i - 1) & 1u, abort_flag, a.err))) break;
+            const uint32_t acc = tmem + (i & 1u) * kAccStep;
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a.err));
+                if (!ok) break;
+                const uint32_t slot = group % kScaleSlots, ta = tmem + kTmemScales + group % 4 * 16, tb = ta + 8;
+                if ((kb & 3) == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a.err));
+                    if (!ok) break;
                 }
-                if (ok) umma_commit(tfull);
+                tc_fence_after();
+                if ((kb & 3) == 0) {
+                    const uint64_t sc = desc_rows16(scales + slot * kScaleBytes);
+                    scales_to_tmem(leads, ta, sc);
+                    scales_to_tmem(leads, tb, sc + (512 >> 4));
+                    scales_to_tmem(leads, tb + 4, sc + (1024 >> 4));
+                }
+                const uint64_t da = desc_sw128(codes + s * (kABytes + kBBytes)), db = da + (kABytes >> 4);
+                const uint32_t idesc = kInstrDesc | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
+                const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
+                if (slices == kTileK / 32) {
+#pragma unroll
+                    for (int j = 0; j < kTileK / 32; ++j)
+                        umma_mxf8(leads, acc, da + j * 2, db + j * 2, idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
+                } else {
+                    for (int j = 0; j < slices; ++j)
+                        umma_mxf8(leads, acc, da + j * 2, db + j * 2, idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
+                }
+                umma_commit(leads, &empty[s]);
+                if ((kb & 3) == 3 || kb == k_blocks - 1) {
+                    umma_commit(leads, &sempty[slot]);
+                    ++group;
+                }
+                if (++s == kStages) {
+                    s = 0;
+                    par ^= 1u;
+                }
             }
+            if (ok) umma_commit(leads, tfull);
         }
     } else if (warp == 2) {
-        // Lane l keeps the scale words of rows l, l + 32, ... of both tiles for four k-blocks.
-        int s = 0;
-        uint32_t par = 0;
+        // A group: the words that cover four k-blocks of the tile's rows, lane l those of rows l, l + 32, ...
+        // Its copies are waited for kScalesAhead groups later.
+        uint32_t sent = 0, done = 0;
         bool ok = true;
-        uint32_t next[12];
-        auto fetch = [&](int64_t t, int kb) {
-            const int64_t m0 = (t % tiles_m) * kTileM, n0 = (t / tiles_m) * kTileN;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int64_t r = m0 + g * 32 + lane;
-                next[g] = r < a.Q ? *reinterpret_cast<const uint32_t*>(a.q_scales + r * scale_pitch + kb) : 0u;
-            }
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                const int64_t r = n0 + g * 32 + lane;
-                next[4 + g] = r < a.n ? *reinterpret_cast<const uint32_t*>(a.scales + r * scale_pitch + kb) : 0u;
-            }
+        auto publish = [&]() {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sfull[done % kScaleSlots]);
+            ++done;
         };
-        if (blockIdx.x < tiles) fetch(blockIdx.x, 0);
-        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            for (int kb0 = 0; kb0 < k_blocks && ok; kb0 += 4) {
-                uint32_t w[12];
+        auto copy = [&](uint32_t dst, const uint8_t* base, int64_t r, int64_t rows, int kb) {
+            const bool there = r < rows;      // else four zero bytes
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst),
+                         "l"(base + (there ? r * scale_pitch + kb : 0)), "r"(there ? 4 : 0)
+                         : "memory");
+        };
+        for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x) {
+            int64_t m0, n0;
+            order.at(t, m0, n0);
+            for (int kb = 0; kb < k_blocks; kb += 4) {
+                const uint32_t slot = sent % kScaleSlots;
+                ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a.err));
+                if (!ok) break;
+                const uint32_t dst = smem_u32(smem + kOffScales + slot * kScaleBytes) + lane * 16;
 #pragma unroll
-                for (int i = 0; i < 12; ++i) w[i] = next[i];
-                if (kb0 + 4 < k_blocks)
-                    fetch(t, kb0 + 4);
-                else if (t + gridDim.x < tiles)
-                    fetch(t + gridDim.x, 0);
-                for (int kb = kb0; kb < min(kb0 + 4, k_blocks); ++kb) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err));
-                    if (!ok) break;
-                    uint4* dst = reinterpret_cast<uint4*>(smem + kOffScales + s * kScaleBytes) + lane;
-                    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                    dst[32] = make_uint4(w[4], w[5], w[6], w[7]);
-                    dst[64] = make_uint4(w[8], w[9], w[10], w[11]);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[s]);
-                    if (++s == kStages) {
-                        s = 0;
-                        par ^= 1u;
-                    }
+                for (int g = 0; g < 4; ++g) copy(dst + g * 4, a.q_scales, m0 + g * 32 + lane, a.Q, kb);
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+                    copy(dst + 512 + (g >> 2) * 512 + (g & 3) * 4, a.scales, n0 + g * 32 + lane, a.n, kb);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (++sent - done > kScalesAhead) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kScalesAhead) : "memory");
+                    publish();
                 }
             }
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        while (ok && done < sent) publish();
     } else if (warp >= 4) {
         const int g = warp & 3, half = (warp - 4) >> 2;      // 32 lanes of tensor memory; which of their two warps
         constexpr int W = 128 / (int)sizeof(T);              // columns of a piece
-        constexpr int kPieces = kTileN / W;
         unsigned char* stage = smem + kOffOut + (warp - 4) * kOutBufs * 4096;
         float* sbias = reinterpret_cast<float*>(smem + kOffBias) + (warp - 4) * (kTileN / 2);
+        constexpr int kTurn = 64, kTurns = kTileN / kTurn / 2;   // columns read at once; turns of a warp
+        const uint32_t leads = elect_leader();
+        uint64_t policy;
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         uint32_t i = 0, sent = 0;
-        for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
-            const int64_t m0 = (t % tiles_m) * kTileM + g * 32, n0 = (t / tiles_m) * kTileN;
-            // pieces in turn from the accumulator's shared columns on: its last 64 or its first 64
+        for (uint32_t t = blockIdx.x; t < order.tiles; t += gridDim.x, ++i) {
+            int64_t m0, n0;
+            order.at(t, m0, n0);
+            m0 += g * 32;
+            const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);      // this warp's, none or fewer past the end
+            // turns from the accumulator's shared columns on: its last 64 or its first 64
             const int start = (i & 1u) ? 0 : kTileN - kShared;
-            const auto col_of = [&](int p) { return (start + p * W) & (kTileN - 1); };
+            const auto col_of = [&](int turn) { return (start + (2 * turn + half) * kTurn) & (kTileN - 1); };
             if (a.bias) {
                 __syncwarp();
 #pragma unroll
-                for (int p = 0; p < kPieces / 2; ++p)
-#pragma unroll
-                    for (int j = 0; j < W; j += 32) {
-                        const int64_t n = n0 + col_of(2 * p + half) + j + lane;
-                        sbias[p * W + j + lane] = n < a.n ? a.bias[n] : 0.f;
-                    }
+                for (int j = 0; j < kTurns * kTurn; j += 32) {
+                    const int64_t n = n0 + col_of(j / kTurn) + j % kTurn + lane;
+                    sbias[j + lane] = n < a.n ? a.bias[n] : 0.f;
+                }
                 __syncwarp();
             }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1u, abort_flag, a.err))) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16) + (i & 1u) * kAccStep;
 #pragma unroll 1
-            for (int p = 0; p < kPieces / 2; ++p) {
-                const int col = col_of(2 * p + half);
-                const bool used = m0 < a.Q && n0 + col < a.n;
-                uint32_t r[W / 32][32];
+            for (int turn = 0; turn < kTurns; ++turn) {
+                const int col0 = col_of(turn);
+                const bool used = rows > 0 && n0 + col0 < a.n;
+                uint32_t r[kTurn / 32][32];
                 if (used) {
-#pragma unroll
-                    for (int w = 0; w < W / 32; ++w) tmem_ld32(acc + (uint32_t)(col + w * 32), r[w]);
+                    tmem_ld32(acc + (uint32_t)col0, r[0]);
+                    tmem_ld32(acc + (uint32_t)col0 + 32, r[1]);
                     tmem_ld_wait();
                 }
-                if (p == 0) {      // the shared columns are the first pieces of the two warps
+                if (turn == 0) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(tfree);
                 }
                 if (!used) continue;
 #pragma unroll
-                for (int j = 0; j < W; j += 4) {
-                    const float4 b = a.bias ? *reinterpret_cast<const float4*>(sbias + p * W + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    uint32_t* x = &r[j / 32][j % 32];
-                    x[0] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[0]), b.x));
-                    x[1] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[1]), b.y));
-                    x[2] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[2]), b.z));
-                    x[3] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[3]), b.w));
-                }
-                if (TMA_OUT) {
-                    unsigned char* buf = stage + (sent++ % kOutBufs) * 4096;
-                    // the piece that used this buffer has left shared memory
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kOutBufs - 1) : "memory");
-                    __syncwarp();
+                for (int p = 0; p < kTurn / W; ++p) {
+                    const int col = col0 + p * W;
+                    if (n0 + col >= a.n) continue;
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        uint4 x;
-                        if (sizeof(T) == 4) {
-                            x = make_uint4(r[0][4 * u], r[0][4 * u + 1], r[0][4 * u + 2], r[0][4 * u + 3]);
-                        } else {
-                            const uint32_t* y = &r[(W / 32 - 1) * u / 4][8 * u % 32];
-                            x = make_uint4(pack2<T>(__uint_as_float(y[0]), __uint_as_float(y[1])),
-                                           pack2<T>(__uint_as_float(y[2]), __uint_as_float(y[3])),
-                                           pack2<T>(__uint_as_float(y[4]), __uint_as_float(y[5])),
-                                           pack2<T>(__uint_as_float(y[6]), __uint_as_float(y[7])));
-                        }
-                        *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = x;
+                    for (int j = 0; j < W; j += 4) {
+                        uint32_t* x = &r[(p * W + j) / 32][(p * W + j) % 32];
+                        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (a.bias) b = *reinterpret_cast<const float4*>(sbias + turn * kTurn + p * W + j);
+                        x[0] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[0]), b.x));
+                        x[1] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[1]), b.y));
+                        x[2] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[2]), b.z));
+                        x[3] = __float_as_uint(fmaf(a.alpha, __uint_as_float(x[3]), b.w));
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) tma_store_2d(&map_out, (int)(n0 + col), (int)m0, buf);
-                } else {
-                    float* tile = reinterpret_cast<float*>(stage);      // column j of row l at l * 32 + (j ^ l)
-                    const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);
-#pragma unroll
-                    for (int w = 0; w < W / 32; ++w) {
+                    if (TMA_OUT) {
+                        constexpr int E = 16 / (int)sizeof(T);
+                        unsigned char* buf = stage + sent++ % kOutBufs * 4096;
+                        // the piece that used this buffer has left shared memory
+                        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kOutBufs - 1) : "memory");
                         __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = __uint_as_float(r[w][j]);
+                        for (int u = 0; u < 8; ++u) {
+                            uint4 x;
+                            const uint32_t* y = &r[(p * W + u * E) / 32][(p * W + u * E) % 32];
+                            if (sizeof(T) == 4)
+                                x = make_uint4(y[0], y[1], y[2], y[3]);
+                            else
+                                x = make_uint4(pack2<T>(__uint_as_float(y[0]), __uint_as_float(y[1])),
+                                               pack2<T>(__uint_as_float(y[2]), __uint_as_float(y[3])),
+                                               pack2<T>(__uint_as_float(y[E - 4]), __uint_as_float(y[E - 3])),
+                                               pack2<T>(__uint_as_float(y[E - 2]), __uint_as_float(y[E - 1])));
+                            *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = x;
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
-                        const int64_t n = n0 + col + w * 32 + lane;
-                        if (n < a.n) {
-                            T* out = static_cast<T*>(a.out) + m0 * a.ld + n;
+                        tma_store_2d(leads, &map_out, (int)(n0 + col), (int)m0, buf, policy);
+                    } else {
+                        float* tile = reinterpret_cast<float*>(stage);      // column j of row l at l * 32 + (j ^ l)
+#pragma unroll
+                        for (int w = 0; w < W / 32; ++w) {
+                            __syncwarp();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = __uint_as_float(r[p * W / 32 + w][j]);
+                            __syncwarp();
+                            const int64_t n = n0 + col + w * 32 + lane;
+                            if (n < a.n) {
+                                T* out = static_cast<T*>(a.out) + m0 * a.ld + n;
 #pragma unroll 4
-                            for (int j = 0; j < rows; ++j) out[j * a.ld] = narrow<T>(tile[j * 32 + (lane ^ j)]);
+                                for (int j = 0; j < rows; ++j) out[j * a.ld] = narrow<T>(tile[j * 32 + (lane ^ j)]);
+                            }
                         }
                     }
                 }
             }
         }
-        if (TMA_OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (TMA_OUT) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
     }
 
@@ -622,8 +689,11 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     // tensor stores need rows that start at 16-byte boundaries
     const bool tma = ((uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T))) % 16 == 0;
+    // rows of a query tile that are loaded: the others' products are not stored, whatever they are
+    // (a row outside the matrix costs the tensor copy more than one inside it)
+    const int a_rows = a.Q >= kTileM ? kTileM : (a.Q + 7) / 8 * 8;
     alignas(64) CUtensorMap map_a, map_b, map_out;
-    if (!matrix_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q_codes, a.Q, a.dim, fp8_code_pitch(a.dim), kTileK, kTileM,
+    if (!matrix_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q_codes, a.Q, a.dim, fp8_code_pitch(a.dim), kTileK, a_rows,
                     CU_TENSOR_MAP_SWIZZLE_128B) ||
         !matrix_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.n, a.dim, fp8_code_pitch(a.dim), kTileK, kTileN,
                     CU_TENSOR_MAP_SWIZZLE_128B))
@@ -636,10 +706,15 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     auto kernel = tma ? fp8_scores_kernel<T, true> : fp8_scores_kernel<T, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return e;
-    const int tiles_m = (a.Q + kTileM - 1) / kTileM;
-    const int64_t tiles = (int64_t)tiles_m * ((a.n + kTileN - 1) / kTileN);
-    const int grid = (int)(tiles < sm_count ? tiles : sm_count);
-    kernel<<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, map_out, a, tiles_m, tiles);
+    TileOrder order;
+    order.tiles_m = (uint32_t)(((int64_t)a.Q + kTileM - 1) / kTileM);
+    order.tiles_n = (uint32_t)(((int64_t)a.n + kTileN - 1) / kTileN);
+    order.tiles = order.tiles_m * order.tiles_n;
+    const int64_t in_l2 = kChunkBytes / (kTileN * fp8_code_pitch(a.dim));
+    order.chunk_n = (uint32_t)(in_l2 < sm_count ? sm_count : in_l2);
+    if (order.chunk_n > order.tiles_n) order.chunk_n = order.tiles_n;
+    const int grid = (int)(order.tiles < (uint32_t)sm_count ? order.tiles : sm_count);
+    kernel<<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, map_out, a, order, a_rows);
     return cudaGetLastError();
 }
 
