@@ -7,8 +7,9 @@
 //
 // A CTA owns kCols columns of one row.  Its own scores and mask words are requested first and stay in
 // flight while it turns the row's two id lists into tables over its columns in shared memory: counts
-// by integer atomics (their order does not show), biases by one warp in list order.  Then it applies
-// the rules and stores.  No table in global memory, nothing to clear between calls, one launch.  The
+// by integer atomics (their order does not show), biases by one warp in list order, and one bit for
+// every column that either list touches: a thread whose columns are untouched reads one word of bits
+// and no table.  Then it applies the rules and stores.  No table in global memory, nothing to clear between calls, one launch.  The
 // history is read once per CTA, from L2: wider columns would read it less often but leave fewer CTAs
 // an SM, and latency, not that traffic, is what a CTA waits for.
 #include <math_constants.h>
@@ -49,6 +50,7 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
     const bool has_seen = a.n_seen > 0, has_bias = a.n_bias > 0;
     uint32_t* count = reinterpret_cast<uint32_t*>(smem);
     float* bias = reinterpret_cast<float*>(smem) + (has_seen ? kCols : 0);
+    uint32_t* touched = reinterpret_cast<uint32_t*>(smem) + kCols * ((has_seen ? 1 : 0) + (has_bias ? 1 : 0));
 
     // the thread's scores: U vectors of V, vector u at column (u * kThreads + tid) * V
     constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
@@ -80,21 +82,28 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
 
     float rho = 1.f, phi = 0.f, pi = 0.f;
     if (has_seen || has_bias) {
+        const int32_t* seen = has_seen ? a.seen + (size_t)q * a.n_seen : nullptr;
+        constexpr int kAhead = 8;      // ids of the history in flight while the tables are cleared
+        int32_t ids_ahead[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ids_ahead[i] = i * kThreads + tid < a.n_seen ? seen[i * kThreads + tid] : -1;
         if (has_seen) {
             rho = a.penalties[(size_t)q * 3];
             phi = a.penalties[(size_t)q * 3 + 1];
             pi = a.penalties[(size_t)q * 3 + 2];
         }
-        const int words = kCols * ((has_seen ? 1 : 0) + (has_bias ? 1 : 0));
+        const int words = (int)(touched - count) + kCols / 32;
         for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         if (has_seen) {
-            const int32_t* seen = a.seen + (size_t)q * a.n_seen;
+            auto add = [&](int32_t id) {
+                const int64_t j = (int64_t)id - c0;
+                if (j >= 0 && j < cols && atomicAdd(&count[j], 1u) == 0u) atomicOr(&touched[j >> 5], 1u << (j & 31));
+            };
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) add(ids_ahead[i]);
 #pragma unroll 4
-            for (int i = tid; i < a.n_seen; i += kThreads) {
-                const int64_t j = (int64_t)seen[i] - c0;
-                if (j >= 0 && j < cols) atomicAdd(&count[j], 1u);
-            }
+            for (int i = kAhead * kThreads + tid; i < a.n_seen; i += kThreads) add(seen[i]);
         }
         if (has_bias && tid < 32) {
             const int32_t* ids = a.bias_ids + (size_t)q * a.n_bias;
@@ -102,24 +111,24 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
             for (int i0 = 0; i0 < a.n_bias; i0 += 32) {
                 const int i = i0 + lane;
                 const int64_t j = i < a.n_bias ? (int64_t)ids[i] - c0 : -1;
-                const bool mine = j >= 0 && j < cols;
-                const float val = mine ? vals[i] : 0.f;
-                // entries of one id: its first lane sums them, in list order, onto what earlier ones left
-                const uint32_t same = __match_any_sync(0xffffffffu, mine ? (int)j : -1 - lane);
-                const bool leads = mine && (same & ((1u << lane) - 1u)) == 0u;
-                float s = leads ? bias[j] : 0.f;
-                for (uint32_t p = 0; p < 32; ++p) {
-                    const float x = __shfl_sync(0xffffffffu, val, p);
-                    if (same >> p & 1u) s += x;
+                uint32_t todo = __ballot_sync(0xffffffffu, j >= 0 && j < cols);
+                if (!todo) continue;
+                const float val = i < a.n_bias ? vals[i] : 0.f;
+                for (; todo; todo &= todo - 1) {      // in list order
+                    const int src = __ffs(todo) - 1;
+                    const int at = __shfl_sync(0xffffffffu, (int)j, src);
+                    const float x = __shfl_sync(0xffffffffu, val, src);
+                    if (lane == 0) {
+                        bias[at] += x;
+                        atomicOr(&touched[at >> 5], 1u << (at & 31));
+                    }
                 }
-                if (leads) bias[j] = s;
-                __syncwarp();
             }
         }
         __syncthreads();
     }
 
-    auto rule = [&](float s, int j, bool out_of) {
+    auto rule = [&](float s, int j) {
         if (has_seen) {
             const uint32_t c = count[j];
             if (c) {
@@ -131,20 +140,29 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
             const float b = bias[j];
             if (b != 0.f) s += b;
         }
-        return from_f32<T>(out_of ? -CUDART_INF_F : s);
+        return s;
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int j = (u * kThreads + tid) * V;
-        if (VEC && j + V <= cols) {
-            alignas(16) T w[V];
+        uint32_t hit = 0;
+        if ((has_seen || has_bias) && j < cols) hit = touched[j >> 5] >> (j & 31) & kAll & ~m[u];
+        if (hit) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) w[i] = rule(to_f32<T>(v[u][i]), j + i, m[u] >> i & 1u);
-            *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<uint4*>(w);
+            for (int i = 0; i < V; ++i)
+                if (hit >> i & 1u) v[u][i] = from_f32<T>(rule(to_f32<T>(v[u][i]), j + i));
+        }
+        if (m[u]) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (m[u] >> i & 1u) v[u][i] = from_f32<T>(-CUDART_INF_F);
+        }
+        if (VEC && j + V <= cols) {
+            *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<uint4*>(v[u]);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (j + i < cols) out[j + i] = rule(to_f32<T>(v[u][i]), j + i, m[u] >> i & 1u);
+                if (j + i < cols) out[j + i] = v[u][i];
         }
     }
 }
@@ -152,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
 template <typename T>
 cudaError_t launch_rules(const RulesArgs& a, cudaStream_t stream) {
     const int64_t chunks = (a.n + kCols - 1) / kCols;
-    const size_t smem = (size_t)kCols * 4 * ((a.n_seen > 0) + (a.n_bias > 0));
+    const size_t smem = (size_t)kCols * 4 * ((a.n_seen > 0) + (a.n_bias > 0)) + kCols / 8;
     const bool vec = ((uintptr_t)a.in | (uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T)) |
                       (uintptr_t)(a.ld_out * sizeof(T))) % 16 == 0;
     auto kernel = vec ? score_rules_kernel<T, true> : score_rules_kernel<T, false>;
