@@ -8,15 +8,17 @@
 // barrier, the running maxima of fixed groups of columns (a thread's, or quarters of a thread's); the
 // k-th largest of these maxima, rounded down to 16 bits, is a lower bound of the k-th best score.  The
 // second reads the slice again, from L2 (slices are sized so that those at work fit), and collects what
-// reaches the bound: k scores and a few more, unless many are equal.  A slice of one tile stays in
-// registers between the passes.  If the buffer in shared memory overflows all the same, the slice is
-// streamed a third time, the buffer cut to its k best by a radix selection (8-bit digits, from the top)
-// whenever it might not take another tile; columns arrive in ascending order, so a score equal to the
-// k-th has a higher id than the k keys it would have to beat and loses.
+// reaches the bound: k scores and a few more, unless many are equal.  It only notes the 16-byte vectors
+// that hold such a score; the whole CTA then takes the noted ones apart at once.  A slice of one step (128 bytes a
+// thread, all in flight at once) stays in registers between the passes.  If the buffer in shared memory
+// overflows all the same, the second pass is repeated with the buffer cut to its k best by a radix
+// selection (8-bit digits, from the top) whenever it might not take what comes next; columns arrive in
+// ascending order, so a score equal to the k-th has a higher id than the k keys it would have to beat
+// and loses.
 //
-// Rows are cut into slices while there are fewer rows than CTAs to keep busy.  The k best of each
-// slice then meet in a second launch, which selects among keys in the same way; it is launched before
-// the first ends (programmatic dependent launch) and waits for it on the device.
+// Rows are cut into slices while there are fewer rows than CTAs to keep busy.  What the slices collect
+// then meets in a second launch, which finds its bound among keys in the same way; it is launched
+// before the first ends (programmatic dependent launch) and waits for it on the device.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -28,15 +30,18 @@ namespace coral {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kTile = 8192;                 // scores per step of a CTA
-constexpr int kCap = kTile + kTopkMax;      // keys held in shared memory
+constexpr int kRoom = 8192;                 // keys that may arrive between two looks at the buffer
+constexpr int kCap = kRoom + kTopkMax;      // keys held in shared memory
+constexpr int kNotes = 4096;                // vectors noted
 constexpr int64_t kSliceBytes = 256 << 10;  // what two CTAs on every SM read twice fits L2
 
 struct Shared {
     uint64_t keys[kCap];
+    uint32_t notes[kNotes];
     uint32_t hist[256];
-    int cnt;
+    int cnt, noted;
     int digit, above;     // the selection's current digit, keys above it
+    uint32_t top;         // the largest maximum
     float least;          // scores below it cannot be among the k best
 };
 
@@ -86,13 +91,13 @@ __device__ __forceinline__ void pick_digit(Shared& sh, int want) {
 }
 
 template <typename T>
-__device__ __forceinline__ T lowest_of();      // -inf
+__device__ __forceinline__ T from_bits(uint32_t b);
 template <>
-__device__ __forceinline__ float lowest_of<float>() { return -CUDART_INF_F; }
+__device__ __forceinline__ float from_bits<float>(uint32_t b) { return __uint_as_float(b); }
 template <>
-__device__ __forceinline__ __nv_bfloat16 lowest_of<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+__device__ __forceinline__ __nv_bfloat16 from_bits<__nv_bfloat16>(uint32_t b) { return __ushort_as_bfloat16((unsigned short)b); }
 template <>
-__device__ __forceinline__ __half lowest_of<__half>() { return __ushort_as_half(0xfc00); }
+__device__ __forceinline__ __half from_bits<__half>(uint32_t b) { return __ushort_as_half((unsigned short)b); }
 
 // The larger of each of two pairs of 16-bit scores (NaN counts as nothing), and of the two of one.
 template <typename T>
@@ -115,7 +120,7 @@ __device__ __forceinline__ float max_of(uint32_t m) {
 
 // Cuts sh.keys[0..cnt) to its k largest (any order); all threads call it, cnt > k, keys distinct.
 // Leaves k in sh.cnt and, in sh.least, the value just above the k-th largest's score.
-__device__ void select_k(Shared& sh, int k) {
+__device__ __noinline__ void select_k(Shared& sh, int k) {
     const int tid = threadIdx.x, cnt = sh.cnt;
     uint64_t prefix = 0;          // digits of the k-th largest key found so far
     int want = k;                 // it is the want-th largest of the keys that share them
@@ -162,35 +167,34 @@ __device__ void select_k(Shared& sh, int k) {
     __syncthreads();
 }
 
-// Writes the row's result, the k best of sh.keys[0..cnt): bitonic sort, descending.
+// Writes the row's result, the k best of sh.keys[0..cnt), in order.
 __device__ void finish_row(Shared& sh, int q, const TopkArgs& a) {
     const int tid = threadIdx.x;
     if (sh.cnt > a.k && sh.cnt > 1024) select_k(sh, a.k);
     const int cnt = sh.cnt;
+    auto write = [&](int rank, uint64_t key) {
+        a.ids_out[(size_t)q * a.k + rank] = key ? (int32_t)~(uint32_t)key + a.id_base : -1;
+        a.scores_out[(size_t)q * a.k + rank] = key ? score_of_key(key) : -3.402823466e+38f;
+    };
     int n2 = 32;
     while (n2 < cnt) n2 <<= 1;
-    if (n2 <= kThreads) {      // a key a thread: partners nearer than a warp by shuffles
-        uint64_t key = tid < cnt ? sh.keys[tid] : 0;
-        for (int w = 2; w <= n2; w <<= 1)
-            for (int j = w >> 1; j > 0; j >>= 1) {
-                uint64_t other;
-                if (j >= 32) {
-                    __syncthreads();
-                    sh.keys[tid] = key;
-                    __syncthreads();
-                    other = sh.keys[tid ^ j];
-                } else {
-                    other = __shfl_xor_sync(0xffffffffu, key, j);
-                }
-                const bool larger = ((tid & j) == 0) == ((tid & w) == 0);
-                key = (key > other) == larger ? key : other;
-            }
+    if (n2 <= kThreads) {
+        // a key's place is the number of larger keys; kThreads / n2 threads share the count of one
+        const int mine = tid & (n2 - 1), part = tid / n2, parts = kThreads / n2;
+        if (tid < n2) sh.notes[tid] = 0;
+        const uint64_t key = mine < cnt ? sh.keys[mine] : 0;
+        const int from = cnt * part / parts, to = cnt * (part + 1) / parts;
+        int larger = 0;
+#pragma unroll 8
+        for (int i = from; i < to; ++i) larger += sh.keys[i] > key ? 1 : 0;
         __syncthreads();
-        sh.keys[tid] = key;
+        if (key) atomicAdd(&sh.notes[mine], (uint32_t)larger);
+        __syncthreads();
+        if (part == 0 && key && sh.notes[mine] < (uint32_t)a.k) write((int)sh.notes[mine], key);
     } else {
         for (int i = cnt + tid; i < n2; i += kThreads) sh.keys[i] = 0;
         __syncthreads();
-        for (int w = 2; w <= n2; w <<= 1)
+        for (int w = 2; w <= n2; w <<= 1)      // bitonic, descending
             for (int j = w >> 1; j > 0; j >>= 1) {
                 for (int i = tid; i < n2; i += kThreads) {
                     const int p = i ^ j;
@@ -204,41 +208,87 @@ __device__ void finish_row(Shared& sh, int q, const TopkArgs& a) {
                 }
                 __syncthreads();
             }
+        for (int i = tid; i < min(cnt, a.k); i += kThreads) write(i, sh.keys[i]);
     }
-    __syncthreads();
-    for (int i = tid; i < a.k; i += kThreads) {
-        const bool there = i < cnt;
-        const uint64_t key = there ? sh.keys[i] : 0;
-        a.ids_out[(size_t)q * a.k + i] = there ? (int32_t)~(uint32_t)key + a.id_base : -1;
-        a.scores_out[(size_t)q * a.k + i] = there ? score_of_key(key) : -3.402823466e+38f;
-    }
+    for (int i = cnt + tid; i < a.k; i += kThreads) write(i, 0);
 }
 
-// One tile in registers: U vectors of V scores a thread, vector u at column t0 + (u * kThreads + tid) * V.
-// What lies past the slice's end reads -inf.
-template <typename T, bool VEC>
-struct Tile {
-    static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-    static constexpr int U = kTile / (kThreads * V);
-    alignas(16) T v[U][V];
+// Leaves in sh.least a lower bound of the k-th best score, from the maxima of disjoint groups of scores:
+// o[0..4) are the high halves of the orders of four groups' maxima.  Bins of a histogram count maxima
+// by their distance from the largest, at full resolution first, where nearly always at least k of them
+// lie within its 255 bins, else 16 and 256 times coarser.
+__device__ __forceinline__ void lower_bound_of_kth(Shared& sh, const uint32_t (&o)[4], int k) {
+    const int tid = threadIdx.x;
+    const uint32_t top = max(max(o[0], o[1]), max(o[2], o[3]));
+    const bool by_thread = k <= kThreads / 2;      // else the quarters are needed
+    if (tid == 0) sh.top = 0;
+    if (tid < 256) sh.hist[tid] = 0;
+    __syncthreads();
+    const uint32_t warp_top = __reduce_max_sync(0xffffffffu, top);
+    if ((tid & 31) == 0) atomicMax(&sh.top, warp_top);
+    __syncthreads();
+    const uint32_t hi = sh.top;
+    uint32_t bound = 0;
+    for (int shift = 0; shift <= 8; shift += 4) {
+        if (by_thread) {
+            const uint32_t d = (hi - top) >> shift;
+            if (d < 255) atomicAdd(&sh.hist[255 - d], 1u);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const uint32_t d = (hi - o[g]) >> shift;
+                if (d < 255) atomicAdd(&sh.hist[255 - d], 1u);
+            }
+        }
+        if (tid == 0) sh.digit = 0;
+        __syncthreads();
+        if (tid < 32) pick_digit(sh, k);
+        __syncthreads();
+        const int digit = sh.digit;
+        if (digit) {
+            const uint32_t below = (uint32_t)(256 - digit) << shift;      // everything in the bin is nearer than this
+            bound = hi >= below ? hi - below + 1 : 0;
+            break;
+        }
+        if (tid < 256) sh.hist[tid] = 0;
+        __syncthreads();
+    }
+    // never below the lowest finite score: -inf is not chosen
+    if (tid == 0) sh.least = bound <= ord_of(-3.402823466e+38f) >> 16 ? -3.402823466e+38f : of_ord(bound << 16);
+    __syncthreads();
+}
 
-    __device__ __forceinline__ void load(const T* row, int64_t t0, int64_t c1) {
+// One step in registers: U vectors of V scores a thread, vector u at column t0 + (u * kThreads + tid) * V
+// of the slice.
+// What lies past the end reads -inf; with vectors, the end is a multiple of V.
+template <typename T, bool VEC>
+struct Step {
+    static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    static constexpr int U = 8;
+    static constexpr int kScores = kThreads * U * V;
+    static constexpr bool kPairs = VEC && sizeof(T) == 2;
+    union {
+        uint4 raw[VEC ? U : 1];
+        T v[U][V];
+    };
+
+    __device__ __forceinline__ Step() {}
+    __device__ __forceinline__ void load(const T* cols, int t0, int end) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t j = t0 + (u * kThreads + threadIdx.x) * V;
-            if (VEC && j + V <= c1) {
-                *reinterpret_cast<uint4*>(v[u]) = *reinterpret_cast<const uint4*>(row + j);
+            const int j = t0 + (u * kThreads + (int)threadIdx.x) * V;
+            if constexpr (VEC) {
+                const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+                raw[u] = make_uint4(none, none, none, none);
+                if (j < end) raw[u] = *reinterpret_cast<const uint4*>(cols + j);
             } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[u][i] = j + i < c1 ? row[j + i] : lowest_of<T>();
+                v[u][0] = j < end ? cols[j] : from_bits<T>(sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u);
             }
         }
     }
     __device__ __forceinline__ float best(int u) const {     // NaN counts as nothing
-        if constexpr (VEC && sizeof(T) == 2) {
-            const uint4 x = *reinterpret_cast<const uint4*>(v[u]);
-            const uint32_t m = max2<T>(max2<T>(x.x, x.y), max2<T>(x.z, x.w));
-            return max_of<T>(m);
+        if constexpr (kPairs) {
+            return max_of<T>(max2<T>(max2<T>(raw[u].x, raw[u].y), max2<T>(raw[u].z, raw[u].w)));
         } else {
             float m = -CUDART_INF_F;
 #pragma unroll
@@ -246,181 +296,177 @@ struct Tile {
             return m;
         }
     }
-    // appends what reaches `least`; positions from kCap on are counted but not written
-    __device__ __forceinline__ void collect(Shared& sh, float least, int64_t t0) const {
+    __device__ __forceinline__ uint32_t reaching(float least) const {      // bit u: vector u holds such a score
+        uint32_t hits = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (best(u) >= least) {
-                const int64_t j = t0 + (u * kThreads + threadIdx.x) * V;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float s = score_of<T>(v[u][i]);
-                    if (s >= least) {
-                        const int at = atomicAdd(&sh.cnt, 1);
-                        if (at < kCap) sh.keys[at] = key_of(s, (uint32_t)(j + i));
-                    }
-                }
-            }
+        for (int u = 0; u < U; ++u) hits |= best(u) >= least ? 1u << u : 0u;
+        return hits;
     }
 };
 
-// Running maxima of four groups of a thread's columns: quarter g of its 16 scores of every tile.
-template <typename T, bool VEC>
-struct Maxima {
-    static constexpr bool kPacked = VEC && sizeof(T) == 2;
-    float m[kPacked ? 1 : 4];
-    uint32_t p[kPacked ? 4 : 1];
-
-    __device__ __forceinline__ Maxima() {
-        if constexpr (kPacked) {
-            const uint32_t none = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) p[g] = none;
-        } else {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) m[g] = -CUDART_INF_F;
-        }
-    }
-    __device__ __forceinline__ void add(const Tile<T, VEC>& t) {
-        if constexpr (kPacked) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint4 x = *reinterpret_cast<const uint4*>(t.v[u]);
-                p[2 * u] = max2<T>(p[2 * u], max2<T>(x.x, x.y));
-                p[2 * u + 1] = max2<T>(p[2 * u + 1], max2<T>(x.z, x.w));
-            }
-        } else {
-            constexpr int V = Tile<T, VEC>::V;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) m[e / 4] = fmaxf(m[e / 4], score_of<T>(t.v[e / V][e % V]));
-        }
-    }
-    __device__ __forceinline__ float group(int g) const {
-        if constexpr (kPacked)
-            return max_of<T>(p[g]);
-        else
-            return m[g];
-    }
-};
-
-// Leaves in sh.least a lower bound of the k-th best score, from the maxima of all groups: the k-th
-// largest, with the low 16 bits of its order cleared.  Two 8-bit digits of a radix selection.
-template <typename T, bool VEC>
-__device__ void first_threshold(Shared& sh, const Maxima<T, VEC>& maxima, int k) {
-    const int tid = threadIdx.x;
-    uint32_t o[4], top = 0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        o[g] = ord_of(maxima.group(g)) >> 16;
-        top = max(top, o[g]);
-    }
-    const bool by_thread = k <= kThreads / 2;
-    int want = k;
-    uint32_t prefix = 0;
-    for (int shift = 8; shift >= 0; shift -= 8) {
-        if (tid < 256) sh.hist[tid] = 0;
-        __syncthreads();
-        if (by_thread) {
-            if (shift == 8 || top >> 8 == prefix) atomicAdd(&sh.hist[(top >> shift) & 255], 1u);
-        } else {
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                if (shift == 8 || o[g] >> 8 == prefix) atomicAdd(&sh.hist[(o[g] >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid < 32) pick_digit(sh, want);
-        __syncthreads();
-        prefix = prefix << 8 | (uint32_t)sh.digit;
-        want -= sh.above;
-        __syncthreads();
-    }
-    // never below the lowest finite score: -inf is not chosen
-    if (tid == 0) sh.least = prefix <= ord_of(-3.402823466e+38f) >> 16 ? -3.402823466e+38f : of_ord(prefix << 16);
-    __syncthreads();
+__device__ __forceinline__ void append(Shared& sh, float s, uint32_t col) {      // counted, but not written, from kCap on
+    const int at = atomicAdd(&sh.cnt, 1);
+    if (at < kCap) sh.keys[at] = key_of(s, col);
 }
 
+// Notes the flagged vectors of a step by number; counted, but not written, from kNotes on.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice) {
+__device__ __forceinline__ void note(Shared& sh, uint32_t hits, int t0) {
+    for (; hits; hits &= hits - 1) {
+        const int at = atomicAdd(&sh.noted, 1);
+        if (at < kNotes) sh.notes[at] = t0 / Step<T, VEC>::V + (__ffs(hits) - 1) * kThreads + threadIdx.x;
+    }
+}
+
+// Appends the scores that reach `least` of the noted vectors, an element a thread.
+template <typename T, bool VEC>
+__device__ __forceinline__ void collect(Shared& sh, int noted, float least, const T* cols, uint32_t c0) {
+    constexpr int V = Step<T, VEC>::V;
+    for (int i = threadIdx.x; i < noted * V; i += kThreads) {
+        const int j = (int)sh.notes[i / V] * V + i % V;
+        const float s = score_of<T>(cols[j]);
+        if (s >= least) append(sh, s, c0 + (uint32_t)j);
+    }
+}
+
+// Running maxima of four groups of a thread's columns: vectors g and g + 4 (g, g + 4, ...) of every step.
+template <typename T, bool VEC>
+struct Maxima {
+    static constexpr bool kPairs = Step<T, VEC>::kPairs;
+    float m[4];
+    uint32_t p[4];
+
+    __device__ __forceinline__ Maxima() {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            m[g] = -CUDART_INF_F;
+            p[g] = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        }
+    }
+    __device__ __forceinline__ void add(const Step<T, VEC>& t) {
+#pragma unroll
+        for (int u = 0; u < Step<T, VEC>::U; ++u) {
+            if constexpr (kPairs)
+                p[u & 3] = max2<T>(p[u & 3], max2<T>(max2<T>(t.raw[u].x, t.raw[u].y), max2<T>(t.raw[u].z, t.raw[u].w)));
+            else
+                m[u & 3] = fmaxf(m[u & 3], t.best(u));
+        }
+    }
+    __device__ __forceinline__ uint32_t high(int g) const { return ord_of(kPairs ? fmaxf(m[g], max_of<T>(p[g])) : m[g]) >> 16; }
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2)
+topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice, const int slots) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem);
+    using Scores = Step<T, VEC>;
     const int tid = threadIdx.x;
     const int q = blockIdx.x / splits, part = blockIdx.x % splits;
+    // columns [c0, c0 + len) of the row; whole vectors end at `end`, what is left takes a thread each
     const int64_t c0 = part * slice;
-    const int64_t c1 = c0 + slice < a.n ? c0 + slice : a.n;
-    const T* row = static_cast<const T*>(a.in) + (size_t)q * a.ld;
+    const int len = c0 < a.n ? (int)(c0 + slice < a.n ? slice : a.n - c0) : 0, end = len - len % Scores::V;
+    const T* cols = static_cast<const T*>(a.in) + (size_t)q * a.ld + c0;
     if (splits > 1) cudaTriggerProgrammaticLaunchCompletion();
-    if (tid == 0) sh.cnt = 0;
-    Tile<T, VEC> tile;
-    if (c1 - c0 <= kTile) {
-        tile.load(row, c0, c1);
-        Maxima<T, VEC> maxima;
-        maxima.add(tile);
-        first_threshold(sh, maxima, a.k);
-        tile.collect(sh, sh.least, c0);
-    } else {
-        Maxima<T, VEC> maxima;
-#pragma unroll 2
-        for (int64_t t0 = c0; t0 < c1; t0 += kTile) {
-            tile.load(row, t0, c1);
-            maxima.add(tile);
-        }
-        first_threshold(sh, maxima, a.k);
-        const float least = sh.least;
-#pragma unroll 2
-        for (int64_t t0 = c0; t0 < c1; t0 += kTile) {
-            tile.load(row, t0, c1);
-            tile.collect(sh, least, t0);
-        }
+    if (tid == 0) sh.cnt = sh.noted = 0;
+    const bool has_rest = end + tid < len;
+    const float rest = has_rest ? score_of<T>(cols[end + tid]) : -CUDART_INF_F;
+    Scores step;
+    Maxima<T, VEC> maxima;
+    for (int t0 = 0; t0 < end; t0 += Scores::kScores) {
+        step.load(cols, t0, end);
+        maxima.add(step);
+    }
+    maxima.m[0] = fmaxf(maxima.m[0], rest);
+    const uint32_t high[4] = {maxima.high(0), maxima.high(1), maxima.high(2), maxima.high(3)};
+    lower_bound_of_kth(sh, high, a.k);
+    const float bound = sh.least;
+    const bool in_registers = end <= Scores::kScores;
+    for (int t0 = 0; t0 < end; t0 += Scores::kScores) {
+        if (!in_registers) step.load(cols, t0, end);
+        note<T, VEC>(sh, step.reaching(bound), t0);
+    }
+    __syncthreads();
+    const int noted = sh.noted;
+    if (noted <= kNotes) collect<T, VEC>(sh, noted, bound, cols, (uint32_t)c0);
+    if (has_rest && rest >= bound) append(sh, rest, (uint32_t)(c0 + end + tid));
+    __syncthreads();
+    if (noted > kNotes || sh.cnt > kCap) {
+        // many equal scores: a vector a thread at a time, the buffer cut whenever the next might not fit
         __syncthreads();
-        if (sh.cnt > kCap) {      // many equal scores
-            __syncthreads();
-            if (tid == 0) sh.cnt = 0;
-            __syncthreads();
-            for (int64_t t0 = c0; t0 < c1; t0 += kTile) {
-                tile.load(row, t0, c1);
-                tile.collect(sh, sh.least, t0);
-                __syncthreads();
-                const int cnt = sh.cnt;
-                if (cnt > kCap - kTile) select_k(sh, a.k);     // no room for another tile
-                else __syncthreads();
+        if (tid == 0) sh.cnt = 0;
+        __syncthreads();
+        for (int t0 = 0; t0 < len; t0 += kThreads * Scores::V) {
+            const float least = sh.least;
+            for (int i = 0; i < Scores::V; ++i) {
+                const int j = t0 + tid * Scores::V + i;
+                const float s = j < len ? score_of<T>(cols[j]) : -CUDART_INF_F;
+                if (s >= least) append(sh, s, (uint32_t)(c0 + j));
             }
+            __syncthreads();
+            const int cnt = sh.cnt;
+            __syncthreads();
+            if (cnt > kCap - kRoom) select_k(sh, a.k);
         }
     }
     __syncthreads();
     if (splits == 1) {
         finish_row(sh, q, a);
     } else {
-        if (sh.cnt > a.k) select_k(sh, a.k);
-        uint64_t* mine = a.ws + ((size_t)q * splits + part) * a.k;
-        for (int i = tid; i < a.k; i += kThreads) mine[i] = i < sh.cnt ? sh.keys[i] : 0;
+        if (sh.cnt > slots) select_k(sh, a.k);
+        uint64_t* mine = a.ws + ((size_t)q * splits + part) * slots;
+        for (int i = tid; i < slots; i += kThreads) mine[i] = i < sh.cnt ? sh.keys[i] : 0;
     }
 }
 
-__global__ void __launch_bounds__(kThreads) topk_join_kernel(const TopkArgs a, const int splits) {
+__global__ void __launch_bounds__(kThreads) topk_join_kernel(const TopkArgs a, const int splits, const int slots) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem);
     const int tid = threadIdx.x, q = blockIdx.x;
-    const int total = splits * a.k;
+    const int total = splits * slots;
     const uint64_t* keys = a.ws + (size_t)q * total;
     if (tid == 0) sh.cnt = 0;
-    __syncthreads();
     cudaGridDependencySynchronize();
-    for (int t0 = 0; t0 < total; t0 += kTile) {
-        for (int i = t0 + tid; i < min(total, t0 + kTile); i += kThreads) {
-            const uint64_t key = keys[i];
-            if (key != 0) sh.keys[atomicAdd(&sh.cnt, 1)] = key;
+    uint32_t high[4] = {0, 0, 0, 0};
+#pragma unroll 2
+    for (int i = tid; i < total; i += 4 * kThreads)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (i + g * kThreads < total) high[g] = max(high[g], (uint32_t)(keys[i + g * kThreads] >> 48));
+    lower_bound_of_kth(sh, high, a.k);
+    const uint32_t least = ord_of(sh.least);
+    for (int careful = 0; careful < 2; ++careful) {
+        for (int i0 = 0; i0 < total; i0 += kRoom) {
+            for (int i = i0 + tid; i < min(total, i0 + kRoom); i += kThreads) {
+                const uint64_t key = keys[i];
+                if ((uint32_t)(key >> 32) >= least) {
+                    const int at = atomicAdd(&sh.cnt, 1);
+                    if (at < kCap) sh.keys[at] = key;
+                }
+            }
+            if (careful) {
+                __syncthreads();
+                const int cnt = sh.cnt;
+                __syncthreads();
+                if (cnt > kCap - kRoom) select_k(sh, a.k);
+            }
         }
         __syncthreads();
         const int cnt = sh.cnt;
         __syncthreads();
-        if (cnt > kCap - kTile) select_k(sh, a.k);
+        if (cnt <= kCap) break;
+        if (tid == 0) sh.cnt = 0;
+        __syncthreads();
     }
     finish_row(sh, q, a);
 }
 
+// Keys a slice may leave: with a little room above k, few slices need a selection of their own.
+int slots_of(int k) { return k + k / 4 + 16; }
+
 int topk_splits(int Q, int64_t n, int k, int bytes, int sm_count) {
     const int64_t want = Q > 0 ? (int64_t)sm_count * 2 / Q : 1;
-    const int64_t least = k > 256 ? 32 * (int64_t)k : kTile;     // a slice is worth its own selection
+    const int64_t least = k > 256 ? 32 * (int64_t)k : kRoom;     // a slice is worth its own selection
     int64_t s = (n + least - 1) / least;
     if (s > want) s = want;
     const int64_t fit = (n * bytes + kSliceBytes - 1) / kSliceBytes;
@@ -436,7 +482,7 @@ cudaError_t launch_topk_t(const TopkArgs& a, int splits, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     // slices start at multiples of 8 scores, so 16-byte loads stay aligned
     const int64_t slice = ((a.n + splits - 1) / splits + 7) / 8 * 8;
-    kernel<<<(unsigned)((int64_t)a.Q * splits), kThreads, sizeof(Shared), stream>>>(a, splits, slice);
+    kernel<<<(unsigned)((int64_t)a.Q * splits), kThreads, sizeof(Shared), stream>>>(a, splits, slice, slots_of(a.k));
     return cudaGetLastError();
 }
 
@@ -444,7 +490,7 @@ cudaError_t launch_topk_t(const TopkArgs& a, int splits, cudaStream_t stream) {
 
 int64_t topk_workspace_bytes(int Q, int64_t n, int k, int sm_count) {
     const int s = topk_splits(Q, n, k, 4, sm_count);      // the wider the type, the more slices
-    return s == 1 ? 0 : (int64_t)Q * s * k * 8;
+    return s == 1 ? 0 : (int64_t)Q * s * slots_of(k) * 8;
 }
 
 cudaError_t launch_topk(const TopkArgs& a, int sm_count, cudaStream_t stream, int* launches) {
@@ -467,7 +513,7 @@ cudaError_t launch_topk(const TopkArgs& a, int sm_count, cudaStream_t stream, in
     cfg.attrs = &early;
     cfg.numAttrs = 1;
     *launches = 2;
-    return cudaLaunchKernelEx(&cfg, topk_join_kernel, a, splits);
+    return cudaLaunchKernelEx(&cfg, topk_join_kernel, a, splits, slots_of(a.k));
 }
 
 }  // namespace coral
