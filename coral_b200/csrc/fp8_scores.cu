@@ -9,6 +9,7 @@
 #include <cuda.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "scores.cuh"
 
@@ -46,38 +47,65 @@ template <>
 __device__ __forceinline__ float wide<__half>(__half v) { return __half2float(v); }
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantSteps = 4;    // 16-byte loads a lane has in flight
+constexpr int kQuantLoads = 8;    // 16-byte loads a lane has in flight
 
-// The largest magnitude of 16 bytes, as the bits of an fp32: magnitudes order as their bits do.
+// The larger magnitude, lane by lane of 16 bytes; NaN counts as nothing.
 template <typename T>
-__device__ __forceinline__ uint32_t abs_max(uint4 v);
+__device__ __forceinline__ float abs_max(uint4 v);
 template <>
-__device__ __forceinline__ uint32_t abs_max<float>(uint4 v) {
-    return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
-}
-__device__ __forceinline__ uint32_t abs_max_halves(uint4 v) {
-    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-    return max(m & 0xffffu, m >> 16);
+__device__ __forceinline__ float abs_max<float>(uint4 v) {
+    return fmaxf(fmaxf(fabsf(__uint_as_float(v.x)), fabsf(__uint_as_float(v.y))),
+                 fmaxf(fabsf(__uint_as_float(v.z)), fabsf(__uint_as_float(v.w))));
 }
 template <>
-__device__ __forceinline__ uint32_t abs_max<__nv_bfloat16>(uint4 v) { return abs_max_halves(v) << 16; }
+__device__ __forceinline__ float abs_max<__nv_bfloat16>(uint4 v) {
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(__habs2(p[0]), __habs2(p[1])), __hmax2(__habs2(p[2]), __habs2(p[3]))));
+    return fmaxf(m.x, m.y);
+}
 template <>
-__device__ __forceinline__ uint32_t abs_max<__half>(uint4 v) {
-    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)abs_max_halves(v))));
+__device__ __forceinline__ float abs_max<__half>(uint4 v) {
+    const __half2* p = reinterpret_cast<const __half2*>(&v);
+    const float2 m = __half22float2(__hmax2(__hmax2(__habs2(p[0]), __habs2(p[1])), __hmax2(__habs2(p[2]), __habs2(p[3]))));
+    return fmaxf(m.x, m.y);
 }
 
-// A block of 128 columns belongs to G lanes that hold 16 bytes each (32 lanes of fp32, 16 of the 16-bit
-// types): one coalesced read, and its maximum one reduction over the magnitudes' bits.  A warp takes
-// kQuantSteps * 32 / G consecutive blocks and writes their scales together.  Bound by memory, and close
-// behind it by instructions: what is not finite (a maximum of an infinity's bits or more) is dealt with
-// in a branch of its own.
+// What is not finite counts as nothing in a block's maximum and its code is NaN (e4m3 has no infinity):
+// it shows in every score of its row and costs the rest of its block no precision.  A NaN takes this
+// course by itself; a block whose maximum came out infinite or NaN is put right here, in the registers of
+// its eight lanes.
+template <typename T, int J>
+__device__ __forceinline__ float drop_infinities(uint4 (&v)[J]) {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v[j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (sizeof(T) == 4) {
+                if ((w[i] & 0x7fffffffu) == 0x7f800000u) w[i] = 0x7fffffffu;
+            } else {
+                const uint32_t inf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+                if ((w[i] & 0x7fffu) == inf) w[i] |= 0x7fffu;
+                if ((w[i] >> 16 & 0x7fffu) == inf) w[i] |= 0x7fff0000u;
+            }
+        }
+        m = fmaxf(m, abs_max<T>(v[j]));
+    }
+    return m;
+}
+
+// A block of 128 columns belongs to eight lanes, 16 columns each, in J loads of 16 bytes that the eight
+// make of 128 consecutive bytes; its maximum takes three shuffles.  A warp takes kQuantLoads / J steps
+// of four consecutive blocks, all loads before the first use, and writes their scales together.  Bound
+// by memory.  (A block to a whole warp or half of one is bound by instructions instead: the few
+// values a lane then has carry the same addresses, bounds and exponents.)
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads)
 fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, uint8_t* __restrict__ codes,
                     uint8_t* __restrict__ scales, uint32_t inv_per_row) {
-    constexpr int E = 16 / (int)sizeof(T), G = kFp8Block / E, P = 32 / G, N = kQuantSteps * P;
-    const int lane = threadIdx.x & 31, in_block = lane % G, g = lane / G;
-    const uint32_t members = G == 32 ? 0xffffffffu : 0xffffu << (g * G);
+    constexpr int E = 16 / (int)sizeof(T), J = 16 / E, S = kQuantLoads / J, N = 4 * S;
+    const int lane = threadIdx.x & 31, in_block = (lane & 7) * E;
     const int per_row = (dim + kFp8Block - 1) / kFp8Block;
     const int code_pitch = (dim + 15) / 16 * 16, scale_pitch = (dim + 511) / 512 * 4;
     const int64_t total = rows * per_row;
@@ -85,93 +113,96 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
     if (first >= total) return;
     const int64_t row0 = total <= 0x7fffffff ? (int64_t)((uint32_t)first / (uint32_t)per_row) : first / per_row;
     const int b0 = (int)(first - row0 * per_row);
-    auto place = [&](int i, int64_t& row, int& b) {      // block first + i, i < N
-        b = b0 + i;
-        const int over = per_row >= N ? (b >= per_row ? 1 : 0) : (int)((uint32_t)b * inv_per_row >> 16);
+    const int left = (int)(total - first < N ? total - first : N);      // blocks of this warp
+    const auto place = [&](int i, int64_t& row, int& b) {               // block first + i
+        const int at = b0 + i, over = per_row == 1 ? at : (int)__umulhi((uint32_t)at, inv_per_row);
         row = row0 + over;
-        b -= over * per_row;
+        b = at - over * per_row;
     };
-    union Piece {
-        uint4 raw;
-        T v[E];
-        __device__ Piece() {}
-    } in[kQuantSteps];
-    int64_t row[kQuantSteps];
-    int b[kQuantSteps];
+    uint4 v[S][J];
 #pragma unroll
-    for (int u = 0; u < kQuantSteps; ++u) {
-        place(u * P + g, row[u], b[u]);
-        const int c = b[u] * kFp8Block + in_block * E;
-        const T* p = x + row[u] * ld + c;
-        in[u].raw = make_uint4(0u, 0u, 0u, 0u);
-        if (first + u * P + g < total) {
-            if (VEC && c + E <= dim) {
-                in[u].raw = __ldcs(reinterpret_cast<const uint4*>(p));
-            } else {
+    for (int u = 0; u < S; ++u) {
+        const int i = u * 4 + (lane >> 3);
+        int64_t row;
+        int b;
+        place(i, row, b);
+        const int c = b * kFp8Block + in_block;
+        const T* from = x + row * ld + c;
 #pragma unroll
-                for (int i = 0; i < E; ++i)
-                    if (c + i < dim) in[u].v[i] = p[i];
+        for (int j = 0; j < J; ++j) {
+            const int cols = dim - c - j * 8 * E;      // of the row from here on
+            v[u][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < left && cols > 0) {
+                if (VEC && cols >= E) {
+                    v[u][j] = __ldcs(reinterpret_cast<const uint4*>(from + j * 8 * E));
+                } else {
+                    T* w = reinterpret_cast<T*>(&v[u][j]);
+#pragma unroll
+                    for (int k = 0; k < E; ++k)
+                        if (k < cols) w[k] = from[j * 8 * E + k];
+                }
             }
         }
     }
     int mine = 0;      // the exponent of block first + lane
 #pragma unroll
-    for (int u = 0; u < kQuantSteps; ++u) {
-        uint32_t m = __reduce_max_sync(members, abs_max<T>(in[u].raw));
-        float v[E];
+    for (int u = 0; u < S; ++u) {
+        const int i = u * 4 + (lane >> 3);
+        int64_t row;
+        int b;
+        place(i, row, b);
+        float m = abs_max<T>(v[u][0]);
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = wide<T>(in[u].v[i]);
-        if (m >= 0x7f800000u) {
-            // What is not finite counts as nothing, and its code is NaN (e4m3 has no infinity): it shows
-            // in every score of its row and costs the rest of its block no precision.
-            m = 0;
+        for (int j = 1; j < J; ++j) m = fmaxf(m, abs_max<T>(v[u][j]));
+        bool again = false;
+        do {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
-                if (a < 0x7f800000u)
-                    m = max(m, a);
-                else
-                    v[i] = __uint_as_float(0x7fffffffu);
-            }
-            m = __reduce_max_sync(members, m);
-        }
-        const int e = scale_exponent(m);
+            for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            again = !again && __any_sync(0xffffffffu, !(m < __uint_as_float(0x7f800000u)));
+            if (again) m = drop_infinities<T, J>(v[u]);
+        } while (again);
+        const int e = scale_exponent(__float_as_uint(m));
         const float f = __uint_as_float((uint32_t)(127 - e) << 23);     // 2^-e: e in [-127, 120], 2^-e never subnormal
-        const int got = P == 1 ? e : __shfl_sync(0xffffffffu, e, lane % P * G);
-        if (lane / P == u) mine = got;
-        const int c = b[u] * kFp8Block + in_block * E;
-        if (first + u * P + g < total && c < code_pitch) {
-            uint32_t w[E / 4];
+        const int got = __shfl_sync(0xffffffffu, e, (lane & 3) * 8);
+        if (lane >> 2 == u) mine = got;
+        uint8_t* to = codes + row * code_pitch + b * kFp8Block + in_block;
+        const int codes_left = i < left ? code_pitch - b * kFp8Block - in_block : 0;
 #pragma unroll
-            for (int i = 0; i < E; i += 4) w[i / 4] = pack_e4m3(v[i] * f, v[i + 1] * f, v[i + 2] * f, v[i + 3] * f);
-            uint8_t* out = codes + row[u] * code_pitch + c;
-            if (E == 4)
-                *reinterpret_cast<uint32_t*>(out) = w[0];
-            else
-                *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[E / 4 - 1]);
+        for (int j = 0; j < J; ++j) {
+            const T* w = reinterpret_cast<const T*>(&v[u][j]);
+            uint32_t q[E / 4];
+#pragma unroll
+            for (int k = 0; k < E; k += 4)
+                q[k / 4] = pack_e4m3(wide<T>(w[k]) * f, wide<T>(w[k + 1]) * f, wide<T>(w[k + 2]) * f, wide<T>(w[k + 3]) * f);
+            if (codes_left > j * 8 * E) {
+                if (E == 4)
+                    *reinterpret_cast<uint32_t*>(to + j * 8 * E) = q[0];
+                else
+                    *reinterpret_cast<uint2*>(to + j * 8 * E) = make_uint2(q[0], q[E / 4 - 1]);
+            }
         }
     }
-    if (lane < N && first + lane < total) {
-        int64_t r;
-        int bl;
-        place(lane, r, bl);
-        uint8_t* s = scales + r * scale_pitch + bl;
+    if (lane < left) {
+        int64_t row;
+        int b;
+        place(lane, row, b);
+        uint8_t* s = scales + row * scale_pitch + b;
         *s = (uint8_t)(mine + 127);
-        if (bl == per_row - 1)      // the scales that pad the row to a multiple of four
-            for (int i = 1; bl + i < scale_pitch; ++i) s[i] = 0;
+        if (b == per_row - 1)      // the scales that pad the row to a multiple of four
+            for (int i = 1; b + i < scale_pitch; ++i) s[i] = 0;
     }
 }
 
 template <typename T>
 cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t* codes, uint8_t* scales,
                        cudaStream_t stream) {
-    const int64_t total = rows * ((dim + kFp8Block - 1) / kFp8Block);
-    const int per_cta = kQuantThreads / 32 * kQuantSteps * (int)(sizeof(float) / sizeof(T));
-    const int64_t ctas = (total + per_cta - 1) / per_cta;
+    const uint32_t per_row = (uint32_t)((dim + kFp8Block - 1) / kFp8Block);
+    const int per_cta = kQuantThreads / 32 * 4 * kQuantLoads / (int)sizeof(T);
+    const int64_t ctas = (rows * per_row + per_cta - 1) / per_cta;
     const bool vec = ((uintptr_t)x | (uintptr_t)(ld * sizeof(T))) % 16 == 0;
     auto kernel = vec ? fp8_quantize_kernel<T, true> : fp8_quantize_kernel<T, false>;
     kernel<<<(unsigned)ctas, kQuantThreads, 0, stream>>>(static_cast<const T*>(x), rows, dim, ld, codes, scales,
-                                                    65536u / (uint32_t)((dim + kFp8Block - 1) / kFp8Block) + 1u);
+                                                    per_row == 1 ? 0u : (uint32_t)((0x100000000ull + per_row - 1) / per_row));
     return cudaGetLastError();
 }
 
@@ -704,7 +735,8 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
                          CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     auto kernel = tma ? fp8_scores_kernel<T, true> : fp8_scores_kernel<T, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    static std::atomic<uint64_t> granted[2];
+    cudaError_t e = grant_smem(kernel, kSmemBytes, granted[tma]);
     if (e != cudaSuccess) return e;
     TileOrder order;
     order.tiles_m = (uint32_t)(((int64_t)a.Q + kTileM - 1) / kTileM);

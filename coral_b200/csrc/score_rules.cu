@@ -40,6 +40,16 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// v[i] of 16 bytes in registers, for an i known at run time only.
+template <typename T, int V>
+__device__ __forceinline__ T element(const T (&v)[V], int i) {
+    T x = v[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j)
+        if (i == j) x = v[j];
+    return x;
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a, const int chunks) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -147,11 +157,6 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
         const int j = (u * kThreads + tid) * V;
         uint32_t hit = 0;
         if ((has_seen || has_bias) && j < cols) hit = touched[j >> 5] >> (j & 31) & kAll & ~m[u];
-        if (hit) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (hit >> i & 1u) v[u][i] = from_f32<T>(rule(to_f32<T>(v[u][i]), j + i));
-        }
         if (m[u]) {
 #pragma unroll
             for (int i = 0; i < V; ++i)
@@ -163,6 +168,10 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (j + i < cols) out[j + i] = v[u][i];
+        }
+        for (; hit; hit &= hit - 1) {      // the few touched columns again
+            const int i = __ffs(hit) - 1;
+            out[j + i] = from_f32<T>(rule(to_f32<T>(element<T, V>(v[u], i)), j + i));
         }
     }
 }

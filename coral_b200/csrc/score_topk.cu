@@ -478,7 +478,8 @@ template <typename T>
 cudaError_t launch_topk_t(const TopkArgs& a, int splits, cudaStream_t stream) {
     const bool vec = ((uintptr_t)a.in | (uintptr_t)(a.ld * sizeof(T))) % 16 == 0;
     auto kernel = vec ? topk_scan_kernel<T, true> : topk_scan_kernel<T, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+    static std::atomic<uint64_t> granted[2];
+    cudaError_t e = grant_smem(kernel, (int)sizeof(Shared), granted[vec]);
     if (e != cudaSuccess) return e;
     // slices start at multiples of 8 scores, so 16-byte loads stay aligned
     const int64_t slice = ((a.n + splits - 1) / splits + 7) / 8 * 8;
@@ -500,7 +501,8 @@ cudaError_t launch_topk(const TopkArgs& a, int sm_count, cudaStream_t stream, in
                                           : launch_topk_t<__half>(a, splits, stream);
     *launches = 1;
     if (e != cudaSuccess || splits == 1) return e;
-    e = cudaFuncSetAttribute(topk_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+    static std::atomic<uint64_t> granted;
+    e = grant_smem(topk_join_kernel, (int)sizeof(Shared), granted);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.Q);

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace coral {
 
 // Element types of the C ABI (CORAL_F32, CORAL_BF16, CORAL_F16).
@@ -25,6 +27,19 @@ inline int64_t fp8_scale_pitch(int dim) { return ((int64_t)dim + 511) / 512 * 4;
 
 cudaError_t launch_fp8_quantize(const void* x, int type, int64_t rows, int dim, int64_t ld, uint8_t* codes,
                                 uint8_t* scales, int sm_count, cudaStream_t stream);
+
+// Opt-in shared memory of a kernel, asked for once per kernel and device.
+template <typename Kernel>
+inline cudaError_t grant_smem(Kernel* kernel, int bytes, std::atomic<uint64_t>& granted) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (granted.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) granted.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 struct Fp8ScoresArgs {
     const uint8_t *q_codes, *q_scales, *codes, *scales;
