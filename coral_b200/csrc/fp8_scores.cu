@@ -210,7 +210,9 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 //
 // out[q][j] = alpha * sum_b 2^(eq_b + ej_b) * (codes of q, codes of j)_b + bias[j], accumulated in
 // fp32 in tensor memory.  One persistent CTA of 12 warps per SM, tiles of 128 queries x 256 rows:
-//   warp 0     one lane issues the tiles' TMA loads (128-byte swizzle, 128 columns a stage);
+//   warp 0     one lane issues the tiles' TMA loads (128-byte swizzle, 128 columns a stage).  A query
+//              tile of at most kStages k-blocks is kept while the next row tile meets it too: with few
+//              k-blocks the tensor copies, which take their time per row, are what a tile waits for;
 //   warp 1     one lane issues, per stage, four tcgen05.mma (M = 128, N = 256, K = 32) and, per four
 //              stages, three tcgen05.cp (their scales to tensor memory);
 //   warp 2     brings scales to a shared-memory ring of their own in the layout tcgen05.cp takes, with
@@ -235,6 +237,7 @@ constexpr int kStages = 3;
 constexpr int kABytes = kTileM * kTileK, kBBytes = kTileN * kTileK;
 constexpr int kScaleBytes = (kTileM + kTileN) * 4;
 constexpr int kAccStep = 192, kShared = 64, kTmemScales = 448;
+constexpr int kOffB = kStages * kABytes;                            // query tiles first, then row tiles
 constexpr int kOffScales = kStages * (kABytes + kBBytes);
 constexpr int kEpiWarps = 8, kOutBufs = 2;
 constexpr int kScaleSlots = 8, kScalesAhead = 6;                    // groups in the ring, and in flight
@@ -412,14 +415,16 @@ template <typename T, bool TMA_OUT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const TileOrder order,
-                  const int a_rows) {
+                  const int a_rows, const bool keeps_a) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);   // [kStages] codes landed
     uint64_t* empty = full + kStages;                                // [kStages] the products that read the stage are done
     uint64_t* sfull = empty + kStages;                               // [kScaleSlots] a group's scales landed
     uint64_t* sempty = sfull + kScaleSlots;                          // [kScaleSlots] and are no longer needed
-    uint64_t* tfull = sempty + kScaleSlots;                          // accumulator complete
+    uint64_t* afull = sempty + kScaleSlots;                          // a kept query tile landed
+    uint64_t* aempty = afull + 1;                                    // the products that read it are done
+    uint64_t* tfull = aempty + 1;                                    // accumulator complete
     uint64_t* tfree = tfull + 1;                                     // the columns the next tile shares are drained
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -437,6 +442,8 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             mbar_init(&sfull[s], 1);
             mbar_init(&sempty[s], 1);
         }
+        mbar_init(afull, 1);
+        mbar_init(aempty, 1);
         mbar_init(tfull, 1);
         mbar_init(tfree, kEpiWarps);
         *abort_flag = 0;
@@ -457,19 +464,29 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             int s = 0;
             uint32_t par = 0;
             bool ok = true;
+            int64_t kept = -1;          // first row of the query tile kept, how many were
+            uint32_t kept_tiles = 0;
             for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x) {
                 int64_t m0, n0;
                 order.at(t, m0, n0);
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
-                    unsigned char* st = smem + s * (kABytes + kBBytes);
-                    mbar_expect_tx(&full[s], a_rows * kTileK + kBBytes);
-                    tma_load_2d(st, &map_a, kb * kTileK, (int)m0, &full[s]);
-                    tma_load_2d(st + kABytes, &map_b, kb * kTileK, (int)n0, &full[s]);
+                    mbar_expect_tx(&full[s], (keeps_a ? 0 : a_rows * kTileK) + kBBytes);
+                    if (!keeps_a) tma_load_2d(smem + s * kABytes, &map_a, kb * kTileK, (int)m0, &full[s]);
+                    tma_load_2d(smem + kOffB + s * kBBytes, &map_b, kb * kTileK, (int)n0, &full[s]);
                     if (++s == kStages) {
                         s = 0;
                         par ^= 1u;
                     }
+                }
+                if (keeps_a && ok && m0 != kept) {
+                    // after the row tile's loads: it fits the ring, and need not wait for the kept tile's end
+                    if (kept >= 0 && !(ok = mbar_wait(aempty, (kept_tiles - 1) & 1u, abort_flag, a.err))) break;
+                    kept = m0;
+                    ++kept_tiles;
+                    mbar_expect_tx(afull, k_blocks * a_rows * kTileK);
+                    for (int kb = 0; kb < k_blocks; ++kb)
+                        tma_load_2d(smem + kb * kABytes, &map_a, kb * kTileK, (int)m0, afull);
                 }
             }
         }
@@ -478,7 +495,21 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + kOffScales);
         uint32_t s = 0, par = 0, i = 0, group = 0;
         bool ok = true;
+        int64_t kept = -1;
+        uint32_t kept_tiles = 0;
         for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x, ++i) {
+            bool last_of_kept = false;
+            if (keeps_a) {
+                int64_t m0, n0, m1 = -1;
+                order.at(t, m0, n0);
+                if (t + gridDim.x < order.tiles) order.at(t + gridDim.x, m1, n0);
+                last_of_kept = m1 != m0;
+                if (m0 != kept) {
+                    kept = m0;
+                    if (!__all_sync(0xffffffffu, mbar_wait(afull, kept_tiles & 1u, abort_flag, a.err))) break;
+                    ++kept_tiles;
+                }
+            }
             if (i > 0 && !__all_sync(0xffffffffu, mbar_wait(tfree, (i - 1) & 1u, abort_flag, a.err))) break;
             const uint32_t acc = tmem + (i & 1u) * kAccStep;
             for (int kb = 0; kb < k_blocks; ++kb) {
@@ -496,7 +527,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     scales_to_tmem(leads, tb, sc + (512 >> 4));
                     scales_to_tmem(leads, tb + 4, sc + (1024 >> 4));
                 }
-                const uint64_t da = desc_sw128(codes + s * (kABytes + kBBytes)), db = da + (kABytes >> 4);
+                const uint64_t da = desc_sw128(codes + (keeps_a ? kb : s) * kABytes), db = desc_sw128(codes + kOffB + s * kBBytes);
                 const uint32_t idesc = kInstrDesc | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
                 const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
                 if (slices == kTileK / 32) {
@@ -517,6 +548,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     par ^= 1u;
                 }
             }
+            if (ok && last_of_kept) umma_commit(leads, aempty);
             if (ok) umma_commit(leads, tfull);
         }
     } else if (warp == 2) {
@@ -746,7 +778,8 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     order.chunk_n = (uint32_t)(in_l2 < sm_count ? sm_count : in_l2);
     if (order.chunk_n > order.tiles_n) order.chunk_n = order.tiles_n;
     const int grid = (int)(order.tiles < (uint32_t)sm_count ? order.tiles : sm_count);
-    kernel<<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, map_out, a, order, a_rows);
+    kernel<<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, map_out, a, order, a_rows,
+                                                         (a.dim + kTileK - 1) / kTileK <= kStages);
     return cudaGetLastError();
 }
 
