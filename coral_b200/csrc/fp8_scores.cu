@@ -411,7 +411,43 @@ struct TileOrder {
     }
 };
 
-template <typename T, bool TMA_OUT>
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 load_peer(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// How a CTA stores its scores.
+constexpr int kPlain = 0;      // coalesced plain stores
+constexpr int kTma = 1;        // tensor stores
+constexpr int kSplit = 2;      // the tile's k-blocks are split over the CTAs of a cluster, see below
+
+// With fewer tiles than SMs and many k-blocks, a cluster of 2, 4 or 8 CTAs shares a tile: rank r takes a
+// range of its k-blocks (whole groups of four).  Then every CTA lays its partial accumulator out in its
+// stages' memory, and rank p adds, over distributed shared memory and in rank order, the parts of the
+// columns it owns and stores them.  The same additions in every run.  (Reading a row's 16-byte pieces
+// side by side: written to the owner by the threads that hold them, a piece of 32 rows each, the parts
+// take five times as long.)
+template <typename T, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const TileOrder order,
@@ -432,6 +468,12 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // known to be uniform
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
     const int scale_pitch = (a.dim + 511) / 512 * 4;
+    constexpr bool TMA_OUT = OUT == kTma, SPLIT = OUT == kSplit;
+    const uint32_t rank = SPLIT ? cluster_rank() : 0, parts = SPLIT ? cluster_size() : 1;
+    const uint32_t t_first = SPLIT ? blockIdx.x / parts : blockIdx.x, t_step = SPLIT ? order.tiles : gridDim.x;
+    const int groups = (k_blocks + 3) / 4;
+    const int k_first = SPLIT ? (int)(groups * rank / parts) * 4 : 0;
+    const int k_end = SPLIT ? min(k_blocks, (int)(groups * (rank + 1) / parts) * 4) : k_blocks;
 
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -466,10 +508,10 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             bool ok = true;
             int64_t kept = -1;          // first row of the query tile kept, how many were
             uint32_t kept_tiles = 0;
-            for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x) {
+            for (uint32_t t = t_first; t < order.tiles && ok; t += t_step) {
                 int64_t m0, n0;
                 order.at(t, m0, n0);
-                for (int kb = 0; kb < k_blocks; ++kb) {
+                for (int kb = k_first; kb < k_end; ++kb) {
                     if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
                     mbar_expect_tx(&full[s], (keeps_a ? 0 : a_rows * kTileK) + kBBytes);
                     if (!keeps_a) tma_load_2d(smem + s * kABytes, &map_a, kb * kTileK, (int)m0, &full[s]);
@@ -497,12 +539,12 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         bool ok = true;
         int64_t kept = -1;
         uint32_t kept_tiles = 0;
-        for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x, ++i) {
+        for (uint32_t t = t_first; t < order.tiles && ok; t += t_step, ++i) {
             bool last_of_kept = false;
             if (keeps_a) {
                 int64_t m0, n0, m1 = -1;
                 order.at(t, m0, n0);
-                if (t + gridDim.x < order.tiles) order.at(t + gridDim.x, m1, n0);
+                if (t + t_step < order.tiles) order.at(t + t_step, m1, n0);
                 last_of_kept = m1 != m0;
                 if (m0 != kept) {
                     kept = m0;
@@ -512,7 +554,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
             if (i > 0 && !__all_sync(0xffffffffu, mbar_wait(tfree, (i - 1) & 1u, abort_flag, a.err))) break;
             const uint32_t acc = tmem + (i & 1u) * kAccStep;
-            for (int kb = 0; kb < k_blocks; ++kb) {
+            for (int kb = k_first; kb < k_end; ++kb) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a.err));
                 if (!ok) break;
                 const uint32_t slot = group % kScaleSlots, ta = tmem + kTmemScales + group % 4 * 16, tb = ta + 8;
@@ -533,13 +575,13 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 if (slices == kTileK / 32) {
 #pragma unroll
                     for (int j = 0; j < kTileK / 32; ++j)
-                        umma_mxf8(leads, acc, da + j * 2, db + j * 2, idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
+                        umma_mxf8(leads, acc, da + j * 2, db + j * 2, idesc, ta, tb, kb != k_first || j != 0 ? 1u : 0u);
                 } else {
                     for (int j = 0; j < slices; ++j)
-                        umma_mxf8(leads, acc, da + j * 2, db + j * 2, idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
+                        umma_mxf8(leads, acc, da + j * 2, db + j * 2, idesc, ta, tb, kb != k_first || j != 0 ? 1u : 0u);
                 }
                 umma_commit(leads, &empty[s]);
-                if ((kb & 3) == 3 || kb == k_blocks - 1) {
+                if ((kb & 3) == 3 || kb == k_end - 1) {
                     umma_commit(leads, &sempty[slot]);
                     ++group;
                 }
@@ -568,10 +610,10 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                          "l"(base + (there ? r * scale_pitch + kb : 0)), "r"(there ? 4 : 0)
                          : "memory");
         };
-        for (uint32_t t = blockIdx.x; t < order.tiles && ok; t += gridDim.x) {
+        for (uint32_t t = t_first; t < order.tiles && ok; t += t_step) {
             int64_t m0, n0;
             order.at(t, m0, n0);
-            for (int kb = 0; kb < k_blocks; kb += 4) {
+            for (int kb = k_first; kb < k_end; kb += 4) {
                 const uint32_t slot = sent % kScaleSlots;
                 ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a.err));
                 if (!ok) break;
@@ -590,6 +632,11 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         while (ok && done < sent) publish();
+    } else if (SPLIT) {
+        if (warp >= 4) {
+            mbar_wait(tfull, 0, abort_flag, a.err);
+            tc_fence_after();
+        }
     } else if (warp >= 4) {
         const int g = warp & 3, half = (warp - 4) >> 2;      // 32 lanes of tensor memory; which of their two warps
         constexpr int W = 128 / (int)sizeof(T);              // columns of a piece
@@ -695,6 +742,76 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         __syncwarp();
     }
 
+    if constexpr (SPLIT) {
+        const int width = kTileN / (int)parts;      // columns a CTA owns
+        int64_t m0, n0;
+        order.at(t_first, m0, n0);
+        const int rows = (int)(a.Q - m0 < kTileM ? a.Q - m0 : kTileM);
+        // the accumulator as [row][column], 16-byte pieces permuted by the row; the products that read
+        // the stages' memory are done
+        const int g = warp & 3, half = (warp - 4) >> 2, held = g * 32 + lane;
+        if (warp >= 4 && g * 32 < rows && !*abort_flag) {
+            const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16);
+#pragma unroll 1
+            for (int col = half * 32; col < kTileN; col += 64) {
+                uint32_t r[32];
+                __syncwarp();
+                tmem_ld32(acc + (uint32_t)col, r);
+                tmem_ld_wait();
+                uint4* to = reinterpret_cast<uint4*>(smem) + held * (kTileN / 4);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    to[(col / 4 + u) ^ (held & 7)] = make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+            }
+            tc_fence_before();
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 4 && !*abort_flag) {
+            // four columns a thread, the threads of a row side by side
+            const int log_pieces = __ffs(width / 4) - 1;
+            const bool whole = ((uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T))) % (4 * sizeof(T)) == 0;
+#pragma unroll 2
+            for (int i = (warp - 4) * 32 + lane; i < rows << log_pieces; i += kEpiWarps * 32) {
+                const int row = i >> log_pieces, piece = i - (row << log_pieces);
+                const uint32_t from = smem_u32(smem) + (row * (kTileN / 4) + (((int)rank * (width / 4) + piece) ^ (row & 7))) * 16;
+                float4 part[8];
+#pragma unroll
+                for (uint32_t p = 0; p < 8; ++p)
+                    if (p < parts) part[p] = load_peer(peer_smem(from, p));
+                float4 sum = part[0];
+#pragma unroll
+                for (uint32_t p = 1; p < 8; ++p) {
+                    if (p >= parts) break;
+                    const float4 x = part[p];
+                    sum.x += x.x;
+                    sum.y += x.y;
+                    sum.z += x.z;
+                    sum.w += x.w;
+                }
+                const int64_t n = n0 + (int64_t)rank * width + piece * 4;
+                T* out = static_cast<T*>(a.out) + (m0 + row) * a.ld + n;
+                alignas(16) T v[4];
+                const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = narrow<T>(fmaf(a.alpha, y[e], a.bias && n + e < a.n ? a.bias[n + e] : 0.f));
+                if (whole && n + 4 <= a.n) {
+                    if (sizeof(T) == 4)
+                        *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(v);
+                    else
+                        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < a.n) out[e] = v[e];
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();      // nobody reads a peer any more
+    }
+
     tc_fence_before();
     __syncthreads();
     if (*abort_flag) {
@@ -745,6 +862,54 @@ bool matrix_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, in
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Clusters of `parts` CTAs of the split kernel that the current device holds at once (fewer than SMs /
+// parts: a cluster stays inside one group of SMs); asked for once per device.
+template <typename Kernel>
+int clusters_at_once(Kernel* kernel, int parts) {
+    static std::atomic<int> known[64][4];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    const int slot = parts == 2 ? 1 : parts == 4 ? 2 : 3;
+    if (dev >= 0 && dev < 64)
+        if (const int n = known[dev][slot].load(std::memory_order_relaxed)) return n - 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)parts);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cudaLaunchAttribute cluster = {};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = (unsigned)parts;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    if (dev >= 0 && dev < 64) known[dev][slot].store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
+// CTAs that share a tile: the count with the shortest time in k-blocks a CTA goes through, one after the
+// other, a wave of shared tiles costing kSplitCost more for its start and its join.
+constexpr int kSplitCost = 5;
+template <typename Kernel>
+int split_of(Kernel* kernel, uint32_t tiles, int k_blocks, int sm_count) {
+    int best = 1;
+    int64_t least = (int64_t)((tiles + sm_count - 1) / sm_count) * k_blocks;
+    for (int p = 2; p <= 8 && 4 * p <= k_blocks + 3; p *= 2) {
+        const int at_once = clusters_at_once(kernel, p);
+        if (at_once < 1) continue;
+        const int64_t cost = (int64_t)((tiles + at_once - 1) / at_once) * (((k_blocks + 3) / 4 + p - 1) / p * 4 + kSplitCost);
+        if (cost < least) {
+            least = cost;
+            best = p;
+        }
+    }
+    return best;
+}
+
 template <typename T>
 cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) {
     const CUtensorMapDataType type = a.type == kTypeF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -766,10 +931,6 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     else if (!matrix_map(&map_out, type, a.out, a.Q, a.n, a.ld * (int64_t)sizeof(T), 128 / (int)sizeof(T), 32,
                          CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
-    auto kernel = tma ? fp8_scores_kernel<T, true> : fp8_scores_kernel<T, false>;
-    static std::atomic<uint64_t> granted[2];
-    cudaError_t e = grant_smem(kernel, kSmemBytes, granted[tma]);
-    if (e != cudaSuccess) return e;
     TileOrder order;
     order.tiles_m = (uint32_t)(((int64_t)a.Q + kTileM - 1) / kTileM);
     order.tiles_n = (uint32_t)(((int64_t)a.n + kTileN - 1) / kTileN);
@@ -777,10 +938,30 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     const int64_t in_l2 = kChunkBytes / (kTileN * fp8_code_pitch(a.dim));
     order.chunk_n = (uint32_t)(in_l2 < sm_count ? sm_count : in_l2);
     if (order.chunk_n > order.tiles_n) order.chunk_n = order.tiles_n;
-    const int grid = (int)(order.tiles < (uint32_t)sm_count ? order.tiles : sm_count);
-    kernel<<<grid, kThreads, kSmemBytes, stream>>>(map_a, map_b, map_out, a, order, a_rows,
-                                                         (a.dim + kTileK - 1) / kTileK <= kStages);
-    return cudaGetLastError();
+    const int k_blocks = (a.dim + kTileK - 1) / kTileK;
+    static std::atomic<uint64_t> granted[3];
+    int parts = 1;
+    if (order.tiles <= (uint32_t)sm_count && k_blocks > 4) {
+        cudaError_t e = grant_smem(fp8_scores_kernel<T, kSplit>, kSmemBytes, granted[kSplit]);
+        if (e != cudaSuccess) return e;
+        parts = split_of(fp8_scores_kernel<T, kSplit>, order.tiles, k_blocks, sm_count);
+    }
+    const int out = parts > 1 ? kSplit : tma ? kTma : kPlain;
+    auto kernel = out == kSplit ? fp8_scores_kernel<T, kSplit> : out == kTma ? fp8_scores_kernel<T, kTma> : fp8_scores_kernel<T, kPlain>;
+    cudaError_t e = grant_smem(kernel, kSmemBytes, granted[out]);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(parts > 1 ? order.tiles * parts : order.tiles < (uint32_t)sm_count ? order.tiles : (uint32_t)sm_count);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute cluster = {};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = (unsigned)parts;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, order, a_rows, k_blocks <= kStages);
 }
 
 }  // namespace

@@ -232,6 +232,24 @@ def test_scores_into_slices(ix, dtype, n, lead, ld):
     assert bool((whole == 77.0).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Q,n,dim", [(3, 700, 2100), (130, 513, 4096), (40, 257, 1100), (128, 300, 8200), (33, 1999, 3000)])
+@pytest.mark.parametrize("lead,pad", [(0, 0), (1, 2), (4, 4)])
+def test_scores_of_few_tiles(ix, dtype, Q, n, dim, lead, pad):
+    """Few tiles with many k-blocks are shared by clusters: any alignment of the output, nothing outside it."""
+    q, base = rows8(ix, Q, dim, 13, 2), rows8(ix, n, dim, 14, 2)
+    bias = torch.randn(n, generator=gen(15), device="cuda")
+    whole = torch.full((Q + 2, lead + n + pad), 77.0, dtype=dtype, device="cuda")
+    out = whole[1:Q + 1, lead:lead + n]
+    ix.fp8_scores(q, base, dim, 2.0 ** -9, bias, out=out)
+    check_scores(out, q, base, dim, 2.0 ** -9, bias)
+    first = out.clone()
+    ix.fp8_scores(q, base, dim, 2.0 ** -9, bias, out=out)
+    assert torch.equal(first, out)
+    out.fill_(77.0)
+    assert bool((whole == 77.0).all())
+
+
 def test_scores_extreme_scales_and_values(ix):
     dim = 512
     q = rows8(ix, 4, dim, 11, 0)
