@@ -95,17 +95,18 @@ __device__ __forceinline__ float drop_infinities(uint4 (&v)[J]) {
     return m;
 }
 
-// A block of 128 columns belongs to eight lanes, 16 columns each, in J loads of 16 bytes that the eight
-// make of 128 consecutive bytes; its maximum takes three shuffles.  A warp takes kQuantLoads / J steps
-// of four consecutive blocks, all loads before the first use, and writes their scales together.  Bound
-// by memory.  (A block to a whole warp or half of one is bound by instructions instead: the few
+// A block of 128 columns belongs to G lanes, 16 columns each, in J loads of 16 bytes that the G lanes make
+// of consecutive bytes; its maximum takes log2 G shuffles.  G is 8, or fewer for rows of one block of
+// at most 64, 32 or 16 columns, which would leave the other lanes idle (800k x 14 bf16: 52 us with
+// eight).  A warp takes kQuantLoads / J steps of 32 / G consecutive blocks, all loads before the first
+// use, and writes the scales together.  Bound by memory.  (A block to a whole warp or half of one is bound by instructions instead: the few
 // values a lane then has carry the same addresses, bounds and exponents.)
-template <typename T, bool VEC>
+template <typename T, bool VEC, int G>
 __global__ void __launch_bounds__(kQuantThreads)
 fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, uint8_t* __restrict__ codes,
                     uint8_t* __restrict__ scales, uint32_t inv_per_row) {
-    constexpr int E = 16 / (int)sizeof(T), J = 16 / E, S = kQuantLoads / J, N = 4 * S;
-    const int lane = threadIdx.x & 31, in_block = (lane & 7) * E;
+    constexpr int E = 16 / (int)sizeof(T), J = 16 / E, S = kQuantLoads / J, P = 32 / G, N = P * S;
+    const int lane = threadIdx.x & 31, in_block = lane % G * E;
     const int per_row = (dim + kFp8Block - 1) / kFp8Block;
     const int code_pitch = (dim + 15) / 16 * 16, scale_pitch = (dim + 511) / 512 * 4;
     const int64_t total = rows * per_row;
@@ -122,7 +123,7 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
     uint4 v[S][J];
 #pragma unroll
     for (int u = 0; u < S; ++u) {
-        const int i = u * 4 + (lane >> 3);
+        const int i = u * P + lane / G;
         int64_t row;
         int b;
         place(i, row, b);
@@ -130,16 +131,16 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
         const T* from = x + row * ld + c;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int cols = dim - c - j * 8 * E;      // of the row from here on
+            const int cols = dim - c - j * G * E;      // of the row from here on
             v[u][j] = make_uint4(0u, 0u, 0u, 0u);
             if (i < left && cols > 0) {
                 if (VEC && cols >= E) {
-                    v[u][j] = __ldcs(reinterpret_cast<const uint4*>(from + j * 8 * E));
+                    v[u][j] = __ldcs(reinterpret_cast<const uint4*>(from + j * G * E));
                 } else {
                     T* w = reinterpret_cast<T*>(&v[u][j]);
 #pragma unroll
                     for (int k = 0; k < E; ++k)
-                        if (k < cols) w[k] = from[j * 8 * E + k];
+                        if (k < cols) w[k] = from[j * G * E + k];
                 }
             }
         }
@@ -147,7 +148,7 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
     int mine = 0;      // the exponent of block first + lane
 #pragma unroll
     for (int u = 0; u < S; ++u) {
-        const int i = u * 4 + (lane >> 3);
+        const int i = u * P + lane / G;
         int64_t row;
         int b;
         place(i, row, b);
@@ -157,14 +158,18 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
         bool again = false;
         do {
 #pragma unroll
-            for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int o = 1; o < G; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             again = !again && __any_sync(0xffffffffu, !(m < __uint_as_float(0x7f800000u)));
             if (again) m = drop_infinities<T, J>(v[u]);
         } while (again);
         const int e = scale_exponent(__float_as_uint(m));
         const float f = __uint_as_float((uint32_t)(127 - e) << 23);     // 2^-e: e in [-127, 120], 2^-e never subnormal
-        const int got = __shfl_sync(0xffffffffu, e, (lane & 3) * 8);
-        if (lane >> 2 == u) mine = got;
+        if constexpr (P <= 8) {      // a lane's own block's, of up to 32 blocks a warp
+            const int got = __shfl_sync(0xffffffffu, e, lane % P * G);
+            if (lane / P == u) mine = got;
+        } else if (i < left && lane % G == 0) {
+            *reinterpret_cast<uint32_t*>(scales + row * 4) = (uint32_t)(e + 127);      // one block a row
+        }
         uint8_t* to = codes + row * code_pitch + b * kFp8Block + in_block;
         const int codes_left = i < left ? code_pitch - b * kFp8Block - in_block : 0;
 #pragma unroll
@@ -174,15 +179,15 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
 #pragma unroll
             for (int k = 0; k < E; k += 4)
                 q[k / 4] = pack_e4m3(wide<T>(w[k]) * f, wide<T>(w[k + 1]) * f, wide<T>(w[k + 2]) * f, wide<T>(w[k + 3]) * f);
-            if (codes_left > j * 8 * E) {
+            if (codes_left > j * G * E) {
                 if (E == 4)
-                    *reinterpret_cast<uint32_t*>(to + j * 8 * E) = q[0];
+                    *reinterpret_cast<uint32_t*>(to + j * G * E) = q[0];
                 else
-                    *reinterpret_cast<uint2*>(to + j * 8 * E) = make_uint2(q[0], q[E / 4 - 1]);
+                    *reinterpret_cast<uint2*>(to + j * G * E) = make_uint2(q[0], q[E / 4 - 1]);
             }
         }
     }
-    if (lane < left) {
+    if (P <= 8 && lane < left) {
         int64_t row;
         int b;
         place(lane, row, b);
@@ -193,17 +198,26 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
     }
 }
 
-template <typename T>
-cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t* codes, uint8_t* scales,
+template <typename T, int G>
+cudaError_t quantize_g(const void* x, int64_t rows, int dim, int64_t ld, uint8_t* codes, uint8_t* scales,
                        cudaStream_t stream) {
     const uint32_t per_row = (uint32_t)((dim + kFp8Block - 1) / kFp8Block);
-    const int per_cta = kQuantThreads / 32 * 4 * kQuantLoads / (int)sizeof(T);
+    const int per_cta = kQuantThreads / G * kQuantLoads / (int)sizeof(T);
     const int64_t ctas = (rows * per_row + per_cta - 1) / per_cta;
     const bool vec = ((uintptr_t)x | (uintptr_t)(ld * sizeof(T))) % 16 == 0;
-    auto kernel = vec ? fp8_quantize_kernel<T, true> : fp8_quantize_kernel<T, false>;
+    auto kernel = vec ? fp8_quantize_kernel<T, true, G> : fp8_quantize_kernel<T, false, G>;
     kernel<<<(unsigned)ctas, kQuantThreads, 0, stream>>>(static_cast<const T*>(x), rows, dim, ld, codes, scales,
                                                     per_row == 1 ? 0u : (uint32_t)((0x100000000ull + per_row - 1) / per_row));
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t* codes, uint8_t* scales,
+                       cudaStream_t stream) {
+    if (dim <= 16) return quantize_g<T, 1>(x, rows, dim, ld, codes, scales, stream);
+    if (dim <= 32) return quantize_g<T, 2>(x, rows, dim, ld, codes, scales, stream);
+    if (dim <= 64) return quantize_g<T, 4>(x, rows, dim, ld, codes, scales, stream);
+    return quantize_g<T, 8>(x, rows, dim, ld, codes, scales, stream);
 }
 
 // ----------------------------------------------------------------------------------- product
@@ -306,11 +320,12 @@ __device__ __forceinline__ void tma_store_2d(uint32_t leads, const CUtensorMap* 
         "@q cp.async.bulk.commit_group;\n\t}" ::"l"(map), "r"(c0), "r"(c1), "r"(smem_u32(src)), "l"(policy), "r"(leads)
         : "memory");
 }
-// Shared-memory matrix descriptor, K-major rows of 128 bytes with the 128-byte swizzle: 8-row groups
-// 1024 bytes apart, descriptor version 1, layout type 2.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Shared-memory matrix descriptor, K-major rows of `row` = 128, 64 or 32 bytes with the swizzle of that
+// width: 8-row groups 8 * row bytes apart, descriptor version 1, layout type 2, 4 or 6.
+__device__ __forceinline__ uint64_t desc_rows(int row) {
+    return (1ull << 16) | ((uint64_t)(8 * row >> 4) << 32) | (1ull << 46) | ((row == 128 ? 2ull : row == 64 ? 4ull : 6ull) << 61);
 }
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t addr) { return desc | ((addr >> 4) & 0x3FFFu); }
 // The same for 32 unswizzled rows of 16 bytes (scales): 8-row groups 128 bytes apart.
 __device__ __forceinline__ uint64_t desc_rows16(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
@@ -451,7 +466,7 @@ template <typename T, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const TileOrder order,
-                  const int a_rows, const bool keeps_a) {
+                  const int a_rows, const int row_bytes, const bool keeps_a) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);   // [kStages] codes landed
@@ -513,7 +528,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 order.at(t, m0, n0);
                 for (int kb = k_first; kb < k_end; ++kb) {
                     if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
-                    mbar_expect_tx(&full[s], (keeps_a ? 0 : a_rows * kTileK) + kBBytes);
+                    mbar_expect_tx(&full[s], ((keeps_a ? 0 : a_rows) + kTileN) * row_bytes);
                     if (!keeps_a) tma_load_2d(smem + s * kABytes, &map_a, kb * kTileK, (int)m0, &full[s]);
                     tma_load_2d(smem + kOffB + s * kBBytes, &map_b, kb * kTileK, (int)n0, &full[s]);
                     if (++s == kStages) {
@@ -526,7 +541,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     if (kept >= 0 && !(ok = mbar_wait(aempty, (kept_tiles - 1) & 1u, abort_flag, a.err))) break;
                     kept = m0;
                     ++kept_tiles;
-                    mbar_expect_tx(afull, k_blocks * a_rows * kTileK);
+                    mbar_expect_tx(afull, k_blocks * a_rows * row_bytes);
                     for (int kb = 0; kb < k_blocks; ++kb)
                         tma_load_2d(smem + kb * kABytes, &map_a, kb * kTileK, (int)m0, afull);
                 }
@@ -535,6 +550,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     } else if (warp == 1) {
         const uint32_t leads = elect_leader();
         const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + kOffScales);
+        const uint64_t desc = desc_rows(row_bytes);
         uint32_t s = 0, par = 0, i = 0, group = 0;
         bool ok = true;
         int64_t kept = -1;
@@ -569,7 +585,8 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     scales_to_tmem(leads, tb, sc + (512 >> 4));
                     scales_to_tmem(leads, tb + 4, sc + (1024 >> 4));
                 }
-                const uint64_t da = desc_sw128(codes + (keeps_a ? kb : s) * kABytes), db = desc_sw128(codes + kOffB + s * kBBytes);
+                const uint64_t da = desc_at(desc, codes + (keeps_a ? kb : s) * kABytes);
+                const uint64_t db = desc_at(desc, codes + kOffB + s * kBBytes);
                 const uint32_t idesc = kInstrDesc | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
                 const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
                 if (slices == kTileK / 32) {
@@ -647,29 +664,39 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         uint64_t policy;
         asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         uint32_t i = 0, sent = 0;
-        for (uint32_t t = blockIdx.x; t < order.tiles; t += gridDim.x, ++i) {
-            int64_t m0, n0;
-            order.at(t, m0, n0);
-            m0 += g * 32;
-            const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);      // this warp's, none or fewer past the end
+        int64_t m_next, n_next;
+        order.at(t_first, m_next, n_next);
+        // the biases of a tile's columns are fetched while the tile before is stored
+        float next_bias[kTurns * kTurn / 32];
+        const auto col_of = [&](uint32_t tile, int turn) {
             // turns from the accumulator's shared columns on: its last 64 or its first 64
-            const int start = (i & 1u) ? 0 : kTileN - kShared;
-            const auto col_of = [&](int turn) { return (start + (2 * turn + half) * kTurn) & (kTileN - 1); };
+            return ((tile & 1u ? 0 : kTileN - kShared) + (2 * turn + half) * kTurn) & (kTileN - 1);
+        };
+        const auto fetch_bias = [&](uint32_t tile, int64_t n0) {
+#pragma unroll
+            for (int j = 0; j < kTurns * kTurn / 32; ++j) {
+                const int64_t n = n0 + col_of(tile, j * 32 / kTurn) + j * 32 % kTurn + lane;
+                next_bias[j] = n < a.n ? a.bias[n] : 0.f;
+            }
+        };
+        if (a.bias) fetch_bias(0, n_next);
+        for (uint32_t t = t_first; t < order.tiles; t += t_step, ++i) {
+            const int64_t m0 = m_next + g * 32, n0 = n_next;
+            if (t + t_step < order.tiles) order.at(t + t_step, m_next, n_next);
+            const int rows = (int)(a.Q - m0 < 32 ? a.Q - m0 : 32);      // this warp's, none or fewer past the end
             if (a.bias) {
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < kTurns * kTurn; j += 32) {
-                    const int64_t n = n0 + col_of(j / kTurn) + j % kTurn + lane;
-                    sbias[j + lane] = n < a.n ? a.bias[n] : 0.f;
-                }
+                for (int j = 0; j < kTurns * kTurn / 32; ++j) sbias[j * 32 + lane] = next_bias[j];
                 __syncwarp();
+                if (t + t_step < order.tiles) fetch_bias(i + 1, n_next);
             }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1u, abort_flag, a.err))) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16) + (i & 1u) * kAccStep;
 #pragma unroll 1
             for (int turn = 0; turn < kTurns; ++turn) {
-                const int col0 = col_of(turn);
+                const int col0 = col_of(i, turn);
                 const bool used = rows > 0 && n0 + col0 < a.n;
                 uint32_t r[kTurn / 32][32];
                 if (used) {
@@ -921,10 +948,16 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     // (a row outside the matrix costs the tensor copy more than one inside it)
     const int a_rows = a.Q >= kTileM ? kTileM : (a.Q + 7) / 8 * 8;
     alignas(64) CUtensorMap map_a, map_b, map_out;
-    if (!matrix_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q_codes, a.Q, a.dim, fp8_code_pitch(a.dim), kTileK, a_rows,
-                    CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !matrix_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.n, a.dim, fp8_code_pitch(a.dim), kTileK, kTileN,
-                    CU_TENSOR_MAP_SWIZZLE_128B))
+    // bytes of a row in a stage: 128, or 32 or 64 where that holds the whole row (columns outside the
+    // matrix cost the tensor copy time, too)
+    const int row_bytes = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : kTileK;
+    const CUtensorMapSwizzle swizzle = row_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
+                                       : row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                         : CU_TENSOR_MAP_SWIZZLE_128B;
+    if (!matrix_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q_codes, a.Q, a.dim, fp8_code_pitch(a.dim), row_bytes, a_rows,
+                    swizzle) ||
+        !matrix_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.n, a.dim, fp8_code_pitch(a.dim), row_bytes, kTileN,
+                    swizzle))
         return cudaErrorInvalidValue;
     if (!tma)
         map_out = map_a;      // not used
@@ -961,7 +994,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, order, a_rows, k_blocks <= kStages);
+    return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, order, a_rows, row_bytes, k_blocks <= kStages);
 }
 
 }  // namespace

@@ -50,7 +50,11 @@ __device__ __forceinline__ T element(const T (&v)[V], int i) {
     return x;
 }
 
-template <typename T, bool VEC>
+// Where the rows lie: elements one by one; whole vectors from the first column on, a ragged end element
+// by element; whole vectors from the first 16-byte boundary of each row on.
+constexpr int kElements = 0, kAligned = 1, kShifted = 2;
+
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a, const int chunks) {
     extern __shared__ __align__(16) unsigned char smem[];
     const int q = blockIdx.x / chunks;
@@ -62,33 +66,48 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
     float* bias = reinterpret_cast<float*>(smem) + (has_seen ? kCols : 0);
     uint32_t* touched = reinterpret_cast<uint32_t*>(smem) + kCols * ((has_seen ? 1 : 0) + (has_bias ? 1 : 0));
 
-    // the thread's scores: U vectors of V, vector u at column (u * kThreads + tid) * V
+    // The thread's scores: U vectors of V, vector u at column head + (u * kThreads + tid) * V, and, of
+    // shifted rows, at most one of the columns before the first and after the last whole vector.
+    constexpr bool VEC = ROWS != kElements, SHIFTED = ROWS == kShifted;
     constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
     constexpr int U = kCols / (kThreads * V);
     constexpr uint32_t kAll = (1u << V) - 1u;
     const T* in = static_cast<const T*>(a.in) + (size_t)q * a.ld + c0;
     T* out = static_cast<T*>(a.out) + (size_t)q * a.ld_out + c0;
     const uint32_t* ex = a.excluded ? a.excluded + (size_t)q * a.ld_excluded + c0 / 32 : nullptr;
+    const int head = SHIFTED ? min(cols, (int)((16 - ((uintptr_t)in & 15)) % 16 / sizeof(T))) : 0;
+    const int end = SHIFTED ? head + (cols - head) / V * V : cols;
+    const int odd = !SHIFTED ? -1 : tid < head ? tid : tid >= 32 && end + tid - 32 < cols ? end + tid - 32 : -1;
+    // V bits of a row of words from bit j on
+    const auto bits_at = [&](const uint32_t* words, int j) {
+        const int shift = j & 31;
+        uint32_t b = words[j >> 5] >> shift;
+        if (SHIFTED && shift + V > 32) b |= words[(j >> 5) + 1] << (32 - shift);
+        return b & kAll;
+    };
     alignas(16) T v[U][V];
     uint32_t m[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int j = (u * kThreads + tid) * V;
-        m[u] = ex && j < cols ? ex[j >> 5] >> (j & 31) & kAll : 0u;
+        const int j = head + (u * kThreads + tid) * V;
+        m[u] = SHIFTED && j >= end ? kAll : ex && j < end ? bits_at(ex, j) : 0u;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int j = (u * kThreads + tid) * V;
+        const int j = head + (u * kThreads + tid) * V;
         if (m[u] != kAll) {      // what is excluded altogether is not read
-            if (VEC && j + V <= cols) {
+            if (SHIFTED || (VEC && j + V <= end)) {
                 *reinterpret_cast<uint4*>(v[u]) = *reinterpret_cast<const uint4*>(in + j);
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (j + i < cols) v[u][i] = in[j + i];
+                    if (j + i < end) v[u][i] = in[j + i];
             }
         }
     }
+    const bool odd_out = odd >= 0 && ex && (ex[odd >> 5] >> (odd & 31) & 1u);
+    T odd_in = from_f32<T>(-CUDART_INF_F);
+    if (odd >= 0 && !odd_out) odd_in = in[odd];
 
     float rho = 1.f, phi = 0.f, pi = 0.f;
     if (has_seen || has_bias) {
@@ -102,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
             phi = a.penalties[(size_t)q * 3 + 1];
             pi = a.penalties[(size_t)q * 3 + 2];
         }
-        const int words = (int)(touched - count) + kCols / 32;
+        const int words = (int)(touched - count) + kCols / 32 + 4;      // one word to spare behind the bits
         for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         if (has_seen) {
@@ -121,18 +140,18 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
             for (int i0 = 0; i0 < a.n_bias; i0 += 32) {
                 const int i = i0 + lane;
                 const int64_t j = i < a.n_bias ? (int64_t)ids[i] - c0 : -1;
-                uint32_t todo = __ballot_sync(0xffffffffu, j >= 0 && j < cols);
-                if (!todo) continue;
-                const float val = i < a.n_bias ? vals[i] : 0.f;
-                for (; todo; todo &= todo - 1) {      // in list order
-                    const int src = __ffs(todo) - 1;
-                    const int at = __shfl_sync(0xffffffffu, (int)j, src);
-                    const float x = __shfl_sync(0xffffffffu, val, src);
-                    if (lane == 0) {
-                        bias[at] += x;
-                        atomicOr(&touched[at >> 5], 1u << (at & 31));
-                    }
+                const bool mine = j >= 0 && j < cols;
+                if (!__any_sync(0xffffffffu, mine)) continue;
+                const float val = mine ? vals[i] : 0.f;
+                // entries of one id take turns, in list order; different ids go together
+                const uint32_t same = __match_any_sync(0xffffffffu, mine ? (int)j : -1 - lane);
+                const uint32_t before = __popc(same & ((1u << lane) - 1u));
+                const uint32_t turns = __reduce_max_sync(0xffffffffu, before);
+                for (uint32_t turn = 0; turn <= turns; ++turn) {
+                    if (mine && before == turn) bias[j] += val;
+                    __syncwarp();
                 }
+                if (mine && before == 0) atomicOr(&touched[j >> 5], 1u << (j & 31));
             }
         }
         __syncthreads();
@@ -154,35 +173,42 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int j = (u * kThreads + tid) * V;
-        uint32_t hit = 0;
-        if ((has_seen || has_bias) && j < cols) hit = touched[j >> 5] >> (j & 31) & kAll & ~m[u];
+        const int j = head + (u * kThreads + tid) * V;
+        if (SHIFTED && j >= end) break;
+        uint32_t hit = (has_seen || has_bias) && j < end ? bits_at(touched, j) & ~m[u] : 0u;
         if (m[u]) {
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (m[u] >> i & 1u) v[u][i] = from_f32<T>(-CUDART_INF_F);
         }
-        if (VEC && j + V <= cols) {
+        if (SHIFTED || (VEC && j + V <= end)) {
             *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<uint4*>(v[u]);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (j + i < cols) out[j + i] = v[u][i];
+                if (j + i < end) out[j + i] = v[u][i];
         }
         for (; hit; hit &= hit - 1) {      // the few touched columns again
             const int i = __ffs(hit) - 1;
             out[j + i] = from_f32<T>(rule(to_f32<T>(element<T, V>(v[u], i)), j + i));
         }
     }
+    if (odd >= 0) {
+        if (!odd_out && (has_seen || has_bias) && (touched[odd >> 5] >> (odd & 31) & 1u))
+            odd_in = from_f32<T>(rule(to_f32<T>(odd_in), odd));
+        out[odd] = odd_in;
+    }
 }
 
 template <typename T>
 cudaError_t launch_rules(const RulesArgs& a, cudaStream_t stream) {
     const int64_t chunks = (a.n + kCols - 1) / kCols;
-    const size_t smem = (size_t)kCols * 4 * ((a.n_seen > 0) + (a.n_bias > 0)) + kCols / 8;
-    const bool vec = ((uintptr_t)a.in | (uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T)) |
-                      (uintptr_t)(a.ld_out * sizeof(T))) % 16 == 0;
-    auto kernel = vec ? score_rules_kernel<T, true> : score_rules_kernel<T, false>;
+    const size_t smem = (size_t)kCols * 4 * ((a.n_seen > 0) + (a.n_bias > 0)) + kCols / 8 + 16;
+    const uintptr_t lie = (uintptr_t)a.in | (uintptr_t)(a.ld * sizeof(T));
+    const bool alike = ((uintptr_t)a.in - (uintptr_t)a.out) % 16 == 0 && (a.ld - a.ld_out) * (int64_t)sizeof(T) % 16 == 0;
+    auto kernel = !alike          ? score_rules_kernel<T, kElements>
+                  : lie % 16 == 0 ? score_rules_kernel<T, kAligned>
+                                  : score_rules_kernel<T, kShifted>;
     kernel<<<(unsigned)(chunks * a.Q), kThreads, smem, stream>>>(a, (int)chunks);
     return cudaGetLastError();
 }

@@ -90,15 +90,6 @@ __device__ __forceinline__ void pick_digit(Shared& sh, int want) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ T from_bits(uint32_t b);
-template <>
-__device__ __forceinline__ float from_bits<float>(uint32_t b) { return __uint_as_float(b); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_bits<__nv_bfloat16>(uint32_t b) { return __ushort_as_bfloat16((unsigned short)b); }
-template <>
-__device__ __forceinline__ __half from_bits<__half>(uint32_t b) { return __ushort_as_half((unsigned short)b); }
-
 // The larger of each of two pairs of 16-bit scores (NaN counts as nothing), and of the two of one.
 template <typename T>
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
@@ -192,23 +183,36 @@ __device__ void finish_row(Shared& sh, int q, const TopkArgs& a) {
         __syncthreads();
         if (part == 0 && key && sh.notes[mine] < (uint32_t)a.k) write((int)sh.notes[mine], key);
     } else {
-        for (int i = cnt + tid; i < n2; i += kThreads) sh.keys[i] = 0;
+        // bitonic, descending; thread t holds keys 2 t and 2 t + 1, partners in its warp by shuffles
         __syncthreads();
-        for (int w = 2; w <= n2; w <<= 1)      // bitonic, descending
-            for (int j = w >> 1; j > 0; j >>= 1) {
-                for (int i = tid; i < n2; i += kThreads) {
-                    const int p = i ^ j;
-                    if (p > i) {
-                        const uint64_t x = sh.keys[i], y = sh.keys[p];
-                        if ((x < y) == ((i & w) == 0)) {
-                            sh.keys[i] = y;
-                            sh.keys[p] = x;
-                        }
-                    }
+        uint64_t x = 2 * tid < cnt ? sh.keys[2 * tid] : 0, y = 2 * tid + 1 < cnt ? sh.keys[2 * tid + 1] : 0;
+        for (int w = 2; w <= 2 * kThreads; w <<= 1) {
+            const bool down = (2 * tid & w) == 0;
+            for (int j = w >> 1; j > 1; j >>= 1) {
+                uint64_t ox, oy;
+                if (j >= 64) {
+                    __syncthreads();
+                    sh.keys[2 * tid] = x;
+                    sh.keys[2 * tid + 1] = y;
+                    __syncthreads();
+                    ox = sh.keys[2 * tid ^ j];
+                    oy = sh.keys[(2 * tid + 1) ^ j];
+                } else {
+                    ox = __shfl_xor_sync(0xffffffffu, x, j >> 1);
+                    oy = __shfl_xor_sync(0xffffffffu, y, j >> 1);
                 }
-                __syncthreads();
+                const bool larger = ((2 * tid & j) == 0) == down;
+                x = (x > ox) == larger ? x : ox;
+                y = (y > oy) == larger ? y : oy;
             }
-        for (int i = tid; i < min(cnt, a.k); i += kThreads) write(i, sh.keys[i]);
+            if ((x < y) == down) {
+                const uint64_t z = x;
+                x = y;
+                y = z;
+            }
+        }
+        if (2 * tid < min(cnt, a.k)) write(2 * tid, x);
+        if (2 * tid + 1 < min(cnt, a.k)) write(2 * tid + 1, y);
     }
     for (int i = cnt + tid; i < a.k; i += kThreads) write(i, 0);
 }
@@ -258,43 +262,34 @@ __device__ __forceinline__ void lower_bound_of_kth(Shared& sh, const uint32_t (&
     __syncthreads();
 }
 
-// One step in registers: U vectors of V scores a thread, vector u at column t0 + (u * kThreads + tid) * V
-// of the slice.
-// What lies past the end reads -inf; with vectors, the end is a multiple of V.
-template <typename T, bool VEC>
+// One step in registers: U vectors of V scores a thread, vector u at t0 + (u * kThreads + tid) * V of the
+// slice's whole 16-byte vectors.  What lies past their end reads -inf.
+template <typename T>
 struct Step {
-    static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    static constexpr int V = 16 / (int)sizeof(T);
     static constexpr int U = 8;
     static constexpr int kScores = kThreads * U * V;
-    static constexpr bool kPairs = VEC && sizeof(T) == 2;
+    static constexpr bool kPairs = sizeof(T) == 2;
     union {
-        uint4 raw[VEC ? U : 1];
+        uint4 raw[U];
         T v[U][V];
     };
 
     __device__ __forceinline__ Step() {}
     __device__ __forceinline__ void load(const T* cols, int t0, int end) {
+        constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int j = t0 + (u * kThreads + (int)threadIdx.x) * V;
-            if constexpr (VEC) {
-                const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-                raw[u] = make_uint4(none, none, none, none);
-                if (j < end) raw[u] = *reinterpret_cast<const uint4*>(cols + j);
-            } else {
-                v[u][0] = j < end ? cols[j] : from_bits<T>(sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u);
-            }
+            raw[u] = make_uint4(none, none, none, none);
+            if (j < end) raw[u] = *reinterpret_cast<const uint4*>(cols + j);
         }
     }
     __device__ __forceinline__ float best(int u) const {     // NaN counts as nothing
-        if constexpr (kPairs) {
+        if constexpr (kPairs)
             return max_of<T>(max2<T>(max2<T>(raw[u].x, raw[u].y), max2<T>(raw[u].z, raw[u].w)));
-        } else {
-            float m = -CUDART_INF_F;
-#pragma unroll
-            for (int i = 0; i < V; ++i) m = fmaxf(m, score_of<T>(v[u][i]));
-            return m;
-        }
+        else
+            return fmaxf(fmaxf(fmaxf(-CUDART_INF_F, v[u][0]), fmaxf(v[u][1], v[u][2])), v[u][3]);
     }
     __device__ __forceinline__ uint32_t reaching(float least) const {      // bit u: vector u holds such a score
         uint32_t hits = 0;
@@ -310,18 +305,18 @@ __device__ __forceinline__ void append(Shared& sh, float s, uint32_t col) {     
 }
 
 // Notes the flagged vectors of a step by number; counted, but not written, from kNotes on.
-template <typename T, bool VEC>
+template <typename T>
 __device__ __forceinline__ void note(Shared& sh, uint32_t hits, int t0) {
     for (; hits; hits &= hits - 1) {
         const int at = atomicAdd(&sh.noted, 1);
-        if (at < kNotes) sh.notes[at] = t0 / Step<T, VEC>::V + (__ffs(hits) - 1) * kThreads + threadIdx.x;
+        if (at < kNotes) sh.notes[at] = t0 / Step<T>::V + (__ffs(hits) - 1) * kThreads + threadIdx.x;
     }
 }
 
 // Appends the scores that reach `least` of the noted vectors, an element a thread.
-template <typename T, bool VEC>
+template <typename T>
 __device__ __forceinline__ void collect(Shared& sh, int noted, float least, const T* cols, uint32_t c0) {
-    constexpr int V = Step<T, VEC>::V;
+    constexpr int V = Step<T>::V;
     for (int i = threadIdx.x; i < noted * V; i += kThreads) {
         const int j = (int)sh.notes[i / V] * V + i % V;
         const float s = score_of<T>(cols[j]);
@@ -330,9 +325,9 @@ __device__ __forceinline__ void collect(Shared& sh, int noted, float least, cons
 }
 
 // Running maxima of four groups of a thread's columns: vectors g and g + 4 (g, g + 4, ...) of every step.
-template <typename T, bool VEC>
+template <typename T>
 struct Maxima {
-    static constexpr bool kPairs = Step<T, VEC>::kPairs;
+    static constexpr bool kPairs = Step<T>::kPairs;
     float m[4];
     uint32_t p[4];
 
@@ -343,9 +338,9 @@ struct Maxima {
             p[g] = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
         }
     }
-    __device__ __forceinline__ void add(const Step<T, VEC>& t) {
+    __device__ __forceinline__ void add(const Step<T>& t) {
 #pragma unroll
-        for (int u = 0; u < Step<T, VEC>::U; ++u) {
+        for (int u = 0; u < Step<T>::U; ++u) {
             if constexpr (kPairs)
                 p[u & 3] = max2<T>(p[u & 3], max2<T>(max2<T>(t.raw[u].x, t.raw[u].y), max2<T>(t.raw[u].z, t.raw[u].w)));
             else
@@ -355,24 +350,30 @@ struct Maxima {
     __device__ __forceinline__ uint32_t high(int g) const { return ord_of(kPairs ? fmaxf(m[g], max_of<T>(p[g])) : m[g]) >> 16; }
 };
 
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
 topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice, const int slots) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem);
-    using Scores = Step<T, VEC>;
+    using Scores = Step<T>;
     const int tid = threadIdx.x;
     const int q = blockIdx.x / splits, part = blockIdx.x % splits;
-    // columns [c0, c0 + len) of the row; whole vectors end at `end`, what is left takes a thread each
-    const int64_t c0 = part * slice;
-    const int len = c0 < a.n ? (int)(c0 + slice < a.n ? slice : a.n - c0) : 0, end = len - len % Scores::V;
-    const T* cols = static_cast<const T*>(a.in) + (size_t)q * a.ld + c0;
+    // Columns [c0, c0 + len) of the row: `head` of them up to a 16-byte boundary, whole vectors to `end`
+    // (counted from the boundary), and what is left; a thread each for the odd ones.
+    const int64_t row0 = part * slice;
+    const int len = row0 < a.n ? (int)(row0 + slice < a.n ? slice : a.n - row0) : 0;
+    const T* first = static_cast<const T*>(a.in) + (size_t)q * a.ld + row0;
+    const int head = min(len, (int)((16 - ((uintptr_t)first & 15)) % 16 / sizeof(T)));
+    const int end = (len - head) / Scores::V * Scores::V, left = len - head - end;
+    const T* cols = first + head;
+    const uint32_t c0 = (uint32_t)(row0 + head);
     if (splits > 1) cudaTriggerProgrammaticLaunchCompletion();
     if (tid == 0) sh.cnt = sh.noted = 0;
-    const bool has_rest = end + tid < len;
-    const float rest = has_rest ? score_of<T>(cols[end + tid]) : -CUDART_INF_F;
+    const int odd = tid < head ? tid - head : end + tid - 32;      // from the boundary
+    const bool has_odd = tid < head || (tid >= 32 && tid - 32 < left);
+    const float rest = has_odd ? score_of<T>(cols[odd]) : -CUDART_INF_F;
     Scores step;
-    Maxima<T, VEC> maxima;
+    Maxima<T> maxima;
     for (int t0 = 0; t0 < end; t0 += Scores::kScores) {
         step.load(cols, t0, end);
         maxima.add(step);
@@ -384,12 +385,12 @@ topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice, const 
     const bool in_registers = end <= Scores::kScores;
     for (int t0 = 0; t0 < end; t0 += Scores::kScores) {
         if (!in_registers) step.load(cols, t0, end);
-        note<T, VEC>(sh, step.reaching(bound), t0);
+        note<T>(sh, step.reaching(bound), t0);
     }
     __syncthreads();
     const int noted = sh.noted;
-    if (noted <= kNotes) collect<T, VEC>(sh, noted, bound, cols, (uint32_t)c0);
-    if (has_rest && rest >= bound) append(sh, rest, (uint32_t)(c0 + end + tid));
+    if (noted <= kNotes) collect<T>(sh, noted, bound, cols, c0);
+    if (has_odd && rest >= bound) append(sh, rest, c0 + (uint32_t)odd);
     __syncthreads();
     if (noted > kNotes || sh.cnt > kCap) {
         // many equal scores: a vector a thread at a time, the buffer cut whenever the next might not fit
@@ -400,8 +401,8 @@ topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice, const 
             const float least = sh.least;
             for (int i = 0; i < Scores::V; ++i) {
                 const int j = t0 + tid * Scores::V + i;
-                const float s = j < len ? score_of<T>(cols[j]) : -CUDART_INF_F;
-                if (s >= least) append(sh, s, (uint32_t)(c0 + j));
+                const float s = j < len ? score_of<T>(first[j]) : -CUDART_INF_F;
+                if (s >= least) append(sh, s, (uint32_t)(row0 + j));
             }
             __syncthreads();
             const int cnt = sh.cnt;
@@ -476,12 +477,11 @@ int topk_splits(int Q, int64_t n, int k, int bytes, int sm_count) {
 
 template <typename T>
 cudaError_t launch_topk_t(const TopkArgs& a, int splits, cudaStream_t stream) {
-    const bool vec = ((uintptr_t)a.in | (uintptr_t)(a.ld * sizeof(T))) % 16 == 0;
-    auto kernel = vec ? topk_scan_kernel<T, true> : topk_scan_kernel<T, false>;
-    static std::atomic<uint64_t> granted[2];
-    cudaError_t e = grant_smem(kernel, (int)sizeof(Shared), granted[vec]);
+    auto kernel = topk_scan_kernel<T>;
+    static std::atomic<uint64_t> granted;
+    cudaError_t e = grant_smem(kernel, (int)sizeof(Shared), granted);
     if (e != cudaSuccess) return e;
-    // slices start at multiples of 8 scores, so 16-byte loads stay aligned
+    // slices start at multiples of 8 scores: as far from a 16-byte boundary as their row
     const int64_t slice = ((a.n + splits - 1) / splits + 7) / 8 * 8;
     kernel<<<(unsigned)((int64_t)a.Q * splits), kThreads, sizeof(Shared), stream>>>(a, splits, slice, slots_of(a.k));
     return cudaGetLastError();
