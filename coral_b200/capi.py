@@ -159,15 +159,17 @@ def _ptr(x, dtype):
 
 
 _torch = None
+_raw_stream = None
 _score_types = {}
 
 
 def _use_torch():
     """torch, imported when the first operator on score rows runs (the rest of the binding takes numpy)."""
-    global _torch
+    global _torch, _raw_stream
     if _torch is None:
         import torch
         _score_types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+        _raw_stream = torch._C._cuda_getCurrentRawStream
         _torch = torch
     return _torch
 
@@ -185,6 +187,7 @@ class Index:
         self.n, self.dim, self.max_degree = int(n), int(dim), int(max_degree)
         self.metric = {"l2": L2, "ip": IP, L2: L2, IP: IP}[metric]
         self._keep = []
+        self._topk_bytes = {}      # workspace sizes by shape
         rc = self._lib.coral_index_create(C.byref(self._h), device, self.n, self.dim, self.max_degree, self.metric)
         if rc != OK:
             msg = self._lib.coral_last_error(None).decode()
@@ -472,12 +475,9 @@ class Index:
         self._check(self._lib.coral_map_ids(self._h, C.c_void_p(d_ids.data_ptr()), int(d_ids.numel()),
                                             C.c_void_p(d_id_map.data_ptr()), C.c_void_p(stream) if stream else None))
 
-    # ---- operators on score rows: CUDA tensors, enqueued on torch's current stream of the handle's device
-    def _stream(self):
-        """torch's default stream, whose handle is 0, is CUDA's legacy stream (1): in the C calls 0 stands
-        for the handle's own stream."""
-        return _torch._C._cuda_getCurrentRawStream(self.device) or 1
-
+    # ---- operators on score rows: CUDA tensors, enqueued on torch's current stream of the handle's device.
+    # torch's default stream, whose handle is 0, is CUDA's legacy stream (1): in the C calls 0 stands for
+    # the handle's own stream.
     def _at(self, name: str, t, dtype, shape):
         """The address of a contiguous tensor of this type and shape on the handle's GPU."""
         try:
@@ -517,7 +517,9 @@ class Index:
         else:
             pc = self._at("codes", out[0], torch.float8_e4m3fn, codes)
             ps = self._at("scales", out[1], torch.float8_e8m0fnu, scales)
-        self._check(self._lib.coral_fp8_quantize(self._h, p, kind, rows, dim, ld, pc, ps, self._stream()))
+        rc = self._lib.coral_fp8_quantize(self._h, p, kind, rows, dim, ld, pc, ps, _raw_stream(self.device) or 1)
+        if rc:
+            self._check(rc)
         return out
 
     def fp8_scores(self, queries, base, dim: int, alpha: float = 1.0, bias=None, dtype=None, out=None):
@@ -538,15 +540,24 @@ class Index:
             # rows start at multiples of 16 bytes whatever n: what follows loads and stores whole vectors
             dtype = dtype or torch.float32
             per = 16 // dtype.itemsize
-            out = base[0].new_empty((Q, (n + per - 1) // per * per), dtype=dtype)
-            if out.shape[1] != n:
+            ld = (n + per - 1) // per * per
+            kind = _score_types.get(dtype)
+            if kind is None:
+                _refuse("dtype", "float32, bfloat16 or float16")
+            out = base[0].new_empty((Q, ld), dtype=dtype)
+            po = out.data_ptr()
+            if ld != n:
                 out = out[:, :n]
-        elif dtype is not None and out.dtype is not dtype:
-            _refuse("out", str(dtype))
-        po, kind, rows, cols, ld = self._rows("out", out)
-        if rows != Q or cols != n:
-            _refuse("out", f"of shape {[Q, n]}")
-        self._check(self._lib.coral_fp8_scores(self._h, pq, sq, Q, pr, sr, n, dim, alpha, pb, po, kind, ld, self._stream()))
+        else:
+            if dtype is not None and out.dtype is not dtype:
+                _refuse("out", str(dtype))
+            po, kind, rows, cols, ld = self._rows("out", out)
+            if rows != Q or cols != n:
+                _refuse("out", f"of shape {[Q, n]}")
+        rc = self._lib.coral_fp8_scores(self._h, pq, sq, Q, pr, sr, n, dim, alpha, pb, po, kind, ld,
+                                        _raw_stream(self.device) or 1)
+        if rc:
+            self._check(rc)
         return out
 
     def adjust_scores(self, scores, seen=None, penalties=None, bias_ids=None, bias=None, excluded=None, out=None):
@@ -557,8 +568,13 @@ class Index:
         torch = _torch or _use_torch()
         p, kind, Q, n, ld = self._rows("scores", scores)
         if out is None:
-            out = torch.empty_strided((Q, n), (ld, 1), dtype=scores.dtype, device=scores.device)
-            po, ld_out = out.data_ptr(), ld
+            # rows as far apart as the input's are when that is tight, else at multiples of 16 bytes
+            per = 16 // scores.dtype.itemsize
+            ld_out = n if ld == n else (n + per - 1) // per * per
+            out = scores.new_empty((Q, ld_out))
+            po = out.data_ptr()
+            if ld_out != n:
+                out = out[:, :n]
         else:
             po, kind_out, rows, cols, ld_out = self._rows("out", out)
             if rows != Q or cols != n or kind_out != kind:
@@ -584,8 +600,10 @@ class Index:
             one = _is_torch(excluded) and excluded.dim() == 2 and excluded.shape[0] == 1
             pe = self._at("excluded", excluded, torch.int32, (1 if one else Q, words))
             ld_ex = 0 if one else words
-        self._check(self._lib.coral_adjust_scores(self._h, p, kind, Q, n, ld, ps, n_seen, pp, pi, pb, n_bias, pe, ld_ex, po,
-                                                  ld_out, self._stream()))
+        rc = self._lib.coral_adjust_scores(self._h, p, kind, Q, n, ld, ps, n_seen, pp, pi, pb, n_bias, pe, ld_ex, po,
+                                           ld_out, _raw_stream(self.device) or 1)
+        if rc:
+            self._check(rc)
         return out
 
     def topk_scores(self, scores, k: int, id_base: int = 0):
@@ -595,14 +613,20 @@ class Index:
         p, kind, Q, n, ld = self._rows("scores", scores)
         if not (0 <= k < 2 ** 31 and 0 <= id_base <= 2 ** 31 - 1 - n):      # what a C int cannot hold
             raise CoralError(ERR_ARG, "k must be in [1, 1024] and id_base in [0, 2^31 - n)")
-        need = C.c_int64(0)
-        self._check(self._lib.coral_topk_workspace(self._h, Q, n, k, C.byref(need)))
-        size = need.value
+        size = self._topk_bytes.get((Q, n, k))
+        if size is None:
+            need = C.c_int64(0)
+            self._check(self._lib.coral_topk_workspace(self._h, Q, n, k, C.byref(need)))
+            if len(self._topk_bytes) >= 256:
+                self._topk_bytes.clear()
+            size = self._topk_bytes[Q, n, k] = need.value
         ids = scores.new_empty((Q, k), dtype=torch.int32)
         best = scores.new_empty((Q, k), dtype=torch.float32)
         ws = scores.new_empty((size,), dtype=torch.uint8) if size else None
-        self._check(self._lib.coral_topk_scores(self._h, p, kind, Q, n, ld, k, id_base, ids.data_ptr(), best.data_ptr(),
-                                                ws.data_ptr() if size else None, size, self._stream()))
+        rc = self._lib.coral_topk_scores(self._h, p, kind, Q, n, ld, k, id_base, ids.data_ptr(), best.data_ptr(),
+                                         ws.data_ptr() if size else None, size, _raw_stream(self.device) or 1)
+        if rc:
+            self._check(rc)
         return ids, best
 
     def scores_check(self):

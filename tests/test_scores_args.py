@@ -31,7 +31,7 @@ def test_a_null_handle_is_refused():
 def test_the_binding_refuses_before_it_calls():
     """CPU tensors, types and shapes are refused without a device."""
     ix = object.__new__(capi.Index)
-    ix._lib, ix._h, ix.device = capi.load(), None, 0
+    ix._lib, ix._h, ix.device, ix._topk_bytes = capi.load(), None, 0, {}
     x = torch.zeros(4, 64)
     for call in (lambda: ix.fp8_quantize(x), lambda: ix.fp8_scores((x, x), (x, x), 64), lambda: ix.fp8_scores((x, x), (x, x), 0),
                  lambda: ix.adjust_scores(x), lambda: ix.topk_scores(x, 3)):
