@@ -569,3 +569,110 @@ def test_c_refusals(ix):
         assert lib.coral_topk_scores(h, *bad, 1) == code, i
     torch.cuda.synchronize()
     assert lib.coral_scores_check(h) == OK
+
+
+# ------------------------------------------------------------------------------------ far and empty
+def test_offsets_past_32_bits(ix):
+    """Rows 1.2e9 elements apart: the third row starts past 2^31 elements (and 2^32 bytes)."""
+    ld, n, dim = 1_200_000_000, 1003, 200
+    g = gen(71)
+    whole = torch.zeros(3, ld, dtype=BF16, device="cuda")
+    x = whole[:, :dim]
+    x.copy_(torch.randn(3, dim, generator=g, device="cuda").to(BF16))
+    codes, scales = ix.fp8_quantize(x)
+    want, want_scales = plain_quantize(x)
+    same_codes(codes, want)
+    assert torch.equal(scales.view(torch.uint8), want_scales)
+    base = rows8(ix, n, dim, 72, 2)
+    out = whole[:, 5000:5000 + n]                                     # 16-byte rows: tensor stores
+    ix.fp8_scores((codes, scales), base, dim, out=out)
+    check_scores(out, (codes, scales), base, dim, 1.0, None)
+    odd = whole[:, 20_001:20_001 + n]
+    ix.fp8_scores((codes, scales), base, dim, out=odd)
+    assert torch.equal(odd, out)
+    ex = words(g, 3, n, 0.3)
+    seen = torch.randint(0, n, (3, 50), generator=g, device="cuda", dtype=torch.int32)
+    pen = torch.tensor([[1.2, 0.1, 0.2]], device="cuda").repeat(3, 1)
+    there = whole[:, 30_000:30_000 + n]
+    check_rules(ix, out, seen, pen, excluded=ex, out=there)
+    check_topk(ix, there, 30)
+    del whole
+    torch.cuda.empty_cache()
+
+
+def test_many_rows(ix):
+    """More rows than a grid's second dimension has: row offsets and block indexes."""
+    x = torch.randn(300_000, 7, generator=gen(73), device="cuda")
+    check_topk(ix, x[:70_000], 2)
+    ids, best = ix.topk_scores(x, 1)
+    assert torch.equal(best[:, 0], x.amax(1)) and torch.equal(ids[:, 0].long(), x.argmax(1))
+    ex = torch.zeros(300_000, 1, dtype=torch.int32, device="cuda")
+    ex[::2] = 5
+    got = ix.adjust_scores(x, excluded=ex)
+    want = x.clone()
+    want[::2, 0] = want[::2, 2] = -float("inf")
+    assert torch.equal(got, want)
+
+
+def test_empty_sizes(ix):
+    for dtype in TYPES:
+        codes, scales = ix.fp8_quantize(torch.zeros(0, 200, dtype=dtype, device="cuda"))
+        assert codes.shape == (0, 208) and scales.shape == (0, 4)
+        some = ix.fp8_quantize(torch.ones(5, 200, dtype=dtype, device="cuda"))
+        assert ix.fp8_scores((codes, scales), some, 200, dtype=dtype).shape == (0, 5)
+        none = ix.fp8_scores(some, (codes, scales), 200, dtype=dtype)
+        assert none.shape == (5, 0)
+        assert ix.adjust_scores(none, excluded=torch.zeros(1, 0, dtype=torch.int32, device="cuda")).shape == (5, 0)
+        x = torch.randn(4, 9, device="cuda").to(dtype)
+        got = ix.adjust_scores(x, torch.zeros(4, 0, dtype=torch.int32, device="cuda"), torch.ones(4, 3, device="cuda"),
+                               torch.zeros(4, 0, dtype=torch.int32, device="cuda"), torch.zeros(4, 0, device="cuda"))
+        assert torch.equal(got, x)
+        ids, best = ix.topk_scores(x[:0], 3)
+        assert ids.shape == (0, 3) and best.shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_topk_of_slices(ix, dtype):
+    """Rows that start anywhere between two 16-byte boundaries, long and short."""
+    for n, k in ((1, 1), (5, 3), (37, 40), (9001, 50), (70_003, 300)):
+        whole = torch.randn(5, n + 11, generator=gen(n), device="cuda").to(dtype)
+        for lead in (0, 1, 3, 6):
+            check_topk(ix, whole[:, lead:lead + n], k)
+
+
+def test_topk_bounds(ix):
+    """Ranges far apart, so that the bound takes its coarser steps, and few scores above the rest."""
+    n = 30_000
+    j = torch.arange(n, device="cuda", dtype=F32)
+    for x in (torch.exp2(j % 250 - 125) * torch.where(j % 2 == 0, 1.0, -1.0), torch.exp2(-(j % 140)), -torch.exp2(j % 120),
+              torch.where(j % 3000 == 7, 1e30, j * 1e-6), torch.where(j % 3000 == 7, float("inf"), -j)):
+        for k in (1, 20, 300, 1000):
+            check_topk(ix, x[None].contiguous(), k)
+
+
+def test_first_use_inside_a_capture():
+    """A process whose very first operator calls are captured (no warm-up that loads the kernels)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from coral_b200 import capi
+ix = capi.Index(1, 4, 32, "ip")
+x = torch.randn(6, 3000, device="cuda"); rows = torch.randn(700, 3000, device="cuda")
+ex = torch.zeros(1, 22, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    base = ix.fp8_quantize(rows)
+    s = ix.fp8_scores(ix.fp8_quantize(x), base, 3000)
+    ids, best = ix.topk_scores(ix.adjust_scores(s, excluded=ex), 5)
+g.replay(); torch.cuda.synchronize(); ix.scores_check()
+want = torch.topk(ix.fp8_scores(ix.fp8_quantize(x), ix.fp8_quantize(rows), 3000), 5)
+torch.cuda.synchronize()
+assert torch.equal(best, want.values) and torch.equal(ids.long(), want.indices)
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
