@@ -225,7 +225,7 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // out[q][j] = alpha * sum_b 2^(eq_b + ej_b) * (codes of q, codes of j)_b + bias[j], accumulated in
 // fp32 in tensor memory.  One persistent CTA of 12 warps per SM, tiles of 128 queries x 256 rows:
 //   warp 0     one lane issues the tiles' TMA loads (128-byte swizzle, 128 columns a stage).  A query
-//              tile of at most kStages k-blocks is kept while the next row tile meets it too: with few
+//              tile of no more k-blocks than stages is kept while the next row tile meets it too: with few
 //              k-blocks the tensor copies, which take their time per row, are what a tile waits for;
 //   warp 1     one lane issues, per stage, four tcgen05.mma (M = 128, N = 256, K = 32) and, per four
 //              stages, three tcgen05.cp (their scales to tensor memory);
@@ -242,25 +242,37 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 //
 // Tensor memory: two accumulators of 256 columns that share 64 (0-255 and 192-447) and, from 448,
 // four slots of 16 columns of scales.  A slot is written again four groups, so at least four stages,
-// later; that stage's codes have landed, so the products of the stage kStages before it are done, and
+// later; that stage's codes have landed, so the products of the stage S <= 4 before it are done, and
 // with them the slot's old ones.  The epilogue reads the shared columns first and then
 // lets the next tile's products start.
 
 constexpr int kTileM = 128, kTileN = 256, kTileK = 128;
-constexpr int kStages = 3;
 constexpr int kABytes = kTileM * kTileK, kBBytes = kTileN * kTileK;
 constexpr int kScaleBytes = (kTileM + kTileN) * 4;
 constexpr int kAccStep = 192, kShared = 64, kTmemScales = 448;
-constexpr int kOffB = kStages * kABytes;                            // query tiles first, then row tiles
-constexpr int kOffScales = kStages * (kABytes + kBBytes);
-constexpr int kEpiWarps = 8, kOutBufs = 2;
 constexpr int kScaleSlots = 8, kScalesAhead = 6;                    // groups in the ring, and in flight
-static_assert(kStages <= 4, "scale slots in tensor memory");
-constexpr int kOffOut = kOffScales + kScaleSlots * kScaleBytes;
-static_assert(kOffOut % 1024 == 0, "swizzled staging");
-constexpr int kOffBias = kOffOut + kEpiWarps * kOutBufs * 4096;     // each warp the biases of its columns
-constexpr int kOffBars = kOffBias + kEpiWarps * (kTileN / 2) * 4;
-constexpr int kSmemBytes = kOffBars + 256 + 1024;
+constexpr int kEpiWarps = 8;
+constexpr int kFewQueries = 32;       // up to here, with more than two k-blocks, four stages, else three
+
+// Shared memory of a kernel with S stages.  Three leave every epilogue warp two pieces of output in
+// flight.  A fourth is worth more where the base's bytes are all the time there is, with few queries:
+// what is in flight over the loaded latency of memory, about 2 us, bounds the rate (1 x 1M x 512 under a
+// power cap that holds the SMs at 1.5 GHz: 91 us with three, 87 with four).  Then only the warps of the
+// first 32 rows store (with one piece in flight for 64 rows, 64 x 1M x 512 took 137 us, not 130), and
+// with one or two k-blocks a tile the epilogue is what takes the time (1 x 2M x 256: 88 and 92 us).
+template <int S>
+struct Layout {
+    static constexpr int kOffB = S * kABytes;                       // query tiles first, then row tiles
+    static constexpr int kOffScales = S * (kABytes + kBBytes);
+    static constexpr int kOffOut = kOffScales + kScaleSlots * kScaleBytes;
+    static constexpr int kOutBytes = (S == 3 ? kEpiWarps : 2) * 2 * 4096;
+    static constexpr int kOffBias = kOffOut + kOutBytes;            // each warp the biases of its columns
+    static constexpr int kOffBars = kOffBias + kEpiWarps * (kTileN / 2) * 4;
+    static constexpr int kBytes = kOffBars + 256 + 1024;
+    static_assert(S <= 4, "scale slots in tensor memory");
+    static_assert(kOffOut % 1024 == 0, "swizzled staging");
+    static_assert(kBytes <= 232448, "shared memory");
+};
 constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr int64_t kChunkBytes = 32ll << 20;      // base bytes per chunk of tiles: a quarter of L2
 constexpr long long kWaitClocks = 4000000000ll;                     // ~2 s
@@ -462,16 +474,17 @@ constexpr int kSplit = 2;      // the tile's k-blocks are split over the CTAs of
 // columns it owns and stores them.  The same additions in every run.  (Reading a row's 16-byte pieces
 // side by side: written to the owner by the threads that hold them, a piece of 32 rows each, the parts
 // take five times as long.)
-template <typename T, int OUT>
+template <typename T, int OUT, int S>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const TileOrder order,
                   const int a_rows, const int row_bytes, const bool keeps_a) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);   // [kStages] codes landed
-    uint64_t* empty = full + kStages;                                // [kStages] the products that read the stage are done
-    uint64_t* sfull = empty + kStages;                               // [kScaleSlots] a group's scales landed
+    using L = Layout<S>;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);   // [S] codes landed
+    uint64_t* empty = full + S;                                      // [S] the products that read the stage are done
+    uint64_t* sfull = empty + S;                                     // [kScaleSlots] a group's scales landed
     uint64_t* sempty = sfull + kScaleSlots;                          // [kScaleSlots] and are no longer needed
     uint64_t* afull = sempty + kScaleSlots;                          // a kept query tile landed
     uint64_t* aempty = afull + 1;                                    // the products that read it are done
@@ -491,7 +504,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const int k_end = SPLIT ? min(k_blocks, (int)(groups * (rank + 1) / parts) * 4) : k_blocks;
 
     if (tid == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -507,6 +520,12 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    // Query rows that are not loaded stay zero: products with whatever lay there would be as wrong to
+    // store, but cost power, and with it clock.
+    for (int i = a_rows * row_bytes + tid * 16; i < kTileM * row_bytes; i += kThreads * 16)
+#pragma unroll
+        for (int s = 0; s < S; ++s) *reinterpret_cast<uint4*>(smem + s * kABytes + i) = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -530,8 +549,8 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
                     mbar_expect_tx(&full[s], ((keeps_a ? 0 : a_rows) + kTileN) * row_bytes);
                     if (!keeps_a) tma_load_2d(smem + s * kABytes, &map_a, kb * kTileK, (int)m0, &full[s]);
-                    tma_load_2d(smem + kOffB + s * kBBytes, &map_b, kb * kTileK, (int)n0, &full[s]);
-                    if (++s == kStages) {
+                    tma_load_2d(smem + L::kOffB + s * kBBytes, &map_b, kb * kTileK, (int)n0, &full[s]);
+                    if (++s == S) {
                         s = 0;
                         par ^= 1u;
                     }
@@ -549,7 +568,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
     } else if (warp == 1) {
         const uint32_t leads = elect_leader();
-        const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + kOffScales);
+        const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + L::kOffScales);
         const uint64_t desc = desc_rows(row_bytes);
         uint32_t s = 0, par = 0, i = 0, group = 0;
         bool ok = true;
@@ -586,7 +605,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     scales_to_tmem(leads, tb + 4, sc + (1024 >> 4));
                 }
                 const uint64_t da = desc_at(desc, codes + (keeps_a ? kb : s) * kABytes);
-                const uint64_t db = desc_at(desc, codes + kOffB + s * kBBytes);
+                const uint64_t db = desc_at(desc, codes + L::kOffB + s * kBBytes);
                 const uint32_t idesc = kInstrDesc | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
                 const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
                 if (slices == kTileK / 32) {
@@ -602,7 +621,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     umma_commit(leads, &sempty[slot]);
                     ++group;
                 }
-                if (++s == kStages) {
+                if (++s == S) {
                     s = 0;
                     par ^= 1u;
                 }
@@ -634,7 +653,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 const uint32_t slot = sent % kScaleSlots;
                 ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a.err));
                 if (!ok) break;
-                const uint32_t dst = smem_u32(smem + kOffScales + slot * kScaleBytes) + lane * 16;
+                const uint32_t dst = smem_u32(smem + L::kOffScales + slot * kScaleBytes) + lane * 16;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) copy(dst + g * 4, a.q_scales, m0 + g * 32 + lane, a.Q, kb);
 #pragma unroll
@@ -657,8 +676,9 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     } else if (warp >= 4) {
         const int g = warp & 3, half = (warp - 4) >> 2;      // 32 lanes of tensor memory; which of their two warps
         constexpr int W = 128 / (int)sizeof(T);              // columns of a piece
-        unsigned char* stage = smem + kOffOut + (warp - 4) * kOutBufs * 4096;
-        float* sbias = reinterpret_cast<float*>(smem + kOffBias) + (warp - 4) * (kTileN / 2);
+        // two pieces in flight a warp; with four stages only the first 32 rows' warps store
+        unsigned char* stage = smem + L::kOffOut + (S == 3 ? warp - 4 : half) * 2 * 4096;
+        float* sbias = reinterpret_cast<float*>(smem + L::kOffBias) + (warp - 4) * (kTileN / 2);
         constexpr int kTurn = 64, kTurns = kTileN / kTurn / 2;   // columns read at once; turns of a warp
         const uint32_t leads = elect_leader();
         uint64_t policy;
@@ -726,9 +746,9 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     }
                     if (TMA_OUT) {
                         constexpr int E = 16 / (int)sizeof(T);
-                        unsigned char* buf = stage + sent++ % kOutBufs * 4096;
+                        unsigned char* buf = stage + (sent++ & 1u) * 4096;
                         // the piece that used this buffer has left shared memory
-                        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kOutBufs - 1) : "memory");
+                        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                         __syncwarp();
 #pragma unroll
                         for (int u = 0; u < 8; ++u) {
@@ -902,7 +922,7 @@ int clusters_at_once(Kernel* kernel, int parts) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)parts);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.dynamicSmemBytes = Layout<4>::kBytes;
     cudaLaunchAttribute cluster = {};
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = (unsigned)parts;
@@ -972,21 +992,27 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     order.chunk_n = (uint32_t)(in_l2 < sm_count ? sm_count : in_l2);
     if (order.chunk_n > order.tiles_n) order.chunk_n = order.tiles_n;
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
-    static std::atomic<uint64_t> granted[3];
+    static std::atomic<uint64_t> granted[5];
     int parts = 1;
     if (order.tiles <= (uint32_t)sm_count && k_blocks > 4) {
-        cudaError_t e = grant_smem(fp8_scores_kernel<T, kSplit>, kSmemBytes, granted[kSplit]);
+        auto split = fp8_scores_kernel<T, kSplit, 4>;
+        cudaError_t e = grant_smem(split, Layout<4>::kBytes, granted[4]);
         if (e != cudaSuccess) return e;
-        parts = split_of(fp8_scores_kernel<T, kSplit>, order.tiles, k_blocks, sm_count);
+        parts = split_of(split, order.tiles, k_blocks, sm_count);
     }
-    const int out = parts > 1 ? kSplit : tma ? kTma : kPlain;
-    auto kernel = out == kSplit ? fp8_scores_kernel<T, kSplit> : out == kTma ? fp8_scores_kernel<T, kTma> : fp8_scores_kernel<T, kPlain>;
-    cudaError_t e = grant_smem(kernel, kSmemBytes, granted[out]);
-    if (e != cudaSuccess) return e;
+    const bool few = a.Q <= kFewQueries && k_blocks > 2;
+    const int stages = parts > 1 || few ? 4 : 3, smem = stages == 4 ? Layout<4>::kBytes : Layout<3>::kBytes;
+    auto kernel = parts > 1 ? fp8_scores_kernel<T, kSplit, 4>
+                  : tma     ? (few ? fp8_scores_kernel<T, kTma, 4> : fp8_scores_kernel<T, kTma, 3>)
+                            : (few ? fp8_scores_kernel<T, kPlain, 4> : fp8_scores_kernel<T, kPlain, 3>);
+    if (parts == 1) {
+        cudaError_t e = grant_smem(kernel, smem, granted[(tma ? 2 : 0) + (few ? 1 : 0)]);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(parts > 1 ? order.tiles * parts : order.tiles < (uint32_t)sm_count ? order.tiles : (uint32_t)sm_count);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute cluster = {};
     cluster.id = cudaLaunchAttributeClusterDimension;
@@ -994,7 +1020,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, order, a_rows, row_bytes, k_blocks <= kStages);
+    return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, order, a_rows, row_bytes, k_blocks <= stages);
 }
 
 }  // namespace
