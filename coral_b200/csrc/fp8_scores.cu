@@ -98,9 +98,11 @@ __device__ __forceinline__ float drop_infinities(uint4 (&v)[J]) {
 // A block of 128 columns belongs to G lanes, 16 columns each, in J loads of 16 bytes that the G lanes make
 // of consecutive bytes; its maximum takes log2 G shuffles.  G is 8, or fewer for rows of one block of
 // at most 64, 32 or 16 columns, which would leave the other lanes idle (800k x 14 bf16: 52 us with
-// eight).  A warp takes kQuantLoads / J steps of 32 / G consecutive blocks, all loads before the first
-// use, and writes the scales together.  Bound by memory.  (A block to a whole warp or half of one is bound by instructions instead: the few
-// values a lane then has carry the same addresses, bounds and exponents.)
+// eight, 11 with one).  A warp takes kQuantLoads / J steps of 32 / G consecutive blocks, all loads before the first
+// use, and writes the scales together.  Bound by memory: 1M x 512 fp32 takes 369 us, 2.56 GB at
+// 6.95 TB/s; 100003 x 200 bf16, cut from rows of 256, 16 us, 61 MB at 3.8 TB/s.  (A block
+// to a whole warp or half of one is bound by instructions instead, 435 and 22 us: the few values a
+// lane then has carry the same addresses, bounds and exponents.)
 template <typename T, bool VEC, int G>
 __global__ void __launch_bounds__(kQuantThreads)
 fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, uint8_t* __restrict__ codes,
@@ -240,6 +242,13 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // all four instructions of a stage name the same byte of the word (the scale ids of the instruction
 // descriptor), byte (k-block mod 4).
 //
+// What bounds it: the base's bytes with few queries (1 x 1M x 512: 82 us, 6.3 TB/s; 64 x 1M x 512 with
+// its 256 MB of scores: 126 us, 6.1 TB/s), the scores' bytes with many and short rows (4001 x 100003 x
+// 256 bf16: 193 us, 4.3 TB/s, where filling as much memory takes 203 us), and with many and long rows
+// shared memory: a stage's 48 KB arrive in 384 cycles and are read in another 384, against 512 cycles
+// of products (4096 x 8192 x 4096: 108 us alone, 2.5 PFLOP/s; 137 us under a power cap).  Pairs of SMs
+// on one tile would halve the row tile's share of that; not built.
+//
 // Tensor memory: two accumulators of 256 columns that share 64 (0-255 and 192-447) and, from 448,
 // four slots of 16 columns of scales.  A slot is written again four groups, so at least four stages,
 // later; that stage's codes have landed, so the products of the stage S <= 4 before it are done, and
@@ -332,12 +341,11 @@ __device__ __forceinline__ void tma_store_2d(uint32_t leads, const CUtensorMap* 
         "@q cp.async.bulk.commit_group;\n\t}" ::"l"(map), "r"(c0), "r"(c1), "r"(smem_u32(src)), "l"(policy), "r"(leads)
         : "memory");
 }
-// Shared-memory matrix descriptor, K-major rows of `row` = 128, 64 or 32 bytes with the swizzle of that
-// width: 8-row groups 8 * row bytes apart, descriptor version 1, layout type 2, 4 or 6.
-__device__ __forceinline__ uint64_t desc_rows(int row) {
-    return (1ull << 16) | ((uint64_t)(8 * row >> 4) << 32) | (1ull << 46) | ((row == 128 ? 2ull : row == 64 ? 4ull : 6ull) << 61);
+// Shared-memory matrix descriptor, K-major rows of 128 bytes with the 128-byte swizzle: 8-row groups
+// 1024 bytes apart, descriptor version 1, layout type 2.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t addr) { return desc | ((addr >> 4) & 0x3FFFu); }
 // The same for 32 unswizzled rows of 16 bytes (scales): 8-row groups 128 bytes apart.
 __device__ __forceinline__ uint64_t desc_rows16(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
@@ -426,7 +434,8 @@ __device__ __forceinline__ uint32_t pack2<float>(float lo, float) { return __flo
 
 // The order of the tiles: the base in chunks of `chunk_n` row tiles that stay in L2, per chunk all query
 // tiles, per query tile the chunk's row tiles.  Neighbouring CTAs then write neighbouring pieces of the
-// same output rows, which DRAM takes faster than the same bytes scattered over many rows.
+// same output rows, which DRAM takes faster than the same bytes scattered over many rows (4001 x 100003
+// x 128 bf16: 203 us, 254 with query tiles first; without the evict-first stores 233 and 277).
 struct TileOrder {
     uint32_t tiles, tiles_m, tiles_n, chunk_n;
     __device__ __forceinline__ void at(uint32_t t, int64_t& m0, int64_t& n0) const {
@@ -478,7 +487,7 @@ template <typename T, int OUT, int S>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ CUtensorMap map_out, const Fp8ScoresArgs a, const TileOrder order,
-                  const int a_rows, const int row_bytes, const bool keeps_a) {
+                  const int a_rows, const bool keeps_a) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     using L = Layout<S>;
@@ -522,7 +531,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
     // Query rows that are not loaded stay zero: products with whatever lay there would be as wrong to
     // store, but cost power, and with it clock.
-    for (int i = a_rows * row_bytes + tid * 16; i < kTileM * row_bytes; i += kThreads * 16)
+    for (int i = a_rows * kTileK + tid * 16; i < kTileM * kTileK; i += kThreads * 16)
 #pragma unroll
         for (int s = 0; s < S; ++s) *reinterpret_cast<uint4*>(smem + s * kABytes + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -547,7 +556,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 order.at(t, m0, n0);
                 for (int kb = k_first; kb < k_end; ++kb) {
                     if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
-                    mbar_expect_tx(&full[s], ((keeps_a ? 0 : a_rows) + kTileN) * row_bytes);
+                    mbar_expect_tx(&full[s], ((keeps_a ? 0 : a_rows) + kTileN) * kTileK);
                     if (!keeps_a) tma_load_2d(smem + s * kABytes, &map_a, kb * kTileK, (int)m0, &full[s]);
                     tma_load_2d(smem + L::kOffB + s * kBBytes, &map_b, kb * kTileK, (int)n0, &full[s]);
                     if (++s == S) {
@@ -560,7 +569,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     if (kept >= 0 && !(ok = mbar_wait(aempty, (kept_tiles - 1) & 1u, abort_flag, a.err))) break;
                     kept = m0;
                     ++kept_tiles;
-                    mbar_expect_tx(afull, k_blocks * a_rows * row_bytes);
+                    mbar_expect_tx(afull, k_blocks * a_rows * kTileK);
                     for (int kb = 0; kb < k_blocks; ++kb)
                         tma_load_2d(smem + kb * kABytes, &map_a, kb * kTileK, (int)m0, afull);
                 }
@@ -569,7 +578,6 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     } else if (warp == 1) {
         const uint32_t leads = elect_leader();
         const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + L::kOffScales);
-        const uint64_t desc = desc_rows(row_bytes);
         uint32_t s = 0, par = 0, i = 0, group = 0;
         bool ok = true;
         int64_t kept = -1;
@@ -604,8 +612,8 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     scales_to_tmem(leads, tb, sc + (512 >> 4));
                     scales_to_tmem(leads, tb + 4, sc + (1024 >> 4));
                 }
-                const uint64_t da = desc_at(desc, codes + (keeps_a ? kb : s) * kABytes);
-                const uint64_t db = desc_at(desc, codes + L::kOffB + s * kBBytes);
+                const uint64_t da = desc_sw128(codes + (keeps_a ? kb : s) * kABytes);
+                const uint64_t db = desc_sw128(codes + L::kOffB + s * kBBytes);
                 const uint32_t idesc = kInstrDesc | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
                 const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
                 if (slices == kTileK / 32) {
@@ -939,7 +947,9 @@ int clusters_at_once(Kernel* kernel, int parts) {
 }
 
 // CTAs that share a tile: the count with the shortest time in k-blocks a CTA goes through, one after the
-// other, a wave of shared tiles costing kSplitCost more for its start and its join.
+// other, a wave of shared tiles costing kSplitCost more for its start and its join.  Shared or not: 1 x
+// 1000 x 4096 6.8 or 16.7 us, 64 x 4096 x 4096 10 or 17, 128 x 2048 x 2048 10 or 12, 16 x 16384 x 2048
+// 12.5 or 14; against the rule, 200 x 3000 x 1000 12.9 or 11.
 constexpr int kSplitCost = 5;
 template <typename Kernel>
 int split_of(Kernel* kernel, uint32_t tiles, int k_blocks, int sm_count) {
@@ -968,16 +978,10 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     // (a row outside the matrix costs the tensor copy more than one inside it)
     const int a_rows = a.Q >= kTileM ? kTileM : (a.Q + 7) / 8 * 8;
     alignas(64) CUtensorMap map_a, map_b, map_out;
-    // bytes of a row in a stage: 128, or 32 or 64 where that holds the whole row (columns outside the
-    // matrix cost the tensor copy time, too)
-    const int row_bytes = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : kTileK;
-    const CUtensorMapSwizzle swizzle = row_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
-                                       : row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                         : CU_TENSOR_MAP_SWIZZLE_128B;
-    if (!matrix_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q_codes, a.Q, a.dim, fp8_code_pitch(a.dim), row_bytes, a_rows,
-                    swizzle) ||
-        !matrix_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.n, a.dim, fp8_code_pitch(a.dim), row_bytes, kTileN,
-                    swizzle))
+    if (!matrix_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q_codes, a.Q, a.dim, fp8_code_pitch(a.dim), kTileK, a_rows,
+                    CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !matrix_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.n, a.dim, fp8_code_pitch(a.dim), kTileK, kTileN,
+                    CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     if (!tma)
         map_out = map_a;      // not used
@@ -1020,7 +1024,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, order, a_rows, row_bytes, k_blocks <= stages);
+    return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, order, a_rows, k_blocks <= stages);
 }
 
 }  // namespace
