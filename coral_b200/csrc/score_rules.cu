@@ -71,6 +71,27 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
     float* bias = reinterpret_cast<float*>(smem) + (has_seen ? kCols : 0);
     uint32_t* touched = reinterpret_cast<uint32_t*>(smem) + kCols * ((has_seen ? 1 : 0) + (has_bias ? 1 : 0));
 
+    // column of an id in the CTA, at least cols for one outside it (modulo 2^32; n is below 2^31)
+    const auto column_of = [&](int32_t id) { return (uint32_t)id - (uint32_t)c0; };
+    // the beginnings of the lists, in flight with the masks
+    constexpr int kAhead = 8;
+    const int32_t* seen = a.seen + (size_t)q * a.n_seen;
+    const int32_t* bias_ids = a.bias_ids + (size_t)q * a.n_bias;
+    const float* bias_vals = a.bias + (size_t)q * a.n_bias;
+    int32_t ids_ahead[kAhead], bias_id = -1;
+    float bias_val = 0.f, rho = 1.f, phi = 0.f, pi = 0.f;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ids_ahead[i] = i * kThreads + tid < a.n_seen ? seen[i * kThreads + tid] : -1;
+    if (tid < 32 && lane < a.n_bias) {
+        bias_id = bias_ids[lane];
+        bias_val = bias_vals[lane];
+    }
+    if (has_seen) {
+        rho = a.penalties[(size_t)q * 3];
+        phi = a.penalties[(size_t)q * 3 + 1];
+        pi = a.penalties[(size_t)q * 3 + 2];
+    }
+
     // The thread's scores: U vectors of V, vector u at column head + (u * kThreads + tid) * V, and, of
     // shifted rows, at most one of the columns before the first and after the last whole vector.
     constexpr bool VEC = ROWS != kElements, SHIFTED = ROWS == kShifted;
@@ -114,25 +135,14 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
     T odd_in = from_f32<T>(-CUDART_INF_F);
     if (odd >= 0 && !odd_out) odd_in = in[odd];
 
-    float rho = 1.f, phi = 0.f, pi = 0.f;
     if (has_seen || has_bias) {
-        const int32_t* seen = has_seen ? a.seen + (size_t)q * a.n_seen : nullptr;
-        constexpr int kAhead = 8;      // ids of the history in flight while the tables are cleared
-        int32_t ids_ahead[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) ids_ahead[i] = i * kThreads + tid < a.n_seen ? seen[i * kThreads + tid] : -1;
-        if (has_seen) {
-            rho = a.penalties[(size_t)q * 3];
-            phi = a.penalties[(size_t)q * 3 + 1];
-            pi = a.penalties[(size_t)q * 3 + 2];
-        }
         const int words = (int)(touched - count) + kCols / 32 + 4;      // one word to spare behind the bits
         for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         if (has_seen) {
             auto add = [&](int32_t id) {
-                const int64_t j = (int64_t)id - c0;
-                if (j >= 0 && j < cols && atomicAdd(&count[j], 1u) == 0u) atomicOr(&touched[j >> 5], 1u << (j & 31));
+                const uint32_t j = column_of(id);
+                if (j < (uint32_t)cols && atomicAdd(&count[j], 1u) == 0u) atomicOr(&touched[j >> 5], 1u << (j & 31));
             };
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) add(ids_ahead[i]);
@@ -140,14 +150,16 @@ __global__ void __launch_bounds__(kThreads) score_rules_kernel(const RulesArgs a
             for (int i = kAhead * kThreads + tid; i < a.n_seen; i += kThreads) add(seen[i]);
         }
         if (has_bias && tid < 32) {
-            const int32_t* ids = a.bias_ids + (size_t)q * a.n_bias;
-            const float* vals = a.bias + (size_t)q * a.n_bias;
             for (int i0 = 0; i0 < a.n_bias; i0 += 32) {
-                const int i = i0 + lane;
-                const int64_t j = i < a.n_bias ? (int64_t)ids[i] - c0 : -1;
-                const bool mine = j >= 0 && j < cols;
+                const uint32_t j = column_of(bias_id);
+                const float val = bias_val;
+                if (i0 + 32 < a.n_bias) {      // the next ones in flight
+                    const int i = i0 + 32 + lane;
+                    bias_id = i < a.n_bias ? bias_ids[i] : -1;
+                    bias_val = i < a.n_bias ? bias_vals[i] : 0.f;
+                }
+                const bool mine = j < (uint32_t)cols;
                 if (!__any_sync(0xffffffffu, mine)) continue;
-                const float val = mine ? vals[i] : 0.f;
                 // entries of one id take turns, in list order; different ids go together
                 const uint32_t same = __match_any_sync(0xffffffffu, mine ? (int)j : -1 - lane);
                 const uint32_t before = __popc(same & ((1u << lane) - 1u));
