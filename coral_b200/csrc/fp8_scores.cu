@@ -242,7 +242,7 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // all four instructions of a stage name the same byte of the word (the scale ids of the instruction
 // descriptor), byte (k-block mod 4).
 //
-// What bounds it: the base's bytes with few queries (1 x 1M x 512: 82 us, 6.3 TB/s; 64 x 1M x 512 with
+// What bounds it: the base's bytes with not too many queries (64 x 1M x 512 with
 // its 256 MB of scores: 126 us, 6.1 TB/s), the scores' bytes with many and short rows (4001 x 100003 x
 // 256 bf16: 193 us, 4.3 TB/s, where filling as much memory takes 203 us), and with many and long rows
 // shared memory: a stage's 48 KB arrive in 384 cycles and are read in another 384, against 512 cycles
@@ -261,20 +261,14 @@ constexpr int kScaleBytes = (kTileM + kTileN) * 4;
 constexpr int kAccStep = 192, kShared = 64, kTmemScales = 448;
 constexpr int kScaleSlots = 8, kScalesAhead = 6;                    // groups in the ring, and in flight
 constexpr int kEpiWarps = 8;
-constexpr int kFewQueries = 32;       // up to here, with more than two k-blocks, four stages, else three
-
-// Shared memory of a kernel with S stages.  Three leave every epilogue warp two pieces of output in
-// flight.  A fourth is worth more where the base's bytes are all the time there is, with few queries:
-// what is in flight over the loaded latency of memory, about 2 us, bounds the rate (1 x 1M x 512 under a
-// power cap that holds the SMs at 1.5 GHz: 91 us with three, 87 with four).  Then only the warps of the
-// first 32 rows store (with one piece in flight for 64 rows, 64 x 1M x 512 took 137 us, not 130), and
-// with one or two k-blocks a tile the epilogue is what takes the time (1 x 2M x 256: 88 and 92 us).
+// Shared memory of a kernel with S stages: three leave every epilogue warp two pieces of output in
+// flight; the split kernel, which stores otherwise, has four.
 template <int S>
 struct Layout {
     static constexpr int kOffB = S * kABytes;                       // query tiles first, then row tiles
     static constexpr int kOffScales = S * (kABytes + kBBytes);
     static constexpr int kOffOut = kOffScales + kScaleSlots * kScaleBytes;
-    static constexpr int kOutBytes = (S == 3 ? kEpiWarps : 2) * 2 * 4096;
+    static constexpr int kOutBytes = S == 3 ? kEpiWarps * 2 * 4096 : 0;
     static constexpr int kOffBias = kOffOut + kOutBytes;            // each warp the biases of its columns
     static constexpr int kOffBars = kOffBias + kEpiWarps * (kTileN / 2) * 4;
     static constexpr int kBytes = kOffBars + 256 + 1024;
@@ -403,6 +397,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
 }
@@ -684,8 +687,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     } else if (warp >= 4) {
         const int g = warp & 3, half = (warp - 4) >> 2;      // 32 lanes of tensor memory; which of their two warps
         constexpr int W = 128 / (int)sizeof(T);              // columns of a piece
-        // two pieces in flight a warp; with four stages only the first 32 rows' warps store
-        unsigned char* stage = smem + L::kOffOut + (S == 3 ? warp - 4 : half) * 2 * 4096;
+        unsigned char* stage = smem + L::kOffOut + (warp - 4) * 2 * 4096;      // two pieces in flight a warp
         float* sbias = reinterpret_cast<float*>(smem + L::kOffBias) + (warp - 4) * (kTileN / 2);
         constexpr int kTurn = 64, kTurns = kTileN / kTurn / 2;   // columns read at once; turns of a warp
         const uint32_t leads = elect_leader();
@@ -883,6 +885,220 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
 }
 
+// ------------------------------------------------------------------------- product, few queries
+//
+// Up to 16 queries: the base rows take the products' M and the queries their N, so a tile is 256 base
+// rows (two products of M = 128, N = 16).  The products then cost a sixteenth of what a query tile of
+// mostly nothing would, and of its power (1 x 1M x 512 ran 97 us at the 1.5 GHz that it left), and a lane
+// holds one base row's scores, so a warp stores a query's 32 scores side by side straight from its
+// registers, at any alignment.  Bound by memory: 1 x 1M x 512 79 us, 6.6 TB/s; 1 x 4M x 128 83 us (a query
+// tile: 165); by the steps of a tile where its rows are short: 8 x 190k x 31 bf16 9.3 us (13.8).  With
+// more queries these stores lose to tensor stores (20 x 500k x 300 fp32: 46 us against 41).
+//
+// Four stages of 34 KB: with five 1 x 1M x 512 takes 83 us, with six 87; memory slows when more is asked
+// for at once.  Tensor memory: two buffers of 32 columns and, from 128, eight slots of 16 columns of
+// scales (as many slots as stages or more: see above).  Roles as above, epilogue warp 4 + 4 h + g for
+// rows 32 g .. 32 g + 31 of half h.
+constexpr int kFewQueries = 16, kFewStages = 4, kFewSlots = 8;
+constexpr int kFewBase = 256 * kTileK, kFewQ = kFewQueries * kTileK;
+constexpr int kFewOffQ = kFewStages * kFewBase;
+constexpr int kFewOffScales = kFewOffQ + kFewStages * kFewQ;
+constexpr int kFewOffBars = kFewOffScales + kScaleSlots * kScaleBytes;
+constexpr int kFewBytes = kFewOffBars + 256 + 1024;
+static_assert(kFewSlots >= kFewStages && kFewBytes <= 232448, "few queries");
+constexpr uint32_t kFewInstrDesc = (1u << 23) | ((uint32_t)(kFewQueries >> 3) << 17) | ((uint32_t)(kTileM >> 7) << 27);
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_b,
+                      const Fp8ScoresArgs a, const uint32_t tiles, const int q_rows) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFewOffBars);      // [kFewStages] codes landed
+    uint64_t* empty = full + kFewStages;                                   // [kFewStages] the products that read them are done
+    uint64_t* sfull = empty + kFewStages;                                  // [kScaleSlots] a group's scales landed
+    uint64_t* sempty = sfull + kScaleSlots;                                // [kScaleSlots] and are no longer needed
+    uint64_t* tfull = sempty + kScaleSlots;                                // [2] accumulator buffer complete
+    uint64_t* tfree = tfull + 2;                                           // [2] and drained
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // known to be uniform
+    const int k_blocks = (a.dim + kTileK - 1) / kTileK;
+    const int scale_pitch = (a.dim + 511) / 512 * 4;
+
+    if (tid == 0) {
+        for (int s = 0; s < kFewStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kScaleSlots; ++s) {
+            mbar_init(&sfull[s], 1);
+            mbar_init(&sempty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tfree[b], kEpiWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // query rows that are not loaded stay zero: their products are not stored, but cost power
+    for (int i = q_rows * kTileK + tid * 16; i < kFewQ; i += kThreads * 16)
+#pragma unroll
+        for (int s = 0; s < kFewStages; ++s)
+            *reinterpret_cast<uint4*>(smem + kFewOffQ + s * kFewQ + i) = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t par = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
+                    mbar_expect_tx(&full[s], kFewBase + q_rows * kTileK);
+                    tma_load_2d(smem + s * kFewBase, &map_b, kb * kTileK, (int)((int64_t)t * 256), &full[s]);
+                    tma_load_2d(smem + kFewOffQ + s * kFewQ, &map_q, kb * kTileK, 0, &full[s]);
+                    if (++s == kFewStages) {
+                        s = 0;
+                        par ^= 1u;
+                    }
+                }
+        }
+    } else if (warp == 1) {
+        const uint32_t leads = elect_leader();
+        const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + kFewOffScales);
+        uint32_t s = 0, par = 0, i = 0, group = 0;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
+            const uint32_t b = i & 1u;
+            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&tfree[b], ((i >> 1) - 1) & 1u, abort_flag, a.err))) break;
+            const uint32_t acc = tmem + b * 32;
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a.err));
+                if (!ok) break;
+                const uint32_t slot = group % kScaleSlots, ta = tmem + 128 + group % kFewSlots * 16, tb = ta + 8;
+                if ((kb & 3) == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a.err));
+                    if (!ok) break;
+                }
+                tc_fence_after();
+                if ((kb & 3) == 0) {
+                    const uint64_t sc = desc_rows16(scales + slot * kScaleBytes);
+                    scales_to_tmem(leads, ta, sc);
+                    scales_to_tmem(leads, ta + 4, sc + (512 >> 4));
+                    scales_to_tmem(leads, tb, sc + (1024 >> 4));
+                }
+                const uint64_t d0 = desc_sw128(codes + s * kFewBase), d1 = d0 + (128 * kTileK >> 4);
+                const uint64_t dq = desc_sw128(codes + kFewOffQ + s * kFewQ);
+                const uint32_t idesc = kFewInstrDesc | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
+                const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
+                for (int j = 0; j < slices; ++j) {
+                    umma_mxf8(leads, acc, d0 + j * 2, dq + j * 2, idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
+                    umma_mxf8(leads, acc + 16, d1 + j * 2, dq + j * 2, idesc, ta + 4, tb, (kb | j) != 0 ? 1u : 0u);
+                }
+                umma_commit(leads, &empty[s]);
+                if ((kb & 3) == 3 || kb == k_blocks - 1) {
+                    umma_commit(leads, &sempty[slot]);
+                    ++group;
+                }
+                if (++s == kFewStages) {
+                    s = 0;
+                    par ^= 1u;
+                }
+            }
+            if (ok) umma_commit(leads, &tfull[b]);
+        }
+    } else if (warp == 2) {
+        // as above: a group's words, base rows first, then the queries'
+        uint32_t sent = 0, done = 0;
+        bool ok = true;
+        auto publish = [&]() {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sfull[done % kScaleSlots]);
+            ++done;
+        };
+        auto copy = [&](uint32_t dst, const uint8_t* base, int64_t r, int64_t rows, int kb) {
+            const bool there = r < rows;      // else four zero bytes
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst),
+                         "l"(base + (there ? r * scale_pitch + kb : 0)), "r"(there ? 4 : 0)
+                         : "memory");
+        };
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+            for (int kb = 0; kb < k_blocks; kb += 4) {
+                const uint32_t slot = sent % kScaleSlots;
+                ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a.err));
+                if (!ok) break;
+                const uint32_t dst = smem_u32(smem + kFewOffScales + slot * kScaleBytes) + lane * 16;
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+                    copy(dst + (g >> 2) * 512 + (g & 3) * 4, a.scales, (int64_t)t * 256 + g * 32 + lane, a.n, kb);
+                copy(dst + 1024, a.q_scales, lane, a.Q, kb);      // rows from 16 on: zero, and not used
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (++sent - done > kScalesAhead) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kScalesAhead) : "memory");
+                    publish();
+                }
+            }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        while (ok && done < sent) publish();
+    } else if (warp >= 4) {
+        const int row = (warp - 4) * 32 + lane;      // of the tile: half (warp - 4) / 4, 32 lanes of tensor memory (warp & 3)
+        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)((warp - 4) >> 2) * 16;
+        uint32_t i = 0;
+        int64_t n = (int64_t)blockIdx.x * 256 + row;
+        float next_bias = a.bias && n < a.n ? a.bias[n] : 0.f;
+        for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+            const float bias = next_bias;
+            T* out = static_cast<T*>(a.out) + n;
+            const bool there = n < a.n;
+            n += (int64_t)gridDim.x * 256;
+            if (a.bias) next_bias = n < a.n ? a.bias[n] : 0.f;
+            const uint32_t b = i & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[b], i >> 1 & 1u, abort_flag, a.err))) break;
+            tc_fence_after();
+            uint32_t r[kFewQueries];
+            tmem_ld16(from + b * 32, r);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tfree[b]);
+#pragma unroll
+            for (int q = 0; q < kFewQueries; ++q) {
+                if (q >= a.Q) break;
+                if (there) *out = narrow<T>(fmaf(a.alpha, __uint_as_float(r[q]), bias));
+                out += a.ld;
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        // a wait ran out: give copies and products in flight time to land (bounded)
+        const long long t_end = clock64() + 20000000ll;
+        while (clock64() < t_end) {
+        }
+        __syncthreads();
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+    }
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -983,11 +1199,6 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
         !matrix_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.n, a.dim, fp8_code_pitch(a.dim), kTileK, kTileN,
                     CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
-    if (!tma)
-        map_out = map_a;      // not used
-    else if (!matrix_map(&map_out, type, a.out, a.Q, a.n, a.ld * (int64_t)sizeof(T), 128 / (int)sizeof(T), 32,
-                         CU_TENSOR_MAP_SWIZZLE_128B))
-        return cudaErrorInvalidValue;
     TileOrder order;
     order.tiles_m = (uint32_t)(((int64_t)a.Q + kTileM - 1) / kTileM);
     order.tiles_n = (uint32_t)(((int64_t)a.n + kTileN - 1) / kTileN);
@@ -996,21 +1207,31 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     order.chunk_n = (uint32_t)(in_l2 < sm_count ? sm_count : in_l2);
     if (order.chunk_n > order.tiles_n) order.chunk_n = order.tiles_n;
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
-    static std::atomic<uint64_t> granted[5];
+    static std::atomic<uint64_t> granted[4];
     int parts = 1;
     if (order.tiles <= (uint32_t)sm_count && k_blocks > 4) {
         auto split = fp8_scores_kernel<T, kSplit, 4>;
-        cudaError_t e = grant_smem(split, Layout<4>::kBytes, granted[4]);
+        cudaError_t e = grant_smem(split, Layout<4>::kBytes, granted[kSplit]);
         if (e != cudaSuccess) return e;
         parts = split_of(split, order.tiles, k_blocks, sm_count);
     }
-    const bool few = a.Q <= kFewQueries && k_blocks > 2;
-    const int stages = parts > 1 || few ? 4 : 3, smem = stages == 4 ? Layout<4>::kBytes : Layout<3>::kBytes;
-    auto kernel = parts > 1 ? fp8_scores_kernel<T, kSplit, 4>
-                  : tma     ? (few ? fp8_scores_kernel<T, kTma, 4> : fp8_scores_kernel<T, kTma, 3>)
-                            : (few ? fp8_scores_kernel<T, kPlain, 4> : fp8_scores_kernel<T, kPlain, 3>);
+    if (parts == 1 && a.Q <= kFewQueries) {
+        auto few = fp8_few_scores_kernel<T>;
+        cudaError_t e = grant_smem(few, kFewBytes, granted[3]);
+        if (e != cudaSuccess) return e;
+        few<<<order.tiles < (uint32_t)sm_count ? order.tiles : (uint32_t)sm_count, kThreads, kFewBytes, stream>>>(
+            map_a, map_b, a, order.tiles, a_rows);
+        return cudaGetLastError();
+    }
+    if (!tma)
+        map_out = map_a;      // not used
+    else if (!matrix_map(&map_out, type, a.out, a.Q, a.n, a.ld * (int64_t)sizeof(T), 128 / (int)sizeof(T), 32,
+                         CU_TENSOR_MAP_SWIZZLE_128B))
+        return cudaErrorInvalidValue;
+    const int stages = parts > 1 ? 4 : 3, smem = stages == 4 ? Layout<4>::kBytes : Layout<3>::kBytes;
+    auto kernel = parts > 1 ? fp8_scores_kernel<T, kSplit, 4> : tma ? fp8_scores_kernel<T, kTma, 3> : fp8_scores_kernel<T, kPlain, 3>;
     if (parts == 1) {
-        cudaError_t e = grant_smem(kernel, smem, granted[(tma ? 2 : 0) + (few ? 1 : 0)]);
+        cudaError_t e = grant_smem(kernel, smem, granted[tma ? kTma : kPlain]);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};

@@ -233,6 +233,23 @@ def test_scores_into_slices(ix, dtype, n, lead, ld):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Q,n,dim,lead,pad", [(1, 1, 1, 0, 0), (1, 255, 40, 1, 0), (15, 257, 128, 3, 5), (16, 60_001, 200, 0, 7),
+                                              (16, 60_000, 70, 8, 8), (17, 60_001, 200, 0, 7), (2, 40_000, 700, 5, 1),
+                                              (9, 38_000, 513, 2, 0)])
+def test_scores_of_few_queries(ix, dtype, Q, n, dim, lead, pad):
+    """Around the number of queries at which base rows and queries change sides."""
+    q, base = rows8(ix, Q, dim, 16, 3), rows8(ix, n, dim, 17, 3)
+    bias = torch.randn(n, generator=gen(18), device="cuda")
+    whole = torch.full((Q + 2, lead + n + pad), 77.0, dtype=dtype, device="cuda")
+    out = whole[1:Q + 1, lead:lead + n]
+    ix.fp8_scores(q, base, dim, 2.0 ** -9, bias, out=out)
+    check_scores(out, q, base, dim, 2.0 ** -9, bias)
+    out.fill_(77.0)
+    assert bool((whole == 77.0).all())
+    check_scores(ix.fp8_scores(q, base, dim, 0.5 ** 9, dtype=dtype), q, base, dim, 0.5 ** 9, None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("Q,n,dim", [(3, 700, 2100), (130, 513, 4096), (40, 257, 1100), (128, 300, 8200), (33, 1999, 3000)])
 @pytest.mark.parametrize("lead,pad", [(0, 0), (1, 2), (4, 4)])
 def test_scores_of_few_tiles(ix, dtype, Q, n, dim, lead, pad):
