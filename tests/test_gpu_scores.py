@@ -5,7 +5,9 @@ Tolerances.  Compression and selection are exact.  A product of two e4m3 codes i
 is scaling by a power of two, so a score's error is that of summing dim terms and of the epilogue's
 one fused multiply-add: at most dim + 2 roundings, each at most 2^-23 (a truncating adder) of the sum
 of magnitudes.  A rule row makes at most 5 + n_bias fp32 roundings (2^-24) of intermediate values that
-never exceed the sum of magnitudes.  Rounding to the output's type adds finfo.eps / 2 of the value."""
+never exceed the sum of magnitudes.  Rounding to the output's type adds finfo.eps / 2 of the value, or,
+below the smallest normal number, where the spacing is smallest_normal * eps whatever the value, half
+of that spacing (fp16: 2^-14 * 2^-10 / 2 = 2^-25, which scores of 1e-5 do meet)."""
 import numpy as np
 import pytest
 import torch
@@ -70,7 +72,8 @@ def check_scores(out, q, base, dim, alpha, bias):
     if bias is not None:
         want = want + bias.double()
         mag = mag + bias.double().abs()
-    tol = (dim + 2) * 2.0 ** -23 * mag + torch.finfo(out.dtype).eps / 2 * want.abs() * (1 + 2.0 ** -10) + 1e-37
+    fi = torch.finfo(out.dtype)
+    tol = (dim + 2) * 2.0 ** -23 * mag + fi.eps / 2 * (want.abs() * (1 + 2.0 ** -10) + fi.smallest_normal) + 1e-37
     err = (out.double() - want).abs()
     assert bool((err <= tol).all()), f"largest error / tolerance {float((err / tol).max()):.3g}"
 
