@@ -776,6 +776,13 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         tma_store_2d(leads, &map_out, (int)(n0 + col), (int)m0, buf, policy);
+                        // the columns after the last whole 16 bytes, which the tensor does not have
+                        const int64_t whole = a.n - a.n % E, u = (whole - n0 - col) / E;
+                        if (whole < a.n && u >= 0 && u < 8 && lane < rows) {
+                            const T* from = reinterpret_cast<const T*>(buf + lane * 128 + (((int)u ^ (lane & 7)) << 4));
+                            T* to = static_cast<T*>(a.out) + (m0 + lane) * a.ld + whole;
+                            for (int e = 0; e < (int)(a.n - whole); ++e) to[e] = from[e];
+                        }
                     } else {
                         float* tile = reinterpret_cast<float*>(stage);      // column j of row l at l * 32 + (j ^ l)
 #pragma unroll
@@ -1188,8 +1195,10 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     const CUtensorMapDataType type = a.type == kTypeF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : a.type == kTypeBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    // tensor stores need rows that start at 16-byte boundaries
-    const bool tma = ((uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T))) % 16 == 0;
+    // Tensor stores need rows that start at 16-byte boundaries, and write whole 16 bytes, past the
+    // tensor's end, too: the tensor they see ends with the last whole ones.
+    const int whole = a.n - a.n % (16 / (int)sizeof(T));
+    const bool tma = whole > 0 && ((uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T))) % 16 == 0;
     // rows of a query tile that are loaded: the others' products are not stored, whatever they are
     // (a row outside the matrix costs the tensor copy more than one inside it)
     const int a_rows = a.Q >= kTileM ? kTileM : (a.Q + 7) / 8 * 8;
@@ -1225,7 +1234,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     }
     if (!tma)
         map_out = map_a;      // not used
-    else if (!matrix_map(&map_out, type, a.out, a.Q, a.n, a.ld * (int64_t)sizeof(T), 128 / (int)sizeof(T), 32,
+    else if (!matrix_map(&map_out, type, a.out, a.Q, whole, a.ld * (int64_t)sizeof(T), 128 / (int)sizeof(T), 32,
                          CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     const int stages = parts > 1 ? 4 : 3, smem = stages == 4 ? Layout<4>::kBytes : Layout<3>::kBytes;

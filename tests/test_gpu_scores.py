@@ -222,7 +222,9 @@ def test_scores(ix, Q, n, dim, dtype, biased):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,lead,ld", [(256, 0, 256), (256, 1, 300), (999, 0, 999), (1000, 3, 1003), (1000, 8, 1008), (64, 0, 4096)])
+@pytest.mark.parametrize("n,lead,ld", [(256, 0, 256), (256, 1, 300), (999, 0, 999), (1000, 3, 1003), (1000, 8, 1008), (64, 0, 4096),
+                                       (999, 0, 1000), (1001, 8, 1032), (257, 0, 264), (250, 16, 512), (1, 0, 8), (5, 8, 24),
+                                       (767, 0, 768), (770, 0, 776)])
 def test_scores_into_slices(ix, dtype, n, lead, ld):
     """Any alignment of the output rows, and nothing outside them is written."""
     Q, dim = 130, 256
