@@ -478,7 +478,9 @@ __device__ __forceinline__ float4 load_peer(uint32_t addr) {
 // How a CTA stores its scores.
 constexpr int kPlain = 0;      // coalesced plain stores
 constexpr int kTma = 1;        // tensor stores
-constexpr int kSplit = 2;      // the tile's k-blocks are split over the CTAs of a cluster, see below
+constexpr int kTmaOdd = 2;     // the same, and the columns after a row's last whole 16 bytes plainly (apart
+                               // from kTma: the few instructions cost 17 x 2M x 100 fp32 87 -> 100 us)
+constexpr int kSplit = 3;      // the tile's k-blocks are split over the CTAs of a cluster, see below
 
 // With fewer tiles than SMs and many k-blocks, a cluster of 2, 4 or 8 CTAs shares a tile: rank r takes a
 // range of its k-blocks (whole groups of four).  Then every CTA lays its partial accumulator out in its
@@ -508,7 +510,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // known to be uniform
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
     const int scale_pitch = (a.dim + 511) / 512 * 4;
-    constexpr bool TMA_OUT = OUT == kTma, SPLIT = OUT == kSplit;
+    constexpr bool TMA_OUT = OUT == kTma || OUT == kTmaOdd, SPLIT = OUT == kSplit;
     const uint32_t rank = SPLIT ? cluster_rank() : 0, parts = SPLIT ? cluster_size() : 1;
     const uint32_t t_first = SPLIT ? blockIdx.x / parts : blockIdx.x, t_step = SPLIT ? order.tiles : gridDim.x;
     const int groups = (k_blocks + 3) / 4;
@@ -691,6 +693,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         float* sbias = reinterpret_cast<float*>(smem + L::kOffBias) + (warp - 4) * (kTileN / 2);
         constexpr int kTurn = 64, kTurns = kTileN / kTurn / 2;   // columns read at once; turns of a warp
         const uint32_t leads = elect_leader();
+        const int odd = a.n % (16 / (int)sizeof(T));      // columns after the last whole 16 bytes
         uint64_t policy;
         asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         uint32_t i = 0, sent = 0;
@@ -776,12 +779,13 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         tma_store_2d(leads, &map_out, (int)(n0 + col), (int)m0, buf, policy);
-                        // the columns after the last whole 16 bytes, which the tensor does not have
-                        const int64_t whole = a.n - a.n % E, u = (whole - n0 - col) / E;
-                        if (whole < a.n && u >= 0 && u < 8 && lane < rows) {
-                            const T* from = reinterpret_cast<const T*>(buf + lane * 128 + (((int)u ^ (lane & 7)) << 4));
-                            T* to = static_cast<T*>(a.out) + (m0 + lane) * a.ld + whole;
-                            for (int e = 0; e < (int)(a.n - whole); ++e) to[e] = from[e];
+                        if constexpr (OUT == kTmaOdd) {
+                            const uint32_t at = (uint32_t)(a.n - odd) - (uint32_t)(n0 + col);      // in the piece, or beyond W
+                            if (at < (uint32_t)W && lane < rows) {
+                                const T* from = reinterpret_cast<const T*>(buf + lane * 128 + ((at / E ^ (lane & 7)) << 4));
+                                T* to = static_cast<T*>(a.out) + (m0 + lane) * a.ld + (a.n - odd);
+                                for (int e = 0; e < odd; ++e) to[e] = from[e];
+                            }
                         }
                     } else {
                         float* tile = reinterpret_cast<float*>(stage);      // column j of row l at l * 32 + (j ^ l)
@@ -1216,7 +1220,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     order.chunk_n = (uint32_t)(in_l2 < sm_count ? sm_count : in_l2);
     if (order.chunk_n > order.tiles_n) order.chunk_n = order.tiles_n;
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
-    static std::atomic<uint64_t> granted[4];
+    static std::atomic<uint64_t> granted[5];
     int parts = 1;
     if (order.tiles <= (uint32_t)sm_count && k_blocks > 4) {
         auto split = fp8_scores_kernel<T, kSplit, 4>;
@@ -1226,7 +1230,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     }
     if (parts == 1 && a.Q <= kFewQueries) {
         auto few = fp8_few_scores_kernel<T>;
-        cudaError_t e = grant_smem(few, kFewBytes, granted[3]);
+        cudaError_t e = grant_smem(few, kFewBytes, granted[4]);
         if (e != cudaSuccess) return e;
         few<<<order.tiles < (uint32_t)sm_count ? order.tiles : (uint32_t)sm_count, kThreads, kFewBytes, stream>>>(
             map_a, map_b, a, order.tiles, a_rows);
@@ -1238,9 +1242,13 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
                          CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     const int stages = parts > 1 ? 4 : 3, smem = stages == 4 ? Layout<4>::kBytes : Layout<3>::kBytes;
-    auto kernel = parts > 1 ? fp8_scores_kernel<T, kSplit, 4> : tma ? fp8_scores_kernel<T, kTma, 3> : fp8_scores_kernel<T, kPlain, 3>;
+    const int out = !tma ? kPlain : whole < a.n ? kTmaOdd : kTma;
+    auto kernel = parts > 1         ? fp8_scores_kernel<T, kSplit, 4>
+                  : out == kTma     ? fp8_scores_kernel<T, kTma, 3>
+                  : out == kTmaOdd  ? fp8_scores_kernel<T, kTmaOdd, 3>
+                                    : fp8_scores_kernel<T, kPlain, 3>;
     if (parts == 1) {
-        cudaError_t e = grant_smem(kernel, smem, granted[tma ? kTma : kPlain]);
+        cudaError_t e = grant_smem(kernel, smem, granted[out]);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
