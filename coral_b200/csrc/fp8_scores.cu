@@ -312,7 +312,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
             if (*abort_flag) return false;
             if (clock64() - t0 > kWaitClocks) {
                 *abort_flag = 1;
-                atomicExch_system(err, 1);
+                *static_cast<volatile int*>(err) = 1;
+                __threadfence_system();
                 return false;
             }
         }
@@ -683,7 +684,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         while (ok && done < sent) publish();
     } else if (SPLIT) {
         if (warp >= 4) {
-            mbar_wait(tfull, 0, abort_flag, a.err);
+            __all_sync(0xffffffffu, mbar_wait(tfull, 0, abort_flag, a.err));
             tc_fence_after();
         }
     } else if (warp >= 4) {
@@ -818,7 +819,8 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         // the accumulator as [row][column], 16-byte pieces permuted by the row; the products that read
         // the stages' memory are done
         const int g = warp & 3, half = (warp - 4) >> 2, held = g * 32 + lane;
-        if (warp >= 4 && g * 32 < rows && !*abort_flag) {
+        const bool sound = __all_sync(0xffffffffu, !*abort_flag);
+        if (warp >= 4 && g * 32 < rows && sound) {
             const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16);
 #pragma unroll 1
             for (int col = half * 32; col < kTileN; col += 64) {
@@ -835,7 +837,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
         __syncwarp();
         cluster_sync();
-        if (warp >= 4 && !*abort_flag) {
+        if (warp >= 4 && sound) {
             // four columns a thread, the threads of a row side by side
             const int log_pieces = __ffs(width / 4) - 1;
             const bool whole = ((uintptr_t)a.out | (uintptr_t)(a.ld * sizeof(T))) % (4 * sizeof(T)) == 0;
