@@ -530,7 +530,10 @@ class Index:
         if not 1 <= dim <= FP8_MAX_DIM:
             raise CoralError(ERR_ARG, f"dim must be in [1, {FP8_MAX_DIM}]")
         cp, sp = (dim + 15) // 16 * 16, (dim + 511) // 512 * 4
-        Q, n = queries[0].shape[0], base[0].shape[0]
+        try:
+            Q, n = len(queries[0]), len(base[0])
+        except (TypeError, IndexError, KeyError):
+            _refuse("queries and base", "pairs (codes, scales)")
         pq = self._at("the queries' codes", queries[0], torch.float8_e4m3fn, (Q, cp))
         sq = self._at("the queries' scales", queries[1], torch.float8_e8m0fnu, (Q, sp))
         pr = self._at("the base's codes", base[0], torch.float8_e4m3fn, (n, cp))

@@ -1514,6 +1514,16 @@ bool rows_overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int si
     return gap < (uintptr_t)(n * size) || row - gap < (uintptr_t)(n * size);
 }
 
+// Whether `bytes` bytes at p (null: none) meet an element of Q rows of `width` bytes, `pitch` apart, at `rows`.
+bool meets(const void* p, int64_t bytes, const void* rows, int64_t Q, int64_t width, int64_t pitch) {
+    const int64_t at = (int64_t)((uintptr_t)p - (uintptr_t)rows);      // of p, from the first row
+    if (!p || bytes <= 0 || at + bytes <= 0 || at >= (Q - 1) * pitch + width) return false;
+    return at < 0 || at % pitch < width || at % pitch + bytes > pitch;
+}
+bool meets(const void* p, int64_t bytes, const void* other, int64_t other_bytes) {
+    return meets(p, bytes, other, 1, other_bytes, other_bytes);
+}
+
 #define ARG(cond, text)                                             \
     do {                                                            \
         if (!(cond)) return fail(h, CORAL_ERR_ARG, text);           \
@@ -1539,6 +1549,11 @@ int coral_fp8_quantize(coral_index_t* h, const void* d_x, int type, int64_t rows
     if (!scope.ok) return fail(h, CORAL_ERR_CUDA, "cudaSetDevice failed");
     ARG(usable(h, d_x, score_align(type)) && usable(h, d_codes, 16) && usable(h, d_scales, 4),
         "arrays must be aligned device memory of the handle's GPU");
+    const int64_t code_bytes = rows * coral::fp8_code_pitch(dim), scale_bytes = rows * coral::fp8_scale_pitch(dim);
+    const int64_t size = coral::type_bytes(type);
+    ARG(!meets(d_codes, code_bytes, d_x, rows, dim * size, ld * size) && !meets(d_scales, scale_bytes, d_x, rows, dim * size, ld * size) &&
+            !meets(d_codes, code_bytes, d_scales, scale_bytes),
+        "an output overlaps another array");
     CK(coral::launch_fp8_quantize(d_x, type, rows, dim, ld, d_codes, d_scales, h->sm_count,
                                   stream ? (cudaStream_t)stream : h->stream));
     h->launches += 1;
@@ -1562,6 +1577,11 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     ARG(usable(h, d_q_codes, 16) && usable(h, d_q_scales, 4) && usable(h, d_codes, 16) && usable(h, d_scales, 4) &&
             (!d_bias || usable(h, d_bias, 4)) && usable(h, d_out, score_align(type)),
         "arrays must be aligned device memory of the handle's GPU");
+    const int64_t size = coral::type_bytes(type), cp = coral::fp8_code_pitch(dim), sp = coral::fp8_scale_pitch(dim);
+    ARG(!meets(d_q_codes, Q * cp, d_out, Q, n * size, ld * size) && !meets(d_q_scales, Q * sp, d_out, Q, n * size, ld * size) &&
+            !meets(d_codes, n * cp, d_out, Q, n * size, ld * size) && !meets(d_scales, n * sp, d_out, Q, n * size, ld * size) &&
+            !meets(d_bias, n * 4, d_out, Q, n * size, ld * size),
+        "d_out overlaps another array");
     coral::Fp8ScoresArgs a{};
     a.q_codes = d_q_codes;
     a.q_scales = d_q_scales;
@@ -1591,6 +1611,7 @@ int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q,
     ARG(ld >= n && ld < (1ll << 31) && ld_out >= n && ld_out < (1ll << 31), "ld and ld_out must be in [n, 2^31)");
     ARG(n_seen >= 0 && n_bias >= 0, "negative list length");
     if (n_bias > coral::kRulesMaxBias) return fail(h, CORAL_ERR_LIMIT, "n_bias must not exceed 1024");
+    if (n_seen > coral::kRulesMaxSeen) return fail(h, CORAL_ERR_LIMIT, "n_seen must not exceed 2^24");
     if ((n + 4095) / 4096 * Q > 0x7fffffffll) return fail(h, CORAL_ERR_LIMIT, "too many score rows for one call");
     if (Q == 0 || n == 0) return CORAL_OK;
     ARG(d_scores && d_out && (n_seen == 0 || (d_seen && d_penalties)) && (n_bias == 0 || (d_bias_ids && d_bias)),
@@ -1607,6 +1628,12 @@ int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q,
         ARG(ld == ld_out || Q == 1, "in place, ld_out must be ld");
     else
         ARG(!rows_overlap(d_scores, ld, d_out, ld_out, coral::type_bytes(type), Q, n), "d_out overlaps d_scores");
+    const int64_t size = coral::type_bytes(type), words = (n + 31) / 32;
+    const auto apart = [&](const void* p, int64_t bytes) { return !meets(p, bytes, d_out, Q, n * size, ld_out * size); };
+    ARG(apart(d_seen, (int64_t)Q * n_seen * 4) && apart(d_penalties, n_seen ? (int64_t)Q * 12 : 0) &&
+            apart(d_bias_ids, (int64_t)Q * n_bias * 4) && apart(d_bias, (int64_t)Q * n_bias * 4) &&
+            apart(d_excluded, ((Q - 1) * ld_excluded + words) * 4),
+        "d_out overlaps another array");
     coral::RulesArgs a{};
     a.in = d_scores;
     a.out = d_out;
@@ -1652,6 +1679,13 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
     ARG((n == 0 || usable(h, d_scores, score_align(type))) && usable(h, d_ids_out, 4) && usable(h, d_scores_out, 4) &&
             (need == 0 || usable(h, d_workspace, 8)),
         "arrays must be aligned device memory of the handle's GPU");
+    const int64_t size = coral::type_bytes(type), chosen = (int64_t)Q * k * 4;
+    ARG((n == 0 || (!meets(d_ids_out, chosen, d_scores, Q, n * size, ld * size) &&
+                    !meets(d_scores_out, chosen, d_scores, Q, n * size, ld * size) &&
+                    !meets(d_workspace, need, d_scores, Q, n * size, ld * size))) &&
+            !meets(d_ids_out, chosen, d_scores_out, chosen) && !meets(d_workspace, need, d_ids_out, chosen) &&
+            !meets(d_workspace, need, d_scores_out, chosen),
+        "an output or the workspace overlaps another array");
     coral::TopkArgs a{};
     a.in = d_scores;
     a.type = type;

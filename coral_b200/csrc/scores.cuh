@@ -19,6 +19,7 @@ constexpr int kFp8Block = 128;        // columns that share one scale
 constexpr int kFp8MaxDim = 1 << 16;
 constexpr int kTopkMax = 1024;        // k of the selection
 constexpr int kRulesMaxBias = 1024;   // biased ids per row
+constexpr int kRulesMaxSeen = 1 << 24;   // history per row: counts are exact in fp32
 
 // Bytes of one compressed row: codes are padded to 16 (tensor copies), scales to 4 (one word read
 // covers 512 columns).

@@ -405,7 +405,8 @@ int coral_search_static_status(int device);
  * All five take device pointers of the handle's GPU (checked; CORAL_ERR_ARG else), need no vectors in
  * the handle, keep no state between calls, enqueue on `stream` (NULL = the handle's stream) without
  * synchronising and leave the caller's current device as it was.  They allocate nothing, so they can
- * be captured into a graph; a workspace belongs to one call at a time.  Empty sizes are allowed and
+ * be captured into a graph; a workspace belongs to one call at a time.  An output that overlaps another
+ * array of its call is refused (but coral_adjust_scores works in place).  Empty sizes are allowed and
  * launch nothing (coral_topk_scores still writes its padding). */
 
 /* element types */
@@ -437,9 +438,9 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
 
 /* Rules on Q score rows of n columns, in fp32, rounded once.  With c = how often j stands in row q of
  * d_seen ([Q][n_seen], entries outside [0, n) are padding) and (rho, phi, pi) = d_penalties[q]
- * ([Q][3], rho > 0):  c > 0: s = (s > 0 ? s / rho : s * rho) - phi * c - pi.  Then s += every
- * d_bias[q][i] with d_bias_ids[q][i] = j, in list order ([Q][n_bias], n_bias <= 1024, ids outside
- * [0, n) are padding).  Then s = -inf where bit j % 32 of word j / 32 of row q of d_excluded is set
+ * ([Q][3], rho > 0; n_seen <= 2^24):  c > 0: s = (s > 0 ? s / rho : s * rho) - phi * c - pi.  Then
+ * s += the sum, in list order, of the d_bias[q][i] with d_bias_ids[q][i] = j ([Q][n_bias], n_bias <=
+ * 1024, ids outside [0, n) are padding).  Then s = -inf where bit j % 32 of word j / 32 of row q of d_excluded is set
  * (the bitset of coral_index_set_deleted; rows ld_excluded words apart, 0 = one row for all).  Each
  * list may be absent (NULL and n_seen / n_bias 0; d_penalties goes with d_seen).  d_out may be
  * d_scores with the same ld; any other overlap is refused. */

@@ -593,6 +593,56 @@ def test_c_refusals(ix):
     assert lib.coral_scores_check(h) == OK
 
 
+def test_overlaps_are_refused(ix):
+    """An output that shares memory with another array of its call, at both ends; side by side is allowed."""
+    lib, h = ix._lib, ix._h
+    buf = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    d = buf.data_ptr()
+    A, L, OK = capi.ERR_ARG, capi.ERR_LIMIT, capi.OK
+    x, far = d + 65536, d + 131072
+
+    def quantize(codes, scales):      # 4 rows of 64 floats, 128 apart: bytes [0, 256) of every 512
+        return lib.coral_fp8_quantize(h, x, 0, 4, 64, 128, codes, scales, 1)
+    assert quantize(far, far + 256) == OK
+    assert quantize(x + 3 * 512 + 256, far) == OK and quantize(x - 256, far) == OK
+    assert quantize(far, x + 256) == OK      # 16 bytes of scales between two rows
+    for codes, scales in ((x, far), (x - 240, far), (x + 3 * 512 + 240, far), (far, x + 252), (far, x + 512 - 12), (far, far + 252), (far, far)):
+        assert quantize(codes, scales) == A
+
+    def scores(qc, qs, c, s, bias, out):      # 4 x 8 scores of 64 columns, 16 floats apart: bytes [0, 32) of every 64
+        return lib.coral_fp8_scores(h, qc, qs, 4, c, s, 8, 64, 1.0, bias, out, 0, 16, 1)
+    ok = [d, d + 256, d + 512, d + 1024, d + 1056]
+    assert scores(*ok, x) == OK and scores(*ok[:4], x + 32, x) == OK
+    for i, size in enumerate((256, 16, 512, 32, 32)):
+        for at in (x, x - size + 16, x + 3 * 64 + 16, x + 64 - size + 16 if size <= 64 else x + 64):
+            bad = list(ok)
+            bad[i] = at
+            assert scores(*bad, x) == A, (i, at - x)
+
+    def adjust(seen, pen, ids, bias, ex):     # 4 x 64 floats, 5 of history, 3 biases
+        return lib.coral_adjust_scores(h, x, 0, 4, 64, 64, seen, 5, pen, ids, bias, 3, ex, 2, far, 64, 1)
+    ok = [d, d + 256, d + 512, d + 768, d + 1024]
+    assert adjust(*ok) == OK
+    for i, size in enumerate((80, 48, 48, 48, 32)):
+        for at, code in ((far - size, OK), (far - size + 4, A), (far + 1020, A), (far + 1024, OK)):
+            bad = list(ok)
+            bad[i] = at
+            assert adjust(*bad) == code, (i, at - far)
+    assert lib.coral_adjust_scores(h, x, 0, 1, 64, 64, d, (1 << 24) + 1, d, None, None, 0, None, 0, far, 64, 1) == L
+
+    need = capi.C.c_int64(0)
+    assert lib.coral_topk_workspace(h, 1, 100_000, 10, capi.C.byref(need)) == OK and need.value > 0
+
+    def topk(ids, best, ws):
+        return lib.coral_topk_scores(h, d, 0, 1, 100_000, 100_000, 10, 0, ids, best, ws, need.value, 1)
+    f = d + 400_000
+    assert topk(f, f + 40, f + 80) == OK
+    for args in ((f - 4, f + 40, f + 80), (f, f - 4, f + 80), (f, f + 36, f + 80), (f, f + 40, f + 72), (f + 8, f + 48, f - 8),
+                 (f + 8, f + 48, f + 16), (d, f, f + 80)):
+        assert topk(*args) == A
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------------------------ far and empty
 def test_offsets_past_32_bits(ix):
     """Rows 1.2e9 elements apart: the third row starts past 2^31 elements (and 2^32 bytes)."""
