@@ -480,7 +480,7 @@ __device__ __forceinline__ float4 load_peer(uint32_t addr) {
 constexpr int kPlain = 0;      // coalesced plain stores
 constexpr int kTma = 1;        // tensor stores
 constexpr int kTmaOdd = 2;     // the same, and the columns after a row's last whole 16 bytes plainly (apart
-                               // from kTma: the few instructions cost 17 x 2M x 100 fp32 87 -> 100 us)
+                               // from kTma: the few instructions cost 33 x 2M x 100 fp32 93 -> 102 us)
 constexpr int kSplit = 3;      // the tile's k-blocks are split over the CTAs of a cluster, see below
 
 // With fewer tiles than SMs and many k-blocks, a cluster of 2, 4 or 8 CTAs shares a tile: rank r takes a
@@ -900,45 +900,56 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 // ------------------------------------------------------------------------- product, few queries
 //
-// Up to 16 queries: the base rows take the products' M and the queries their N, so a tile is 256 base
-// rows (two products of M = 128, N = 16).  The products then cost a sixteenth of what a query tile of
+// Up to 32 queries: the base rows take the products' M and the queries their N, so a tile is 256 base
+// rows (two products of M = 128, N = NQ).  The products then cost a fraction of what a query tile of
 // mostly nothing would, and of its power (1 x 1M x 512 ran 97 us at the 1.5 GHz that it left), and a lane
-// holds one base row's scores, so a warp stores a query's 32 scores side by side straight from its
-// registers, at any alignment.  Bound by memory: 1 x 1M x 512 79 us, 6.6 TB/s; 1 x 4M x 128 83 us (a query
-// tile: 165); by the steps of a tile where its rows are short: 8 x 190k x 31 bf16 9.3 us (13.8).  With
-// more queries these stores lose to tensor stores (20 x 500k x 300 fp32: 46 us against 41).
+// holds one base row's scores, so all eight epilogue warps have work and a warp stores a query's 32 scores
+// side by side straight from its registers, at any alignment.  Bound by memory: 1 x 1M x 512 79 us,
+// 6.6 TB/s; 32 x 1M x 512 fp32 98 us (a query tile: 100); 1 x 4M x 128 83 us (165); where rows are short,
+// by the tensor copies, which take their time per row: 16 x 1000003 x 100 bf16 32 us, 32 x 300k x 128 17 us
+// (21.5), 17 x 2M x 100 70 us (87); against the rule, 32 x 1M x 130 bf16 51.8 us (51).  The query tile is
+// kept, if its k-blocks fit the stages: its rows copied with every row tile cost 16 x 1000003 x 100 47 us.
+// 64 queries lose: 64 x 1M x 128 bf16 takes 50 us against 47 in query tiles.  (Scores through shared memory and tensor stores: 16.5 us for 32 x
+// 300k x 128, but 76 for 17 x 2M x 100 and 84 for 1 x 1M x 512.)
 //
-// Four stages of 34 KB: with five 1 x 1M x 512 takes 83 us, with six 87; memory slows when more is asked
-// for at once.  Tensor memory: two buffers of 32 columns and, from 128, eight slots of 16 columns of
-// scales (as many slots as stages or more: see above).  Roles as above, epilogue warp 4 + 4 h + g for
+// Four stages of 34 or 36 KB: with five 1 x 1M x 512 takes 83 us, with six 87; memory slows when more is
+// asked for at once.  Tensor memory: two buffers of 2 NQ columns and, from 128, eight slots of 16 columns
+// of scales (as many slots as stages or more: see above).  Roles as above, epilogue warp 4 + 4 h + g for
 // rows 32 g .. 32 g + 31 of half h.
-constexpr int kFewQueries = 16, kFewStages = 4, kFewSlots = 8;
-constexpr int kFewBase = 256 * kTileK, kFewQ = kFewQueries * kTileK;
-constexpr int kFewOffQ = kFewStages * kFewBase;
-constexpr int kFewOffScales = kFewOffQ + kFewStages * kFewQ;
-constexpr int kFewOffBars = kFewOffScales + kScaleSlots * kScaleBytes;
-constexpr int kFewBytes = kFewOffBars + 256 + 1024;
-static_assert(kFewSlots >= kFewStages && kFewBytes <= 232448, "few queries");
-constexpr uint32_t kFewInstrDesc = (1u << 23) | ((uint32_t)(kFewQueries >> 3) << 17) | ((uint32_t)(kTileM >> 7) << 27);
+constexpr int kFewQueries = 32, kFewStages = 4, kFewSlots = 8;
+constexpr int kFewBase = 256 * kTileK;
+template <int NQ>
+struct Few {
+    static constexpr int kQ = NQ * kTileK;                          // bytes of a stage's queries
+    static constexpr int kOffQ = kFewStages * kFewBase;
+    static constexpr int kOffScales = kOffQ + kFewStages * kQ;
+    static constexpr int kOffBars = kOffScales + kScaleSlots * kScaleBytes;
+    static constexpr int kBytes = kOffBars + 256 + 1024;
+    static constexpr uint32_t kInstr = (1u << 23) | ((uint32_t)(NQ >> 3) << 17) | ((uint32_t)(kTileM >> 7) << 27);
+    static_assert(NQ <= 32 && kFewSlots >= kFewStages && kBytes <= 232448, "few queries");
+};
 
-template <typename T>
+template <typename T, int NQ>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_b,
                       const Fp8ScoresArgs a, const uint32_t tiles, const int q_rows) {
+    using F = Few<NQ>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFewOffBars);      // [kFewStages] codes landed
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::kOffBars);      // [kFewStages] codes landed
     uint64_t* empty = full + kFewStages;                                   // [kFewStages] the products that read them are done
     uint64_t* sfull = empty + kFewStages;                                  // [kScaleSlots] a group's scales landed
     uint64_t* sempty = sfull + kScaleSlots;                                // [kScaleSlots] and are no longer needed
     uint64_t* tfull = sempty + kScaleSlots;                                // [2] accumulator buffer complete
     uint64_t* tfree = tfull + 2;                                           // [2] and drained
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree + 2);
+    uint64_t* qfull = tfree + 2;                                           // the query tile landed, if it is kept
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // known to be uniform
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
     const int scale_pitch = (a.dim + 511) / 512 * 4;
+    const bool keeps_q = k_blocks <= kFewStages;      // as above
 
     if (tid == 0) {
         for (int s = 0; s < kFewStages; ++s) {
@@ -953,14 +964,15 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             mbar_init(&tfull[b], 1);
             mbar_init(&tfree[b], kEpiWarps);
         }
+        mbar_init(qfull, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // query rows that are not loaded stay zero: their products are not stored, but cost power
-    for (int i = q_rows * kTileK + tid * 16; i < kFewQ; i += kThreads * 16)
+    for (int i = q_rows * kTileK + tid * 16; i < F::kQ; i += kThreads * 16)
 #pragma unroll
         for (int s = 0; s < kFewStages; ++s)
-            *reinterpret_cast<uint4*>(smem + kFewOffQ + s * kFewQ + i) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(smem + F::kOffQ + s * F::kQ + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(tmem_slot)) : "memory");
@@ -976,12 +988,17 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             int s = 0;
             uint32_t par = 0;
             bool ok = true;
+            if (keeps_q) {
+                mbar_expect_tx(qfull, k_blocks * q_rows * kTileK);
+                for (int kb = 0; kb < k_blocks; ++kb)
+                    tma_load_2d(smem + F::kOffQ + kb * F::kQ, &map_q, kb * kTileK, 0, qfull);
+            }
             for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
-                    mbar_expect_tx(&full[s], kFewBase + q_rows * kTileK);
+                    mbar_expect_tx(&full[s], kFewBase + (keeps_q ? 0 : q_rows) * kTileK);
                     tma_load_2d(smem + s * kFewBase, &map_b, kb * kTileK, (int)((int64_t)t * 256), &full[s]);
-                    tma_load_2d(smem + kFewOffQ + s * kFewQ, &map_q, kb * kTileK, 0, &full[s]);
+                    if (!keeps_q) tma_load_2d(smem + F::kOffQ + s * F::kQ, &map_q, kb * kTileK, 0, &full[s]);
                     if (++s == kFewStages) {
                         s = 0;
                         par ^= 1u;
@@ -990,13 +1007,13 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
     } else if (warp == 1) {
         const uint32_t leads = elect_leader();
-        const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + kFewOffScales);
+        const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + F::kOffScales);
         uint32_t s = 0, par = 0, i = 0, group = 0;
-        bool ok = true;
+        bool ok = !keeps_q || __all_sync(0xffffffffu, mbar_wait(qfull, 0, abort_flag, a.err));
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
             const uint32_t b = i & 1u;
             if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&tfree[b], ((i >> 1) - 1) & 1u, abort_flag, a.err))) break;
-            const uint32_t acc = tmem + b * 32;
+            const uint32_t acc = tmem + b * 2 * NQ;
             for (int kb = 0; kb < k_blocks; ++kb) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a.err));
                 if (!ok) break;
@@ -1013,12 +1030,12 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     scales_to_tmem(leads, tb, sc + (1024 >> 4));
                 }
                 const uint64_t d0 = desc_sw128(codes + s * kFewBase), d1 = d0 + (128 * kTileK >> 4);
-                const uint64_t dq = desc_sw128(codes + kFewOffQ + s * kFewQ);
-                const uint32_t idesc = kFewInstrDesc | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
+                const uint64_t dq = desc_sw128(codes + F::kOffQ + (keeps_q ? kb : s) * F::kQ);
+                const uint32_t idesc = F::kInstr | (uint32_t)(kb & 3) << 29 | (uint32_t)(kb & 3) << 4;
                 const int slices = (min(a.dim - kb * kTileK, kTileK) + 31) / 32;
                 for (int j = 0; j < slices; ++j) {
                     umma_mxf8(leads, acc, d0 + j * 2, dq + j * 2, idesc, ta, tb, (kb | j) != 0 ? 1u : 0u);
-                    umma_mxf8(leads, acc + 16, d1 + j * 2, dq + j * 2, idesc, ta + 4, tb, (kb | j) != 0 ? 1u : 0u);
+                    umma_mxf8(leads, acc + NQ, d1 + j * 2, dq + j * 2, idesc, ta + 4, tb, (kb | j) != 0 ? 1u : 0u);
                 }
                 umma_commit(leads, &empty[s]);
                 if ((kb & 3) == 3 || kb == k_blocks - 1) {
@@ -1053,11 +1070,11 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const uint32_t slot = sent % kScaleSlots;
                 ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a.err));
                 if (!ok) break;
-                const uint32_t dst = smem_u32(smem + kFewOffScales + slot * kScaleBytes) + lane * 16;
+                const uint32_t dst = smem_u32(smem + F::kOffScales + slot * kScaleBytes) + lane * 16;
 #pragma unroll
                 for (int g = 0; g < 8; ++g)
                     copy(dst + (g >> 2) * 512 + (g & 3) * 4, a.scales, (int64_t)t * 256 + g * 32 + lane, a.n, kb);
-                copy(dst + 1024, a.q_scales, lane, a.Q, kb);      // rows from 16 on: zero, and not used
+                copy(dst + 1024, a.q_scales, lane, a.Q, kb);      // rows from Q on: zero, and not used
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (++sent - done > kScalesAhead) {
                     asm volatile("cp.async.wait_group %0;" ::"n"(kScalesAhead) : "memory");
@@ -1068,7 +1085,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         while (ok && done < sent) publish();
     } else if (warp >= 4) {
         const int row = (warp - 4) * 32 + lane;      // of the tile: half (warp - 4) / 4, 32 lanes of tensor memory (warp & 3)
-        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)((warp - 4) >> 2) * 16;
+        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)((warp - 4) >> 2) * NQ;
         uint32_t i = 0;
         int64_t n = (int64_t)blockIdx.x * 256 + row;
         float next_bias = a.bias && n < a.n ? a.bias[n] : 0.f;
@@ -1081,14 +1098,17 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const uint32_t b = i & 1u;
             if (!__all_sync(0xffffffffu, mbar_wait(&tfull[b], i >> 1 & 1u, abort_flag, a.err))) break;
             tc_fence_after();
-            uint32_t r[kFewQueries];
-            tmem_ld16(from + b * 32, r);
+            uint32_t r[NQ];
+            if constexpr (NQ == 16)
+                tmem_ld16(from + b * 2 * NQ, r);
+            else
+                tmem_ld32(from + b * 2 * NQ, r);
             tmem_ld_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tfree[b]);
 #pragma unroll
-            for (int q = 0; q < kFewQueries; ++q) {
+            for (int q = 0; q < NQ; ++q) {
                 if (q >= a.Q) break;
                 if (there) *out = narrow<T>(fmaf(a.alpha, __uint_as_float(r[q]), bias));
                 out += a.ld;
@@ -1222,7 +1242,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
     order.chunk_n = (uint32_t)(in_l2 < sm_count ? sm_count : in_l2);
     if (order.chunk_n > order.tiles_n) order.chunk_n = order.tiles_n;
     const int k_blocks = (a.dim + kTileK - 1) / kTileK;
-    static std::atomic<uint64_t> granted[5];
+    static std::atomic<uint64_t> granted[6];
     int parts = 1;
     if (order.tiles <= (uint32_t)sm_count && k_blocks > 4) {
         auto split = fp8_scores_kernel<T, kSplit, 4>;
@@ -1231,10 +1251,12 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
         parts = split_of(split, order.tiles, k_blocks, sm_count);
     }
     if (parts == 1 && a.Q <= kFewQueries) {
-        auto few = fp8_few_scores_kernel<T>;
-        cudaError_t e = grant_smem(few, kFewBytes, granted[4]);
+        const bool most = a.Q > 16;
+        auto few = most ? fp8_few_scores_kernel<T, 32> : fp8_few_scores_kernel<T, 16>;
+        const int bytes = most ? Few<32>::kBytes : Few<16>::kBytes;
+        cudaError_t e = grant_smem(few, bytes, granted[most ? 5 : 4]);
         if (e != cudaSuccess) return e;
-        few<<<order.tiles < (uint32_t)sm_count ? order.tiles : (uint32_t)sm_count, kThreads, kFewBytes, stream>>>(
+        few<<<order.tiles < (uint32_t)sm_count ? order.tiles : (uint32_t)sm_count, kThreads, bytes, stream>>>(
             map_a, map_b, a, order.tiles, a_rows);
         return cudaGetLastError();
     }

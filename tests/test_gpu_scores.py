@@ -240,7 +240,8 @@ def test_scores_into_slices(ix, dtype, n, lead, ld):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("Q,n,dim,lead,pad", [(1, 1, 1, 0, 0), (1, 255, 40, 1, 0), (15, 257, 128, 3, 5), (16, 60_001, 200, 0, 7),
                                               (16, 60_000, 70, 8, 8), (17, 60_001, 200, 0, 7), (2, 40_000, 700, 5, 1),
-                                              (9, 38_000, 513, 2, 0)])
+                                              (9, 38_000, 513, 2, 0), (32, 40_003, 200, 1, 0), (31, 39_000, 513, 0, 8),
+                                              (24, 300, 16, 3, 2), (33, 40_000, 130, 0, 0), (32, 90_000, 1300, 0, 3)])
 def test_scores_of_few_queries(ix, dtype, Q, n, dim, lead, pad):
     """Around the number of queries at which base rows and queries change sides."""
     q, base = rows8(ix, Q, dim, 16, 3), rows8(ix, n, dim, 17, 3)
