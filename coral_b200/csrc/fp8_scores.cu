@@ -100,7 +100,7 @@ __device__ __forceinline__ float drop_infinities(uint4 (&v)[J]) {
 // at most 64, 32 or 16 columns, which would leave the other lanes idle (800k x 14 bf16: 52 us with
 // eight, 11 with one).  A warp takes kQuantLoads / J steps of 32 / G consecutive blocks, all loads before the first
 // use, and writes the scales together.  Bound by memory: 1M x 512 fp32 takes 369 us, 2.56 GB at
-// 6.95 TB/s; 100003 x 200 bf16, cut from rows of 256, 16 us, 61 MB at 3.8 TB/s.  (A block
+// 6.95 TB/s; 100003 x 200 bf16, cut from rows of 256, 15 us, 61 MB at 4.0 TB/s.  (A block
 // to a whole warp or half of one is bound by instructions instead, 435 and 22 us: the few values a
 // lane then has carry the same addresses, bounds and exponents.)
 template <typename T, bool VEC, int G>
@@ -243,10 +243,10 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // descriptor), byte (k-block mod 4).
 //
 // What bounds it: the base's bytes with not too many queries (64 x 1M x 512 with
-// its 256 MB of scores: 126 us, 6.1 TB/s), the scores' bytes with many and short rows (4001 x 100003 x
+// its 256 MB of scores: 129 us, 6.0 TB/s), the scores' bytes with many and short rows (4001 x 100003 x
 // 256 bf16: 193 us, 4.3 TB/s, where filling as much memory takes 203 us), and with many and long rows
 // shared memory: a stage's 48 KB arrive in 384 cycles and are read in another 384, against 512 cycles
-// of products (4096 x 8192 x 4096: 108 us alone, 2.5 PFLOP/s; 137 us under a power cap).  Pairs of SMs
+// of products (4096 x 8192 x 4096: 108 to 118 us alone, 2.3 to 2.5 PFLOP/s; 137 us under a power cap).  Pairs of SMs
 // on one tile would halve the row tile's share of that; not built.
 //
 // Tensor memory: two accumulators of 256 columns that share 64 (0-255 and 192-447) and, from 448,

@@ -9,12 +9,12 @@
 // flight while it turns the row's two id lists into tables over its columns in shared memory: counts
 // by integer atomics (their order does not show), biases by one warp in list order, and one bit for
 // every column that either list touches: a thread whose columns are untouched reads one word of bits
-// and no table.  Then it applies the rules and stores.  No table in global memory, nothing to clear between calls, one launch.  The
-// history is read once per CTA, from L2: wider columns would read it less often but leave fewer CTAs
-// an SM, and latency, not that traffic, is what a CTA waits for.
+// and no table.  Then it applies the rules and stores.  No table in global memory, nothing to clear
+// between calls, one launch.  The history is read once per CTA, from L2: wider columns would read it
+// less often but leave fewer CTAs an SM, and latency, not that traffic, is what a CTA waits for.
 //
-// Measured: 32 x 1M fp32 with a shared mask 41 us, 250 MB at 6.1 TB/s; 64 x 128000 bf16, histories of
-// 2000, nine tenths excluded, 12.6 us (20 MB would take 3: three waves of CTAs, each a chain of mask,
+// Measured: 32 x 1M fp32 with a shared mask 42 us, 250 MB at 5.9 TB/s; 64 x 128000 bf16, histories of
+// 2000, nine tenths excluded, 11.7 us (20 MB would take 3: three waves of CTAs, each a chain of mask,
 // scores, tables and stores).  With tables read for every column, eight to a thread, the latter took
 // 27 us, on bank conflicts.
 #include <math_constants.h>

@@ -400,7 +400,7 @@ int coral_search_static_status(int device);
  * A dense pass over a compressed base under per-query rules: rows are compressed once
  * (coral_fp8_quantize), a batch of queries at its arrival, coral_fp8_scores forms every score on the
  * tensor cores, coral_adjust_scores applies the rules and coral_topk_scores chooses.  Chunks or
- * shards of the base meet in coral_merge_shards (id_base makes ids global).
+ * shards of the base meet in coral_merge_shards of a CORAL_IP handle (id_base makes ids global).
  *
  * All five take device pointers of the handle's GPU (checked; CORAL_ERR_ARG else), need no vectors in
  * the handle, keep no state between calls, enqueue on `stream` (NULL = the handle's stream) without
