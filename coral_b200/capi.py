@@ -574,7 +574,7 @@ class Index:
             # rows as far apart as the input's are when that is tight, else at multiples of 16 bytes
             per = 16 // scores.dtype.itemsize
             ld_out = n if ld == n else (n + per - 1) // per * per
-            out = scores.new_empty((Q, ld_out))
+            out = torch.empty_like(scores) if ld == n else scores.new_empty((Q, ld_out))
             po = out.data_ptr()
             if ld_out != n:
                 out = out[:, :n]
