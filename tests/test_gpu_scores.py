@@ -411,6 +411,27 @@ def chain_inputs(ix, Q, n, dim, seed):
     return x, base, bias, seen, pen, ex
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k", [(1500, 1000), (5000, 800), (70_000, 1024), (70_000, 400), (300, 300), (9000, 40)])
+def test_topk_crowded_ranges(ix, dtype, n, k):
+    """Rows whose best scores crowd parts of their range: all equal, few values, one far away, infinities,
+    both signs, exponents apart, the largest and the smallest numbers."""
+    g = gen(91)
+    fi = torch.finfo(dtype)
+    r = torch.randn(n, generator=g, device="cuda").to(dtype)
+    far = r.clone()
+    far[n // 2] = fi.max
+    inf = r.clone()
+    inf[::3] = float("inf")
+    ends = torch.where(r > 0, torch.full_like(r, fi.max), torch.full_like(r, -fi.max))
+    tiny = r * fi.smallest_normal
+    spread = torch.exp2(torch.randint(-14, 15, (n,), generator=g, device="cuda").double()).to(dtype) * torch.sign(r)
+    few = torch.randint(0, 4, (n,), generator=g, device="cuda").to(dtype)
+    one = torch.zeros_like(r)
+    one[n - 1] = 1
+    check_topk(ix, torch.stack([torch.full_like(r, 2.5), few, far, inf, ends, tiny, spread, one, torch.zeros_like(r)]), k)
+
+
 def test_the_operators_together(ix):
     """Compressed rows, rules and choice as one search, and the same over two chunks of the base."""
     Q, n, dim, k = 37, 5000, 200, 50
