@@ -512,6 +512,33 @@ def test_other_streams(ix):
         assert torch.equal(ids, want[0]) and torch.equal(best, want[1])
 
 
+def test_two_threads_at_once(ix):
+    """The chain from two threads, each with its stream and inputs, on one handle."""
+    import threading
+    sets = [chain_inputs(ix, 6, 30_000 + 1000 * i, 256, 95 + i) for i in range(2)]
+    want = [run_all(ix, x, base, 256, bias, seen, pen, ex, 20) for x, base, bias, seen, pen, ex in sets]
+    torch.cuda.synchronize()
+    got, wrong = [None, None], []
+
+    def work(i):
+        x, base, bias, seen, pen, ex = sets[i]
+        stream = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = run_all(ix, x, base, 256, bias, seen, pen, ex, 20)
+                    stream.synchronize()
+                    assert torch.equal(got[i][0], want[i][0]) and torch.equal(got[i][1], want[i][1])
+        except BaseException as e:
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+
+
 def test_launches_are_counted(ix):
     before = ix.launch_count
     run_all(ix, *chain_inputs(ix, 2, 100, 64, 61)[:2], 64, None, None, None, None, 5)
