@@ -23,7 +23,8 @@
 // Measured: 256 x 128000 bf16, k = 100: 20 us, of which the first pass takes 8 to 11 (65.5 MB at up to
 // 6 TB/s), the bound 2, the second pass 4.5, the order 1.5; one pass against a running threshold, with
 // the buffer cut now and then, took 45 us, because nearly every warp then held something to append.
-// 1 x 1M fp32, k = 10: 7.5 us in two launches.
+// 1 x 1M fp32, k = 10: 7.2 us in two launches; k = 1000: 39 us (48 with one key a thread in flight in the
+// second), of which the order of the joined keys takes 8.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -443,12 +444,18 @@ __global__ void __launch_bounds__(kThreads) topk_join_kernel(const TopkArgs a, c
     const uint32_t least = ord_of(sh.least);
     for (int careful = 0; careful < 2; ++careful) {
         for (int i0 = 0; i0 < total; i0 += kRoom) {
-            for (int i = i0 + tid; i < min(total, i0 + kRoom); i += kThreads) {
-                const uint64_t key = keys[i];
-                if ((uint32_t)(key >> 32) >= least) {
-                    const int at = atomicAdd(&sh.cnt, 1);
-                    if (at < kCap) sh.keys[at] = key;
-                }
+            constexpr int kTogether = 4;      // loads in flight
+            static_assert(kRoom % (kTogether * kThreads) == 0, "rounds");
+            for (int i1 = i0 + tid; i1 < min(total, i0 + kRoom); i1 += kTogether * kThreads) {
+                uint64_t key[kTogether];
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u) key[u] = i1 + u * kThreads < total ? keys[i1 + u * kThreads] : 0;
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u)
+                    if ((uint32_t)(key[u] >> 32) >= least) {
+                        const int at = atomicAdd(&sh.cnt, 1);
+                        if (at < kCap) sh.keys[at] = key[u];
+                    }
             }
             if (careful) {
                 __syncthreads();
