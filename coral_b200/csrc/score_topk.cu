@@ -23,8 +23,8 @@
 // Measured: 256 x 128000 bf16, k = 100: 20 us, of which the first pass takes 8 to 11 (65.5 MB at up to
 // 6 TB/s), the bound 2, the second pass 4.5, the order 1.5; one pass against a running threshold, with
 // the buffer cut now and then, took 45 us, because nearly every warp then held something to append.
-// 1 x 1M fp32, k = 10: 7.2 us in two launches; k = 1000: 39 us (48 with one key a thread in flight in the
-// second), of which the order of the joined keys takes 8.
+// 1 x 1M fp32, k = 10: 7.2 us in two launches; k = 1000: 35 us (9 more with one key a thread in flight in
+// the second).
 #include <math_constants.h>
 
 #include <type_traits>
@@ -474,12 +474,15 @@ __global__ void __launch_bounds__(kThreads) topk_join_kernel(const TopkArgs a, c
     finish_row(sh, q, a);
 }
 
-// Keys a slice may leave: with a little room above k, few slices need a selection of their own.
-int slots_of(int k) { return k + k / 4 + 16; }
+// Keys a slice may leave: with some room above k, few slices need a selection of their own.  The bound is
+// the looser the larger k (30 x 1M fp32, k = 1000: 68 us with a half, 73 with a quarter; 1 x 1M, k = 10:
+// 7.3 with a quarter, 7.5 with a half).
+int slots_of(int k) { return k + (k > 256 ? k / 2 : k / 4) + 16; }
 
 int topk_splits(int Q, int64_t n, int k, int bytes, int sm_count) {
     const int64_t want = Q > 0 ? (int64_t)sm_count * 2 / Q : 1;
-    const int64_t least = k > 256 ? 32 * (int64_t)k : kRoom;     // a slice is worth its own selection
+    const int64_t least = k > 256 ? 48 * (int64_t)k : kRoom;     // a slice is worth its own selection (48 k
+    // columns; 32 k: 1 x 1M fp32, k = 1000 38 us for 35; 64 k: 10 x 100k, k = 1000 25.7 for 24.1)
     int64_t s = (n + least - 1) / least;
     if (s > want) s = want;
     const int64_t fit = (n * bytes + kSliceBytes - 1) / kSliceBytes;
