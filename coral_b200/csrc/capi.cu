@@ -55,6 +55,7 @@ struct Options {
     int schedule = 0;      // order large batches for L2 locality: 0 = automatic (batches >= 8192), 1 = always, -1 = never
     int schedule_tc = 1;   // scheduling keys on the tensor cores (1) or by the fp32 SIMT tile kernel (0)
     int dense_passes = 3;  // tf32 passes of the dense scans behind coral_exact_knn: 3 = fp32-grade, 1 = plain tf32
+    int score_wait_us = 2000000;  // what a bounded wait of coral_fp8_scores may take
 };
 
 }  // namespace
@@ -577,6 +578,11 @@ int coral_set_option(coral_index_t* h, const char* name, int value) {
     if (!h || !name) return CORAL_ERR_ARG;
     Options& o = h->opt;
     std::string s(name);
+    if (s == "score_wait_us") {
+        if (value < 0 || value > 2000000) return fail(h, CORAL_ERR_ARG, "score_wait_us must be in [0, 2000000]");
+        o.score_wait_us = value;
+        return CORAL_OK;
+    }
     if (s == "ctas_per_sm") o.ctas_per_sm = value;
     else if (s == "warps") o.warps = value;
     else if (s == "chunk_bytes") o.chunk_bytes = value;
@@ -618,6 +624,7 @@ int coral_get_option(coral_index_t* h, const char* name, int* value) {
     else if (s == "probe_carry") *value = o.probe_carry;
     else if (s == "dense_passes") *value = o.dense_passes;
     else if (s == "schedule_tc") *value = o.schedule_tc;
+    else if (s == "score_wait_us") *value = o.score_wait_us;
     else if (s == "sort_tile") *value = o.sort_tile;
     else if (s == "scout_ids") *value = o.scout_ids;
     else if (s == "visit_cache_bits") *value = o.visit_cache_bits;
@@ -1524,6 +1531,8 @@ bool meets(const void* p, int64_t bytes, const void* other, int64_t other_bytes)
     return meets(p, bytes, other, 1, other_bytes, other_bytes);
 }
 
+constexpr long long kClocksPerUs = 2000;      // of an SM, for limits: B200 runs at up to 1965 MHz
+
 #define ARG(cond, text)                                             \
     do {                                                            \
         if (!(cond)) return fail(h, CORAL_ERR_ARG, text);           \
@@ -1596,6 +1605,7 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     a.type = type;
     a.ld = ld;
     a.err = h->h_scores_err;
+    a.wait_clocks = h->opt.score_wait_us * kClocksPerUs;
     CK(coral::launch_fp8_scores(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
     h->launches += 1;
     return CORAL_OK;

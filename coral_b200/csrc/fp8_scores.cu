@@ -278,7 +278,6 @@ struct Layout {
 };
 constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr int64_t kChunkBytes = 32ll << 20;      // base bytes per chunk of tiles: a quarter of L2
-constexpr long long kWaitClocks = 4000000000ll;                     // ~2 s
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -291,6 +290,17 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ uint32_t mbar_test_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok;
+}
 __device__ __forceinline__ uint32_t mbar_try_wait(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -302,21 +312,22 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint64_t* bar, uint32_t parity
         : "memory");
     return ok;
 }
-// Bounded wait: gives up when the clock limit runs out or another role of the CTA gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
-    if (mbar_try_wait(bar, parity)) return true;
+// Bounded wait: gives up when a.wait_clocks have gone by (0: if the phase is not over already) or another
+// role of the CTA gave up.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const Fp8ScoresArgs& a) {
+    if (mbar_test_wait(bar, parity)) return true;
     const long long t0 = clock64();
-    for (uint32_t spins = 1;; ++spins) {
-        if (mbar_try_wait(bar, parity)) return true;
+    for (uint32_t spins = 0;; ++spins) {
         if ((spins & 15u) == 0u) {
             if (*abort_flag) return false;
-            if (clock64() - t0 > kWaitClocks) {
+            if (clock64() - t0 >= a.wait_clocks) {
                 *abort_flag = 1;
-                *static_cast<volatile int*>(err) = 1;
+                *static_cast<volatile int*>(a.err) = 1;
                 __threadfence_system();
                 return false;
             }
         }
+        if (mbar_try_wait(bar, parity)) return true;
     }
 }
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
@@ -561,7 +572,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 int64_t m0, n0;
                 order.at(t, m0, n0);
                 for (int kb = k_first; kb < k_end; ++kb) {
-                    if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
+                    if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a))) break;
                     mbar_expect_tx(&full[s], ((keeps_a ? 0 : a_rows) + kTileN) * kTileK);
                     if (!keeps_a) tma_load_2d(smem + s * kABytes, &map_a, kb * kTileK, (int)m0, &full[s]);
                     tma_load_2d(smem + L::kOffB + s * kBBytes, &map_b, kb * kTileK, (int)n0, &full[s]);
@@ -572,7 +583,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 }
                 if (keeps_a && ok && m0 != kept) {
                     // after the row tile's loads: it fits the ring, and need not wait for the kept tile's end
-                    if (kept >= 0 && !(ok = mbar_wait(aempty, (kept_tiles - 1) & 1u, abort_flag, a.err))) break;
+                    if (kept >= 0 && !(ok = mbar_wait(aempty, (kept_tiles - 1) & 1u, abort_flag, a))) break;
                     kept = m0;
                     ++kept_tiles;
                     mbar_expect_tx(afull, k_blocks * a_rows * kTileK);
@@ -597,18 +608,18 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 last_of_kept = m1 != m0;
                 if (m0 != kept) {
                     kept = m0;
-                    if (!__all_sync(0xffffffffu, mbar_wait(afull, kept_tiles & 1u, abort_flag, a.err))) break;
+                    if (!__all_sync(0xffffffffu, mbar_wait(afull, kept_tiles & 1u, abort_flag, a))) break;
                     ++kept_tiles;
                 }
             }
-            if (i > 0 && !__all_sync(0xffffffffu, mbar_wait(tfree, (i - 1) & 1u, abort_flag, a.err))) break;
+            if (i > 0 && !__all_sync(0xffffffffu, mbar_wait(tfree, (i - 1) & 1u, abort_flag, a))) break;
             const uint32_t acc = tmem + (i & 1u) * kAccStep;
             for (int kb = k_first; kb < k_end; ++kb) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a.err));
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a));
                 if (!ok) break;
                 const uint32_t slot = group % kScaleSlots, ta = tmem + kTmemScales + group % 4 * 16, tb = ta + 8;
                 if ((kb & 3) == 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a.err));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a));
                     if (!ok) break;
                 }
                 tc_fence_after();
@@ -665,7 +676,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             order.at(t, m0, n0);
             for (int kb = k_first; kb < k_end; kb += 4) {
                 const uint32_t slot = sent % kScaleSlots;
-                ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a.err));
+                ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a));
                 if (!ok) break;
                 const uint32_t dst = smem_u32(smem + L::kOffScales + slot * kScaleBytes) + lane * 16;
 #pragma unroll
@@ -684,7 +695,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         while (ok && done < sent) publish();
     } else if (SPLIT) {
         if (warp >= 4) {
-            __all_sync(0xffffffffu, mbar_wait(tfull, 0, abort_flag, a.err));
+            __all_sync(0xffffffffu, mbar_wait(tfull, 0, abort_flag, a));
             tc_fence_after();
         }
     } else if (warp >= 4) {
@@ -725,7 +736,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 __syncwarp();
                 if (t + t_step < order.tiles) fetch_bias(i + 1, n_next);
             }
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1u, abort_flag, a.err))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1u, abort_flag, a))) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(g * 32) << 16) + (i & 1u) * kAccStep;
 #pragma unroll 1
@@ -995,7 +1006,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
             for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a.err))) break;
+                    if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a))) break;
                     mbar_expect_tx(&full[s], kFewBase + (keeps_q ? 0 : q_rows) * kTileK);
                     tma_load_2d(smem + s * kFewBase, &map_b, kb * kTileK, (int)((int64_t)t * 256), &full[s]);
                     if (!keeps_q) tma_load_2d(smem + F::kOffQ + s * F::kQ, &map_q, kb * kTileK, 0, &full[s]);
@@ -1009,17 +1020,17 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const uint32_t leads = elect_leader();
         const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + F::kOffScales);
         uint32_t s = 0, par = 0, i = 0, group = 0;
-        bool ok = !keeps_q || __all_sync(0xffffffffu, mbar_wait(qfull, 0, abort_flag, a.err));
+        bool ok = !keeps_q || __all_sync(0xffffffffu, mbar_wait(qfull, 0, abort_flag, a));
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
             const uint32_t b = i & 1u;
-            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&tfree[b], ((i >> 1) - 1) & 1u, abort_flag, a.err))) break;
+            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&tfree[b], ((i >> 1) - 1) & 1u, abort_flag, a))) break;
             const uint32_t acc = tmem + b * 2 * NQ;
             for (int kb = 0; kb < k_blocks; ++kb) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a.err));
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a));
                 if (!ok) break;
                 const uint32_t slot = group % kScaleSlots, ta = tmem + 128 + group % kFewSlots * 16, tb = ta + 8;
                 if ((kb & 3) == 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a.err));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a));
                     if (!ok) break;
                 }
                 tc_fence_after();
@@ -1068,7 +1079,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
             for (int kb = 0; kb < k_blocks; kb += 4) {
                 const uint32_t slot = sent % kScaleSlots;
-                ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a.err));
+                ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a));
                 if (!ok) break;
                 const uint32_t dst = smem_u32(smem + F::kOffScales + slot * kScaleBytes) + lane * 16;
 #pragma unroll
@@ -1096,7 +1107,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             n += (int64_t)gridDim.x * 256;
             if (a.bias) next_bias = n < a.n ? a.bias[n] : 0.f;
             const uint32_t b = i & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[b], i >> 1 & 1u, abort_flag, a.err))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[b], i >> 1 & 1u, abort_flag, a))) break;
             tc_fence_after();
             uint32_t r[NQ];
             if constexpr (NQ == 16)

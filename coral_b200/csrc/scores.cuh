@@ -50,7 +50,8 @@ struct Fp8ScoresArgs {
     void* out;
     int type;
     int64_t ld;          // elements between rows of out
-    int* err;            // bounded-wait flag
+    int* err;            // set when a bounded wait ran out
+    long long wait_clocks;   // what a wait may take
 };
 cudaError_t launch_fp8_scores(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream);
 

@@ -174,7 +174,8 @@ float coral_last_total_ms(coral_index_t* h);
 /* Number of kernels this library launched on behalf of the handle so far. */
 int64_t coral_launch_count(coral_index_t* h);
 
-/* Tuning knobs (set before coral_search_prepare; none of them changes a result):
+/* Tuning knobs (set before coral_search_prepare; none of them changes a result, but for
+ * "score_wait_us", which can end a call without one):
  *   "ctas_per_sm", "warps"   resident CTAs per SM and warps per CTA; 0 = automatic (the warps in
  *                            3..6 that keep most warps resident; 8 warps for batches <= 4 x SMs)
  *   "chunk_bytes"            bytes of a row moved by one bulk copy; 0 = automatic (256, or up to
@@ -202,6 +203,9 @@ int64_t coral_launch_count(coral_index_t* h);
  *   "schedule"               run large batches grouped by the entry points' neighbour each query is
  *                            closest to, for L2 locality: 0 = automatic for batches >= 8192,
  *                            1 = always, -1 = never
+ *   "score_wait_us"          for how long a wait inside a coral_fp8_scores kernel may last before the
+ *                            kernel gives up (see coral_scores_check): 0 to 2000000 us, the default;
+ *                            calls already made, and graphs that hold them, keep the limit they had
  * coral_get_option also answers "plan_stages", "plan_warps", "plan_chunk_bytes",
  * "plan_smem_bytes", "plan_hash_bits", "plan_ctas_per_sm" (the plan of the most recent search or
  * prepare), "last_cluster_size", "last_scheduled", "frontier_size", "grid_cap", "deg_pad", "dim".

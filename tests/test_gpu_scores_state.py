@@ -1,0 +1,52 @@
+"""What a handle keeps for the score operators: the limit of bounded waits and the failures they leave."""
+import pytest
+import torch
+
+from coral_b200 import capi
+from tests.test_gpu_scores import BF16, F32, check_scores, rows8
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def ix():
+    with capi.Index(1, 4, 32, "ip") as h:
+        yield h
+        torch.cuda.synchronize()
+
+
+# A call of every kernel and way of storing: up to 16 and 32 queries, tiles shared by clusters, query tiles
+# with tensor stores, with an odd end and with plain stores.
+CALLS = [(3, 40_000, 200, F32, 0), (20, 40_000, 200, BF16, 0), (3, 700, 2100, F32, 0), (200, 60_000, 700, BF16, 0),
+         (200, 40_001, 200, F32, 0), (200, 40_001, 200, BF16, 1)]
+
+
+@pytest.mark.parametrize("Q,n,dim,dtype,lead", CALLS)
+def test_a_wait_that_runs_out_is_reported(ix, Q, n, dim, dtype, lead):
+    """With a limit of 0 the wait for the first codes runs out: the call ends, the check reports it once, and
+    the next call is right."""
+    q, base = rows8(ix, Q, dim, 1, 2), rows8(ix, n, dim, 2, 2)
+    out = torch.zeros(Q, n + 8, dtype=dtype, device="cuda")[:, lead:lead + n]
+    for _ in range(2):
+        ix.set_option("score_wait_us", 0)
+        ix.fp8_scores(q, base, dim, 2.0 ** -9, out=out)
+        torch.cuda.synchronize()
+        with pytest.raises(capi.CoralError) as e:
+            ix.scores_check()
+        assert e.value.code == capi.ERR_KERNEL and "wait" in str(e.value)
+        ix.scores_check()
+        ix.set_option("score_wait_us", 2_000_000)
+        ix.fp8_scores(q, base, dim, 2.0 ** -9, out=out)
+        torch.cuda.synchronize()
+        ix.scores_check()
+        check_scores(out, q, base, dim, 2.0 ** -9, None)
+
+
+def test_the_limit_of_waits(ix):
+    assert ix.get_option("score_wait_us") == 2_000_000
+    for v in (-1, 2_000_001):
+        with pytest.raises(capi.CoralError) as e:
+            ix.set_option("score_wait_us", v)
+        assert e.value.code == capi.ERR_ARG
+    ix.set_option("score_wait_us", 7)
+    assert ix.get_option("score_wait_us") == 7
