@@ -1481,13 +1481,15 @@ int coral_map_ids(coral_index_t* h, int32_t* d_ids, int64_t count, const int32_t
 
 namespace {
 
-// The device made current for one call, the caller's put back at its end.
+// The device made current for one call, the caller's put back at its end.  It is set even where it is
+// current already: in a thread that has used no GPU yet the device is current and its context is not, and
+// the driver's own calls (tensor maps) then fail.
 struct DeviceScope {
     int before = -1;
     bool ok = false;
     explicit DeviceScope(int device) {
         if (cudaGetDevice(&before) != cudaSuccess) before = -1;
-        ok = before == device || cudaSetDevice(device) == cudaSuccess;
+        ok = cudaSetDevice(device) == cudaSuccess;
         if (before == device) before = -1;
         if (!ok) cudaGetLastError();
     }
