@@ -633,5 +633,6 @@ class Index:
         return ids, best
 
     def scores_check(self):
-        """Raises when a bounded wait of an earlier fp8_scores ran out (call after synchronising)."""
+        """Raises when a bounded wait of an fp8_scores kernel ran out since this thread's last check (call after
+        synchronising); see coral_scores_check."""
         self._check(self._lib.coral_scores_check(self._h))

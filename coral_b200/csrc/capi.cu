@@ -5,9 +5,11 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <cstring>
 #include <map>
+#include <mutex>
 #include <new>
 #include <string>
 #include <vector>
@@ -27,6 +29,11 @@ using coral::SearchPlan;
 namespace {
 
 thread_local std::string g_create_error;
+
+// Handles are told apart by a number of their own: an address comes again after coral_index_destroy.
+std::atomic<uint64_t> g_handles;
+// Per handle, how many of its failed waits this thread has been told of.
+thread_local std::map<uint64_t, uint64_t> t_failures_told;
 
 // Control block shared with the kernel: word 0 = query counter | error flag, word 1 = hop
 // total, words 4..8 = record of the first failed index check (self-checking build only).
@@ -61,6 +68,7 @@ struct Options {
 }  // namespace
 
 struct coral_index {
+    const uint64_t number = g_handles.fetch_add(1) + 1;
     int device = 0;
     int sm_count = 0;
     int smem_optin = 0;
@@ -113,6 +121,8 @@ struct coral_index {
     unsigned long long* h_ctrl = nullptr;  // pinned mirror
     int64_t* d_hits = nullptr;
     int* h_scores_err = nullptr;           // pinned, written by the device when a bounded wait runs out
+    std::mutex failures_mu;
+    uint64_t failures = 0;                 // times that h_scores_err was found set
     std::map<int, std::pair<SearchPlan, int>> plans;  // L -> (plan, CTAs per SM)
 
     // graph build (NAP + CE): distances of the stored edges, degrees, claim words, batch scratch
@@ -431,6 +441,7 @@ int coral_index_destroy(coral_index_t* h) {
     if (h->ev_t1) cudaEventDestroy(h->ev_t1);
     if (h->stream) cudaStreamDestroy(h->stream);
     cudaGetLastError();
+    t_failures_told.erase(h->number);
     delete h;
     return CORAL_OK;
 }
@@ -1533,6 +1544,23 @@ bool meets(const void* p, int64_t bytes, const void* other, int64_t other_bytes)
     return meets(p, bytes, other, 1, other_bytes, other_bytes);
 }
 
+// How many of the handle's failed waits this thread has been told of; for a thread that comes to the handle
+// with a call of its own (`with_call`), those found before it do not count.  Null: out of host memory.
+uint64_t* failures_told(coral_index* h, bool with_call) {
+    const auto it = t_failures_told.find(h->number);
+    if (it != t_failures_told.end()) return &it->second;
+    uint64_t before = 0;
+    if (with_call) {
+        std::lock_guard<std::mutex> lock(h->failures_mu);
+        before = h->failures;
+    }
+    try {
+        return &t_failures_told.emplace(h->number, before).first->second;
+    } catch (const std::bad_alloc&) {
+        return nullptr;
+    }
+}
+
 constexpr long long kClocksPerUs = 2000;      // of an SM, for limits: B200 runs at up to 1965 MHz
 
 #define ARG(cond, text)                                             \
@@ -1608,6 +1636,7 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     a.ld = ld;
     a.err = h->h_scores_err;
     a.wait_clocks = h->opt.score_wait_us * kClocksPerUs;
+    if (!failures_told(h, true)) return fail(h, CORAL_ERR_LIMIT, "out of host memory");
     CK(coral::launch_fp8_scores(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
     h->launches += 1;
     return CORAL_OK;
@@ -1717,10 +1746,18 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
 
 int coral_scores_check(coral_index_t* h) {
     ARG(h, "null handle");
-    const int err = *static_cast<volatile int*>(h->h_scores_err);
-    *h->h_scores_err = 0;
-    if (err) return fail(h, CORAL_ERR_KERNEL, "a bounded wait in the score kernel ran out; its scores are invalid");
-    return CORAL_OK;
+    uint64_t* told = failures_told(h, false);
+    if (!told) return fail(h, CORAL_ERR_LIMIT, "out of host memory");
+    uint64_t now;
+    {
+        std::lock_guard<std::mutex> lock(h->failures_mu);
+        // in one step: a failure that the device writes meanwhile is kept for the next check
+        if (__atomic_exchange_n(h->h_scores_err, 0, __ATOMIC_ACQ_REL)) ++h->failures;
+        now = h->failures;
+    }
+    if (*told == now) return CORAL_OK;
+    *told = now;
+    return fail(h, CORAL_ERR_KERNEL, "a bounded wait in the score kernel ran out; its scores are invalid");
 }
 
 }  // extern "C"

@@ -463,8 +463,11 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
                       int32_t id_base, int32_t* d_ids_out, float* d_scores_out, void* d_workspace,
                       int64_t workspace_bytes, void* stream);
 
-/* After the stream has been synchronised: CORAL_ERR_KERNEL if a bounded wait of coral_fp8_scores ran
- * out since the last check (its scores are invalid), else CORAL_OK. */
+/* After the stream has been synchronised: CORAL_ERR_KERNEL if a bounded wait of a coral_fp8_scores kernel
+ * of this handle ran out, on any stream, since the calling thread's last check (since its first
+ * coral_fp8_scores call on the handle, if it has not checked; since the handle's creation, if it has done
+ * neither), else CORAL_OK.  The scores of the call that ran out are invalid; which call it was is not kept.
+ * Every thread is told: one thread's check takes nothing away from another's. */
 int coral_scores_check(coral_index_t* h);
 
 /* Last error text of the handle (or of handle creation when h is NULL). */

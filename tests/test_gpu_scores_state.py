@@ -1,4 +1,6 @@
 """What a handle keeps for the score operators: the limit of bounded waits and the failures they leave."""
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -50,3 +52,47 @@ def test_the_limit_of_waits(ix):
         assert e.value.code == capi.ERR_ARG
     ix.set_option("score_wait_us", 7)
     assert ix.get_option("score_wait_us") == 7
+
+
+class Worker:
+    """A thread that does what it is told, one thing after the other."""
+
+    def __init__(self):
+        self.pool = ThreadPoolExecutor(1)
+
+    def __call__(self, f, *args):
+        return self.pool.submit(f, *args).result()
+
+
+def failed(ix):
+    try:
+        ix.scores_check()
+        return False
+    except capi.CoralError as e:
+        assert e.code == capi.ERR_KERNEL
+        return True
+
+
+def test_every_thread_is_told_of_a_failed_wait(ix):
+    q, base = rows8(ix, 3, 200, 1, 2), rows8(ix, 5000, 200, 2, 2)
+
+    def call(limit):
+        ix.set_option("score_wait_us", limit)
+        ix.fp8_scores(q, base, 200)
+        torch.cuda.synchronize()
+        ix.set_option("score_wait_us", 2_000_000)
+    first, second, late, watcher = (Worker() for _ in range(4))
+    first(call, 2_000_000)
+    second(call, 2_000_000)
+    assert not first(failed, ix) and not second(failed, ix)
+    first(call, 0)
+    assert second(failed, ix) and first(failed, ix)           # one's check leaves the other's
+    assert not second(failed, ix) and not first(failed, ix)   # once
+    late(call, 2_000_000)
+    assert not late(failed, ix)                               # what was found before it came is not its own
+    assert watcher(failed, ix) and not watcher(failed, ix)    # no call of its own: all since the handle's creation
+    second(call, 0)
+    first(call, 2_000_000)
+    assert [w(failed, ix) for w in (first, late, second, watcher)] == [True] * 4
+    with capi.Index(1, 4, 32, "ip") as other:
+        assert not first(failed, other) and not watcher(failed, other)
