@@ -28,7 +28,15 @@ using coral::SearchPlan;
 
 namespace {
 
-thread_local std::string g_create_error;
+thread_local std::string g_create_error;      // failures without a handle
+
+// A thread's last failure with a handle: another thread's on the same handle does not replace the text
+// that this one is about to ask for.
+struct LastError {
+    uint64_t handle = 0;
+    std::string text;
+};
+thread_local LastError t_error;
 
 // Handles are told apart by a number of their own: an address comes again after coral_index_destroy.
 std::atomic<uint64_t> g_handles;
@@ -141,16 +149,24 @@ struct coral_index {
 
     float last_kernel_ms = 0.f, last_total_ms = 0.f;
     int64_t launches = 0;
-    std::string err;
+    std::atomic<int64_t> score_launches{0};   // of the score operators, which threads call side by side
+    std::mutex err_mu;
+    std::string err;                       // of any thread's last failure
 };
 
 namespace {
 
 int fail(coral_index* h, int code, const std::string& msg) {
-    if (h)
-        h->err = msg;
-    else
+    if (!h) {
         g_create_error = msg;
+        return code;
+    }
+    {
+        std::lock_guard<std::mutex> lock(h->err_mu);
+        h->err = msg;
+    }
+    t_error.text = msg;
+    t_error.handle = h->number;
     return code;
 }
 
@@ -360,7 +376,14 @@ int coral_internal_grant_slot(int device, int metric, int cluster) {
 }
 int coral_compiled_sm(void) { return 100; }
 
-const char* coral_last_error(coral_index_t* h) { return h ? h->err.c_str() : g_create_error.c_str(); }
+const char* coral_last_error(coral_index_t* h) {
+    if (!h) return g_create_error.c_str();
+    if (t_error.handle == h->number) return t_error.text.c_str();
+    thread_local std::string any;      // of another thread, or of a call before this thread's last failure elsewhere
+    std::lock_guard<std::mutex> lock(h->err_mu);
+    any = h->err;
+    return any.c_str();
+}
 
 int coral_index_create(coral_index_t** out, int device, int64_t n, int dim, int max_degree, int metric) {
     coral_index* h = nullptr;
@@ -956,7 +979,7 @@ int coral_search(coral_index_t* h, const float* queries, int Q, int L, int k, in
 
 float coral_last_kernel_ms(coral_index_t* h) { return h ? h->last_kernel_ms : 0.f; }
 float coral_last_total_ms(coral_index_t* h) { return h ? h->last_total_ms : 0.f; }
-int64_t coral_launch_count(coral_index_t* h) { return h ? h->launches : 0; }
+int64_t coral_launch_count(coral_index_t* h) { return h ? h->launches + h->score_launches : 0; }
 
 int coral_count_hits(coral_index_t* h, const int32_t* res, const int32_t* gt, int Q, int k, int gt_dim,
                      int64_t* hits_out) {
@@ -1595,7 +1618,7 @@ int coral_fp8_quantize(coral_index_t* h, const void* d_x, int type, int64_t rows
         "an output overlaps another array");
     CK(coral::launch_fp8_quantize(d_x, type, rows, dim, ld, d_codes, d_scales, h->sm_count,
                                   stream ? (cudaStream_t)stream : h->stream));
-    h->launches += 1;
+    h->score_launches += 1;
     return CORAL_OK;
 }
 
@@ -1638,7 +1661,7 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     a.wait_clocks = h->opt.score_wait_us * kClocksPerUs;
     if (!failures_told(h, true)) return fail(h, CORAL_ERR_LIMIT, "out of host memory");
     CK(coral::launch_fp8_scores(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
-    h->launches += 1;
+    h->score_launches += 1;
     return CORAL_OK;
 }
 
@@ -1692,7 +1715,7 @@ int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q,
     a.excluded = d_excluded;
     a.ld_excluded = ld_excluded;
     CK(coral::launch_score_rules(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
-    h->launches += 1;
+    h->score_launches += 1;
     return CORAL_OK;
 }
 
@@ -1740,7 +1763,7 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
     a.ws = static_cast<uint64_t*>(d_workspace);
     int launches = 0;
     CK(coral::launch_topk(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream, &launches));
-    h->launches += launches;
+    h->score_launches += launches;
     return CORAL_OK;
 }
 

@@ -409,9 +409,11 @@ int coral_search_static_status(int device);
  * All five take device pointers of the handle's GPU (checked; CORAL_ERR_ARG else), need no vectors in
  * the handle, keep no state between calls, enqueue on `stream` (NULL = the handle's stream) without
  * synchronising and leave the caller's current device as it was.  They allocate nothing, so they can
- * be captured into a graph; a workspace belongs to one call at a time.  An output that overlaps another
- * array of its call is refused (but coral_adjust_scores works in place).  Empty sizes are allowed and
- * launch nothing (coral_topk_scores still writes its padding). */
+ * be captured into a graph (which must not be replayed after the handle is destroyed); a workspace belongs
+ * to one call at a time.  Threads may make these calls on one handle side by side (any other call on the
+ * handle waits for them, coral_set_option too).  An output that overlaps another array of its call is
+ * refused (but coral_adjust_scores works in place).  Empty sizes are allowed and launch nothing
+ * (coral_topk_scores still writes its padding). */
 
 /* element types */
 #define CORAL_F32 0
@@ -470,7 +472,9 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
  * Every thread is told: one thread's check takes nothing away from another's. */
 int coral_scores_check(coral_index_t* h);
 
-/* Last error text of the handle (or of handle creation when h is NULL). */
+/* Last error text of the handle (or of handle creation when h is NULL): the calling thread's own if its
+ * last failure was on this handle, else the last of any thread's.  The text stays until the calling
+ * thread's next call. */
 const char* coral_last_error(coral_index_t* h);
 
 #ifdef __cplusplus
