@@ -1546,6 +1546,13 @@ bool usable(const coral_index* h, const void* p, size_t align) {
 bool score_type(int type) { return type == CORAL_F32 || type == CORAL_BF16 || type == CORAL_F16; }
 size_t score_align(int type) { return (size_t)coral::type_bytes(type); }
 
+// Whether some GPU's memory could hold Q rows of n elements, ld apart (16 TB; so that offsets in bytes and
+// numbers of CTAs cannot overflow).  Arrays' real extents are the caller's.
+bool fits(int64_t Q, int64_t n, int64_t ld, int64_t size) {
+    return Q <= 1 || ld == 0 || (Q - 1) <= ((1ll << 44) - n * size) / size / ld;
+}
+constexpr char kTooFar[] = "the rows reach further than any GPU's memory";
+
 // Whether elements of two arrays of Q rows x n columns can share memory (pointers differ).
 bool rows_overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int size, int64_t Q, int64_t n) {
     const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
@@ -1605,6 +1612,7 @@ int coral_fp8_quantize(coral_index_t* h, const void* d_x, int type, int64_t rows
     ARG(dim >= 1 && dim <= coral::kFp8MaxDim, "dim must be in [1, 65536]");
     ARG(rows >= 0 && rows <= 0x7fffffffll, "rows must be in [0, 2^31)");
     ARG(ld >= dim && ld < (1ll << 31), "ld must be in [dim, 2^31)");
+    if (!fits(rows, dim, ld, 4)) return fail(h, CORAL_ERR_LIMIT, kTooFar);
     if (rows == 0) return CORAL_OK;
     ARG(d_x && d_codes && d_scales, "null argument");
     DeviceScope scope(h->device);
@@ -1632,6 +1640,7 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     ARG(ld >= n && ld < (1ll << 31), "ld must be in [n, 2^31)");
     if (((int64_t)Q + 127) / 128 * ((n + 255) / 256) > 0x7fffffffll / 2)
         return fail(h, CORAL_ERR_LIMIT, "too many scores for one call");
+    if (!fits(Q, n, ld, 4)) return fail(h, CORAL_ERR_LIMIT, kTooFar);
     if (Q == 0 || n == 0) return CORAL_OK;
     ARG(d_q_codes && d_q_scales && d_codes && d_scales && d_out, "null argument");
     DeviceScope scope(h->device);
@@ -1681,6 +1690,8 @@ int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q,
     ARG(d_scores && d_out && (n_seen == 0 || (d_seen && d_penalties)) && (n_bias == 0 || (d_bias_ids && d_bias)),
         "null argument");
     ARG(!d_excluded || ld_excluded == 0 || ld_excluded >= (n + 31) / 32, "ld_excluded must be 0 or at least (n + 31) / 32");
+    if (!fits(Q, n, ld, 4) || !fits(Q, n, ld_out, 4) || (d_excluded && !fits(Q, (n + 31) / 32, ld_excluded, 4)))
+        return fail(h, CORAL_ERR_LIMIT, kTooFar);
     DeviceScope scope(h->device);
     if (!scope.ok) return fail(h, CORAL_ERR_CUDA, "cudaSetDevice failed");
     ARG(usable(h, d_scores, score_align(type)) && usable(h, d_out, score_align(type)) &&
@@ -1736,6 +1747,7 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
     ARG(ld >= n && ld < (1ll << 31), "ld must be in [n, 2^31)");
     ARG(id_base >= 0 && id_base + n <= 0x7fffffffll, "id_base must be in [0, 2^31 - n)");
     if (Q == 0) return CORAL_OK;
+    if (n > 0 && !fits(Q, n, ld, 4)) return fail(h, CORAL_ERR_LIMIT, kTooFar);
     ARG((n == 0 || d_scores) && d_ids_out && d_scores_out && (need == 0 || d_workspace), "null argument");
     if (workspace_bytes < need) return fail(h, CORAL_ERR_LIMIT, "workspace smaller than coral_topk_workspace");
     DeviceScope scope(h->device);

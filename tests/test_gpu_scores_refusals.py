@@ -1,0 +1,36 @@
+"""Refusals of the score operators: sizes that no array has."""
+import pytest
+import torch
+
+from coral_b200 import capi
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def ix():
+    with capi.Index(1, 4, 32, "ip") as h:
+        yield h
+        torch.cuda.synchronize()
+
+
+def test_rows_that_reach_too_far(ix):
+    """Strides whose last row's offset overflows, or nearly: refused, whatever the checks of overlap make of them."""
+    lib, h = ix._lib, ix._h
+    buf = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    d, far, L, OK = buf.data_ptr(), (1 << 31) - 1, capi.ERR_LIMIT, capi.OK
+    e = d + (1 << 19)
+    for rows, ld in ((far, far), (far, 1 << 16), (1 << 20, 1 << 29), (3, 1 << 61)):
+        if ld <= far:
+            assert lib.coral_fp8_quantize(h, d, 0, rows, 64, ld, e, e, 1) == L
+            assert lib.coral_fp8_scores(h, d, d, rows, d, d, 1, 64, 1.0, None, e, 0, ld, 1) == L
+            assert lib.coral_adjust_scores(h, d, 0, rows, 1, ld, None, 0, None, None, None, 0, None, 0, e, 1, 1) == L
+            assert lib.coral_adjust_scores(h, d, 0, rows, 1, 1, None, 0, None, None, None, 0, None, 0, e, ld, 1) == L
+            assert lib.coral_topk_scores(h, d, 0, rows, 1, ld, 1, 0, e, e, None, 0, 1) == L
+        assert lib.coral_adjust_scores(h, d, 0, rows, 1, 1, None, 0, None, None, None, 0, d, ld, e, 1, 1) == L
+    # rows of many columns that fill more than any memory: more CTAs than a grid has
+    assert lib.coral_topk_scores(h, d, 0, far, far, far, 1, 0, e, e, e, 1 << 62, 1) == L
+    # one row has no next one
+    assert lib.coral_topk_scores(h, d, 0, 1, 16, far, 2, 0, e, e + 64, None, 0, 1) == OK
+    assert lib.coral_adjust_scores(h, d, 0, 1, 16, far, None, 0, None, None, None, 0, d, 1 << 61, e, far, 1) == OK
+    torch.cuda.synchronize()
