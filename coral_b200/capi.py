@@ -174,6 +174,13 @@ def _use_torch():
     return _torch
 
 
+def _apart(n: int, dtype):
+    """Elements between rows of n that start at multiples of 16 bytes (n where that is no number below 2^31)."""
+    per = 16 // dtype.itemsize
+    ld = (n + per - 1) // per * per
+    return n if ld >> 31 else ld
+
+
 def _refuse(name: str, what: str):
     raise CoralError(ERR_ARG, f"{name} must be {what}")
 
@@ -542,8 +549,7 @@ class Index:
         if out is None:
             # rows start at multiples of 16 bytes whatever n: what follows loads and stores whole vectors
             dtype = dtype or torch.float32
-            per = 16 // dtype.itemsize
-            ld = (n + per - 1) // per * per
+            ld = _apart(n, dtype)
             kind = _score_types.get(dtype)
             if kind is None:
                 _refuse("dtype", "float32, bfloat16 or float16")
@@ -572,8 +578,7 @@ class Index:
         p, kind, Q, n, ld = self._rows("scores", scores)
         if out is None:
             # rows as far apart as the input's are when that is tight, else at multiples of 16 bytes
-            per = 16 // scores.dtype.itemsize
-            ld_out = n if ld == n else (n + per - 1) // per * per
+            ld_out = n if ld == n else _apart(n, scores.dtype)
             out = torch.empty_like(scores) if ld == n else scores.new_empty((Q, ld_out))
             po = out.data_ptr()
             if ld_out != n:

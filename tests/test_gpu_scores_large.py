@@ -1,5 +1,5 @@
 """Score operators at their far ends: output rows past 2^31 elements, several chunks of the tile order, long
-rows with exact sums, and scales far apart.
+rows with exact sums, scales far apart, and as many columns as there are ids.
 
 Exact sums: codes are small integers and scales powers of two whose product is 1, 2 or 4, so that every
 partial sum of at most 65536 products of at most 4 * 4 is an integer below 2^24 in magnitude, whatever the
@@ -7,7 +7,7 @@ order: the product has to equal the one in 64 bits."""
 import pytest
 import torch
 
-from tests.test_gpu_scores import BF16, F16, F32, check_scores, decode, gen, rows8
+from tests.test_gpu_scores import BF16, F16, F32, FLT_MAX, check_scores, decode, gen, rows8
 from tests.test_gpu_scores_state import ix  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +112,42 @@ def test_scales_far_apart(ix, Q, n, far):  # noqa: F811
         q, base = exact_rows(Q, dim, exponents, 10), exact_rows(n, dim, -exponents, 11)
         out = ix.fp8_scores(q, base, dim)
         assert torch.equal(out.double(), exact_scores(q, base, dim, exponents))
+
+
+def test_as_many_columns_as_ids(ix):  # noqa: F811
+    """2^31 - 1 rows of one column through all four operators: the first, the last, and some between."""
+    n = 2 ** 31 - 1
+    at = torch.tensor([0, 1, 255, 256, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 300, 2 ** 31 - 257, 2 ** 31 - 256, 2 ** 31 - 3, 2 ** 31 - 2],
+                      device="cuda")
+    val = torch.tensor([3.0, 5.0, 8.0, -2.0, 9.0, 13.0, 4.0, 7.0, 14.0, 6.0, 15.0], device="cuda")
+    x = torch.zeros(n, 1, dtype=BF16, device="cuda")
+    x[at, 0] = val.to(BF16)
+    base = ix.fp8_quantize(x)
+    del x
+    some = tuple(t[at] for t in base)
+    assert torch.equal(decode(*some, 1)[:, 0].float(), val)
+    q = ix.fp8_quantize(torch.ones(1, 1, device="cuda"))
+    s = ix.fp8_scores(q, base, 1, dtype=BF16)
+    del base, some
+    assert s.shape == (1, n) and torch.equal(s[0, at].float(), val)
+    assert sum(int(torch.count_nonzero(s[0, j:j + 2 ** 28])) for j in range(0, n, 2 ** 28)) == len(at)
+    seen = torch.tensor([[2 ** 31 - 2, 0, -1, 2 ** 30, 2 ** 30]], dtype=torch.int32, device="cuda")
+    pen = torch.tensor([[1.0, 1.0, 0.5]], device="cuda")
+    ids = torch.tensor([[2 ** 31 - 3, -5]], dtype=torch.int32, device="cuda")
+    bias = torch.tensor([[10.0, 99.0]], device="cuda")
+    ex = torch.zeros(1, -(-n // 32), dtype=torch.int32, device="cuda")
+    ex[0, (2 ** 31 - 256) // 32] = 1
+    s = ix.adjust_scores(s, seen, pen, ids, bias, ex, out=s)
+    want = {0: 1.5, 1: 5.0, 255: 8.0, 256: -2.0, 2 ** 30 - 1: 9.0, 2 ** 30: 10.5, 2 ** 31 - 300: 4.0, 2 ** 31 - 257: 7.0,
+            2 ** 31 - 256: -float("inf"), 2 ** 31 - 3: 16.0, 2 ** 31 - 2: 13.5}
+    assert s[0, at].tolist() == [want[j] for j in at.tolist()]
+    ids, best = ix.topk_scores(s, 9)
+    order = sorted((j for j in want if want[j] > 0), key=lambda j: -want[j])
+    assert ids[0].tolist() == order and best[0].tolist() == [want[j] for j in order]
+    ids, best = ix.topk_scores(s, 1000)      # the rest: zeros, by id
+    zeros = [j for j in range(1100) if j not in want][:1000 - len(order)]
+    assert ids[0].tolist() == order + zeros
+    s[0] = -float("inf")
+    s[0, n - 1] = -FLT_MAX / 2
+    ids, best = ix.topk_scores(s, 2)
+    assert ids[0].tolist() == [n - 1, -1]
