@@ -549,18 +549,18 @@ class Index:
         if out is None:
             # rows start at multiples of 16 bytes whatever n: what follows loads and stores whole vectors
             dtype = dtype or torch.float32
-            ld = _apart(n, dtype)
             kind = _score_types.get(dtype)
             if kind is None:
                 _refuse("dtype", "float32, bfloat16 or float16")
+            ld = _apart(n, dtype)
             out = base[0].new_empty((Q, ld), dtype=dtype)
             po = out.data_ptr()
             if ld != n:
                 out = out[:, :n]
         else:
+            po, kind, rows, cols, ld = self._rows("out", out)
             if dtype is not None and out.dtype is not dtype:
                 _refuse("out", str(dtype))
-            po, kind, rows, cols, ld = self._rows("out", out)
             if rows != Q or cols != n:
                 _refuse("out", f"of shape {[Q, n]}")
         rc = self._lib.coral_fp8_scores(self._h, pq, sq, Q, pr, sr, n, dim, alpha, pb, po, kind, ld,

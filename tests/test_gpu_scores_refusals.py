@@ -34,3 +34,14 @@ def test_rows_that_reach_too_far(ix):
     assert lib.coral_topk_scores(h, d, 0, 1, 16, far, 2, 0, e, e + 64, None, 0, 1) == OK
     assert lib.coral_adjust_scores(h, d, 0, 1, 16, far, None, 0, None, None, None, 0, d, 1 << 61, e, far, 1) == OK
     torch.cuda.synchronize()
+
+
+def test_types_that_are_none(ix):
+    """What is no type, and what is no tensor, is refused as every argument is."""
+    x = torch.randn(4, 64, device="cuda")
+    q = ix.fp8_quantize(x)
+    for kw in ({"dtype": "float32"}, {"dtype": float}, {"dtype": torch.float64}, {"out": 5}, {"out": 5, "dtype": torch.float32},
+               {"out": [[0.0] * 4] * 4, "dtype": torch.float32}):
+        with pytest.raises(capi.CoralError) as e:
+            ix.fp8_scores(q, q, 64, **kw)
+        assert e.value.code == capi.ERR_ARG
