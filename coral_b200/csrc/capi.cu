@@ -1624,7 +1624,7 @@ int coral_fp8_quantize(coral_index_t* h, const void* d_x, int type, int64_t rows
     ARG(!meets(d_codes, code_bytes, d_x, rows, dim * size, ld * size) && !meets(d_scales, scale_bytes, d_x, rows, dim * size, ld * size) &&
             !meets(d_codes, code_bytes, d_scales, scale_bytes),
         "an output overlaps another array");
-    CK(coral::launch_fp8_quantize(d_x, type, rows, dim, ld, d_codes, d_scales, h->sm_count,
+    CK(coral::launch_fp8_quantize(d_x, type, rows, dim, ld, d_codes, d_scales,
                                   stream ? (cudaStream_t)stream : h->stream));
     h->score_launches += 1;
     return CORAL_OK;
@@ -1725,7 +1725,7 @@ int coral_adjust_scores(coral_index_t* h, const void* d_scores, int type, int Q,
     a.n_bias = n_bias;
     a.excluded = d_excluded;
     a.ld_excluded = ld_excluded;
-    CK(coral::launch_score_rules(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
+    CK(coral::launch_score_rules(a, stream ? (cudaStream_t)stream : h->stream));
     h->score_launches += 1;
     return CORAL_OK;
 }

@@ -1303,7 +1303,7 @@ cudaError_t scores_t(const Fp8ScoresArgs& a, int sm_count, cudaStream_t stream) 
 }  // namespace
 
 cudaError_t launch_fp8_quantize(const void* x, int type, int64_t rows, int dim, int64_t ld, uint8_t* codes,
-                                uint8_t* scales, int, cudaStream_t stream) {
+                                uint8_t* scales, cudaStream_t stream) {
     if (type == kTypeF32) return quantize_t<float>(x, rows, dim, ld, codes, scales, stream);
     if (type == kTypeBf16) return quantize_t<__nv_bfloat16>(x, rows, dim, ld, codes, scales, stream);
     return quantize_t<__half>(x, rows, dim, ld, codes, scales, stream);

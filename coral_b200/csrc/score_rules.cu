@@ -232,7 +232,7 @@ cudaError_t launch_rules(const RulesArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_score_rules(const RulesArgs& a, int, cudaStream_t stream) {
+cudaError_t launch_score_rules(const RulesArgs& a, cudaStream_t stream) {
     if (a.type == kTypeF32) return launch_rules<float>(a, stream);
     if (a.type == kTypeBf16) return launch_rules<__nv_bfloat16>(a, stream);
     return launch_rules<__half>(a, stream);

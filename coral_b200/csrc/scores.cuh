@@ -27,7 +27,7 @@ inline int64_t fp8_code_pitch(int dim) { return ((int64_t)dim + 15) / 16 * 16; }
 inline int64_t fp8_scale_pitch(int dim) { return ((int64_t)dim + 511) / 512 * 4; }
 
 cudaError_t launch_fp8_quantize(const void* x, int type, int64_t rows, int dim, int64_t ld, uint8_t* codes,
-                                uint8_t* scales, int sm_count, cudaStream_t stream);
+                                uint8_t* scales, cudaStream_t stream);
 
 // Opt-in shared memory of a kernel, asked for once per kernel and device.
 template <typename Kernel>
@@ -69,7 +69,7 @@ struct RulesArgs {
     const uint32_t* excluded;   // rows of words, ld_excluded apart (0: one row for all)
     int64_t ld_excluded;
 };
-cudaError_t launch_score_rules(const RulesArgs& a, int sm_count, cudaStream_t stream);
+cudaError_t launch_score_rules(const RulesArgs& a, cudaStream_t stream);
 
 struct TopkArgs {
     const void* in;
