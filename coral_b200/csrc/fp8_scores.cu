@@ -37,15 +37,6 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     return r;
 }
 
-template <typename T>
-__device__ __forceinline__ float wide(T v);
-template <>
-__device__ __forceinline__ float wide<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float wide<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float wide<__half>(__half v) { return __half2float(v); }
-
 constexpr int kQuantThreads = 256;
 constexpr int kQuantLoads = 8;    // 16-byte loads a lane has in flight
 
@@ -180,7 +171,7 @@ fp8_quantize_kernel(const T* __restrict__ x, int64_t rows, int dim, int64_t ld, 
             uint32_t q[E / 4];
 #pragma unroll
             for (int k = 0; k < E; k += 4)
-                q[k / 4] = pack_e4m3(wide<T>(w[k]) * f, wide<T>(w[k + 1]) * f, wide<T>(w[k + 2]) * f, wide<T>(w[k + 3]) * f);
+                q[k / 4] = pack_e4m3(to_f32<T>(w[k]) * f, to_f32<T>(w[k + 1]) * f, to_f32<T>(w[k + 2]) * f, to_f32<T>(w[k + 3]) * f);
             if (codes_left > j * G * E) {
                 if (E == 4)
                     *reinterpret_cast<uint32_t*>(to + j * G * E) = q[0];
@@ -422,15 +413,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-template <typename T>
-__device__ __forceinline__ T narrow(float v);
-template <>
-__device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -811,7 +793,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                             if (n < a.n) {
                                 T* out = static_cast<T*>(a.out) + m0 * a.ld + n;
 #pragma unroll 4
-                                for (int j = 0; j < rows; ++j) out[j * a.ld] = narrow<T>(tile[j * 32 + (lane ^ j)]);
+                                for (int j = 0; j < rows; ++j) out[j * a.ld] = from_f32<T>(tile[j * 32 + (lane ^ j)]);
                             }
                         }
                     }
@@ -876,7 +858,7 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 const float y[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    v[e] = narrow<T>(fmaf(a.alpha, y[e], a.bias && n + e < a.n ? a.bias[n + e] : 0.f));
+                    v[e] = from_f32<T>(fmaf(a.alpha, y[e], a.bias && n + e < a.n ? a.bias[n + e] : 0.f));
                 if (whole && n + 4 <= a.n) {
                     if (sizeof(T) == 4)
                         *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(v);
@@ -1121,7 +1103,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
                 if (q >= a.Q) break;
-                if (there) *out = narrow<T>(fmaf(a.alpha, __uint_as_float(r[q]), bias));
+                if (there) *out = from_f32<T>(fmaf(a.alpha, __uint_as_float(r[q]), bias));
                 out += a.ld;
             }
         }

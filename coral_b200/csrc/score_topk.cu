@@ -51,15 +51,6 @@ struct Shared {
     float least;          // scores below it cannot be among the k best
 };
 
-template <typename T>
-__device__ __forceinline__ float score_of(T v);
-template <>
-__device__ __forceinline__ float score_of<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float score_of<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float score_of<__half>(__half v) { return __half2float(v); }
-
 __device__ __forceinline__ uint32_t ord_of(float s) {
     const uint32_t u = __float_as_uint(s + 0.f);      // one zero
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
@@ -325,7 +316,7 @@ __device__ __forceinline__ void collect(Shared& sh, int noted, float least, cons
     constexpr int V = Step<T>::V;
     for (int i = threadIdx.x; i < noted * V; i += kThreads) {
         const int j = (int)sh.notes[i / V] * V + i % V;
-        const float s = score_of<T>(cols[j]);
+        const float s = to_f32<T>(cols[j]);
         if (s >= least) append(sh, s, c0 + (uint32_t)j);
     }
 }
@@ -377,7 +368,7 @@ topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice, const 
     if (tid == 0) sh.cnt = sh.noted = 0;
     const int odd = tid < head ? tid - head : end + tid - 32;      // from the boundary
     const bool has_odd = tid < head || (tid >= 32 && tid - 32 < left);
-    const float rest = has_odd ? score_of<T>(cols[odd]) : -CUDART_INF_F;
+    const float rest = has_odd ? to_f32<T>(cols[odd]) : -CUDART_INF_F;
     Scores step;
     Maxima<T> maxima;
     for (int t0 = 0; t0 < end; t0 += Scores::kScores) {
@@ -407,7 +398,7 @@ topk_scan_kernel(const TopkArgs a, const int splits, const int64_t slice, const 
             const float least = sh.least;
             for (int i = 0; i < Scores::V; ++i) {
                 const int j = t0 + tid * Scores::V + i;
-                const float s = j < len ? score_of<T>(first[j]) : -CUDART_INF_F;
+                const float s = j < len ? to_f32<T>(first[j]) : -CUDART_INF_F;
                 if (s >= least) append(sh, s, (uint32_t)(row0 + j));
             }
             __syncthreads();

@@ -15,6 +15,24 @@ namespace coral {
 constexpr int kTypeF32 = 0, kTypeBf16 = 1, kTypeF16 = 2;
 inline int type_bytes(int type) { return type == kTypeF32 ? 4 : 2; }
 
+// Elements and fp32, to nearest even on the way back.
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
 constexpr int kFp8Block = 128;        // columns that share one scale
 constexpr int kFp8MaxDim = 1 << 16;
 constexpr int kTopkMax = 1024;        // k of the selection
