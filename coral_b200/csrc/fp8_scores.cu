@@ -303,23 +303,32 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint64_t* bar, uint32_t parity
         : "memory");
     return ok;
 }
-// Bounded wait: gives up when a.wait_clocks have gone by (0: if the phase is not over already) or another
-// role of the CTA gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const Fp8ScoresArgs& a) {
-    if (mbar_test_wait(bar, parity)) return true;
+// Bounded wait for a phase that a test has not found over: gives up when `limit` clocks have gone by (0: at
+// once; try_wait would itself wait for a while) or another role of the CTA gave up.
+__device__ __forceinline__ bool mbar_wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, long long limit) {
     const long long t0 = clock64();
-    for (uint32_t spins = 0;; ++spins) {
+    for (uint32_t spins = 1; limit != 0; ++spins) {
+        if (mbar_try_wait(bar, parity)) return true;
         if ((spins & 15u) == 0u) {
             if (*abort_flag) return false;
-            if (clock64() - t0 >= a.wait_clocks) {
-                *abort_flag = 1;
-                *static_cast<volatile int*>(a.err) = 1;
-                __threadfence_system();
-                return false;
-            }
+            if (clock64() - t0 > limit) break;
         }
-        if (mbar_try_wait(bar, parity)) return true;
     }
+    *abort_flag = 1;
+    *static_cast<volatile int*>(err) = 1;
+    __threadfence_system();
+    return false;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const Fp8ScoresArgs& a) {
+    return mbar_test_wait(bar, parity) || mbar_wait_on(bar, parity, abort_flag, a.err, a.wait_clocks);
+}
+// The same with the loop out of line, for the kernel of few queries (1 x 4M x 128: 83.2 us, 84.0 with it inline;
+// the query tiles lose by it: 4096 x 8192 x 4096 119.8 us for 117.6).
+__device__ __noinline__ bool mbar_wait_apart(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, long long limit) {
+    return mbar_wait_on(bar, parity, abort_flag, err, limit);
+}
+__device__ __forceinline__ bool mbar_wait_few(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const Fp8ScoresArgs& a) {
+    return mbar_test_wait(bar, parity) || mbar_wait_apart(bar, parity, abort_flag, a.err, a.wait_clocks);
 }
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
     asm volatile(
@@ -988,7 +997,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
             for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!(ok = mbar_wait(&empty[s], par ^ 1u, abort_flag, a))) break;
+                    if (!(ok = mbar_wait_few(&empty[s], par ^ 1u, abort_flag, a))) break;
                     mbar_expect_tx(&full[s], kFewBase + (keeps_q ? 0 : q_rows) * kTileK);
                     tma_load_2d(smem + s * kFewBase, &map_b, kb * kTileK, (int)((int64_t)t * 256), &full[s]);
                     if (!keeps_q) tma_load_2d(smem + F::kOffQ + s * F::kQ, &map_q, kb * kTileK, 0, &full[s]);
@@ -1002,17 +1011,17 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const uint32_t leads = elect_leader();
         const uint32_t codes = smem_u32(smem), scales = smem_u32(smem + F::kOffScales);
         uint32_t s = 0, par = 0, i = 0, group = 0;
-        bool ok = !keeps_q || __all_sync(0xffffffffu, mbar_wait(qfull, 0, abort_flag, a));
+        bool ok = !keeps_q || __all_sync(0xffffffffu, mbar_wait_few(qfull, 0, abort_flag, a));
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
             const uint32_t b = i & 1u;
-            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&tfree[b], ((i >> 1) - 1) & 1u, abort_flag, a))) break;
+            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_few(&tfree[b], ((i >> 1) - 1) & 1u, abort_flag, a))) break;
             const uint32_t acc = tmem + b * 2 * NQ;
             for (int kb = 0; kb < k_blocks; ++kb) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, abort_flag, a));
+                ok = __all_sync(0xffffffffu, mbar_wait_few(&full[s], par, abort_flag, a));
                 if (!ok) break;
                 const uint32_t slot = group % kScaleSlots, ta = tmem + 128 + group % kFewSlots * 16, tb = ta + 8;
                 if ((kb & 3) == 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a));
+                    ok = __all_sync(0xffffffffu, mbar_wait_few(&sfull[slot], group / kScaleSlots & 1u, abort_flag, a));
                     if (!ok) break;
                 }
                 tc_fence_after();
@@ -1061,7 +1070,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
             for (int kb = 0; kb < k_blocks; kb += 4) {
                 const uint32_t slot = sent % kScaleSlots;
-                ok = __all_sync(0xffffffffu, mbar_wait(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a));
+                ok = __all_sync(0xffffffffu, mbar_wait_few(&sempty[slot], (sent / kScaleSlots & 1u) ^ 1u, abort_flag, a));
                 if (!ok) break;
                 const uint32_t dst = smem_u32(smem + F::kOffScales + slot * kScaleBytes) + lane * 16;
 #pragma unroll
@@ -1089,7 +1098,7 @@ fp8_few_scores_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             n += (int64_t)gridDim.x * 256;
             if (a.bias) next_bias = n < a.n ? a.bias[n] : 0.f;
             const uint32_t b = i & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[b], i >> 1 & 1u, abort_flag, a))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait_few(&tfull[b], i >> 1 & 1u, abort_flag, a))) break;
             tc_fence_after();
             uint32_t r[NQ];
             if constexpr (NQ == 16)
