@@ -532,7 +532,8 @@ class Index:
     def fp8_scores(self, queries, base, dim: int, alpha: float = 1.0, bias=None, dtype=None, out=None):
         """alpha * <query, row> + bias[row] of compressed queries and base rows (pairs as fp8_quantize
         returns them) of `dim` columns: [Q, n] in `dtype` (float32 unless given), or into `out`, whose
-        rows may be apart.  See coral_fp8_scores."""
+        rows may be apart.  A new result's rows start at multiples of 16 bytes: where n is no multiple of 4
+        (8 in 16 bits) it is a view of a wider matrix, not contiguous for Q > 1.  See coral_fp8_scores."""
         torch = _torch or _use_torch()
         if not 1 <= dim <= FP8_MAX_DIM:
             raise CoralError(ERR_ARG, f"dim must be in [1, {FP8_MAX_DIM}]")
@@ -572,8 +573,8 @@ class Index:
     def adjust_scores(self, scores, seen=None, penalties=None, bias_ids=None, bias=None, excluded=None, out=None):
         """Rules on a matrix of scores (see coral_adjust_scores): seen int32 [Q, *] with -1 padding,
         penalties float32 [Q, 3] (repetition, frequency, presence), bias_ids int32 and bias float32
-        [Q, *], excluded int32 words [Q or 1, (n + 31) // 32].  Writes `out` (a new matrix unless given;
-        `scores` itself works in place) and returns it."""
+        [Q, *], excluded int32 words [Q or 1, (n + 31) // 32].  Writes `out` (a new matrix unless given, its
+        rows apart where those of `scores` are; `scores` itself works in place) and returns it."""
         torch = _torch or _use_torch()
         p, kind, Q, n, ld = self._rows("scores", scores)
         if out is None:

@@ -233,11 +233,13 @@ cudaError_t quantize_t(const void* x, int64_t rows, int dim, int64_t ld, uint8_t
 // all four instructions of a stage name the same byte of the word (the scale ids of the instruction
 // descriptor), byte (k-block mod 4).
 //
-// What bounds it: the base's bytes with not too many queries (64 x 1M x 512 with
-// its 256 MB of scores: 129 us, 6.0 TB/s), the scores' bytes with many and short rows (4001 x 100003 x
-// 256 bf16: 193 us, 4.3 TB/s, where filling as much memory takes 203 us), and with many and long rows
+// What bounds it: the base's bytes with not too many queries (64 x 1M x 512 with its 256 MB of scores:
+// 129 us, 6.0 TB/s); memory with many queries and short rows (4001 x 100003 x 256 bf16: 194 us, 800 MB
+// written at 4.1 TB/s), and the load side where rows of codes lie an odd multiple of 16 bytes apart and
+// every other one starts inside a 32-byte sector (200 columns: 243 us, 226 with rows 224 bytes apart; 192
+// columns: 205); with many and long rows
 // shared memory: a stage's 48 KB arrive in 384 cycles and are read in another 384, against 512 cycles
-// of products (4096 x 8192 x 4096: 108 to 118 us alone, 2.3 to 2.5 PFLOP/s; 137 us under a power cap).  Pairs of SMs
+// of products (4096 x 8192 x 4096: 116 to 120 us alone, 2.3 to 2.4 PFLOP/s; 138 us under a power cap).  Pairs of SMs
 // on one tile would halve the row tile's share of that; not built.
 //
 // Tensor memory: two accumulators of 256 columns that share 64 (0-255 and 192-447) and, from 448,
@@ -908,8 +910,9 @@ fp8_scores_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // holds one base row's scores, so all eight epilogue warps have work and a warp stores a query's 32 scores
 // side by side straight from its registers, at any alignment.  Bound by memory: 1 x 1M x 512 79 us,
 // 6.6 TB/s; 32 x 1M x 512 fp32 98 us (a query tile: 100); 1 x 4M x 128 83 us (165); where rows are short,
-// by the tensor copies, which take their time per row: 16 x 1000003 x 100 bf16 32 us, 32 x 300k x 128 17 us
-// (21.5), 17 x 2M x 100 70 us (87); against the rule, 32 x 1M x 130 bf16 51.8 us (51).  The query tile is
+// by the tensor copies, which take their time per row more than per byte (16 x 1M bf16: 64 columns 28 us, 128
+// columns 32; 17 x 2M fp32: 53 and 71): 16 x 1000003 x 100 bf16 32 us, 32 x 300k x 128 17 us (21.5), 17 x 2M x
+// 100 70 us (87); against the rule, 32 x 1M x 130 bf16 51.8 us (51).  The query tile is
 // kept, if its k-blocks fit the stages: its rows copied with every row tile cost 16 x 1000003 x 100 47 us.
 // 64 queries lose: 64 x 1M x 128 bf16 takes 50 us against 47 in query tiles.  (Scores through shared memory and tensor stores: 16.5 us for 32 x
 // 300k x 128, but 76 for 17 x 2M x 100 and 84 for 1 x 1M x 512.)

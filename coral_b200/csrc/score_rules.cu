@@ -11,11 +11,11 @@
 // every column that either list touches: a thread whose columns are untouched reads one word of bits
 // and no table.  Then it applies the rules and stores.  No table in global memory, nothing to clear
 // between calls, one launch.  The history is read once per CTA, from L2: wider columns would read it
-// less often but leave fewer CTAs an SM, and latency, not that traffic, is what a CTA waits for.
+// less often but leave fewer CTAs an SM.
 //
 // Measured: 32 x 1M fp32 with a shared mask 42 us, 250 MB at 5.9 TB/s; 64 x 128000 bf16, histories of
-// 2000, nine tenths excluded, 11.7 us (20 MB would take 3: three waves of CTAs, each a chain of mask,
-// scores, tables and stores).  With tables read for every column, eight to a thread, the latter took
+// 2000, nine tenths excluded, 11.7 us (20 MB would take 3: each of a row's 32 CTAs reads the whole history and
+// clears its tables, in three waves and a chain of mask, scores, tables and stores).  With tables read for every column, eight to a thread, the latter took
 // 27 us, on bank conflicts.
 #include <math_constants.h>
 

@@ -23,7 +23,7 @@
 // Measured: 256 x 128000 bf16, k = 100: 20 us, of which the first pass takes 8 to 11 (65.5 MB at up to
 // 6 TB/s), the bound 2, the second pass 4.5, the order 1.5; one pass against a running threshold, with
 // the buffer cut now and then, took 45 us, because nearly every warp then held something to append.
-// 1 x 1M fp32, k = 10: 7.2 us in two launches; k = 1000: 35 us (9 more with one key a thread in flight in
+// 1 x 1M fp32, k = 10: 7.4 us in two launches; k = 1000: 35 us (9 more with one key a thread in flight in
 // the second).
 #include <math_constants.h>
 
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads) topk_join_kernel(const TopkArgs a, c
 
 // Keys a slice may leave: with some room above k, few slices need a selection of their own.  The bound is
 // the looser the larger k (30 x 1M fp32, k = 1000: 68 us with a half, 73 with a quarter; 1 x 1M, k = 10:
-// 7.3 with a quarter, 7.5 with a half).
+// 0.2 us more with a half).
 int slots_of(int k) { return k + (k > 256 ? k / 2 : k / 4) + 16; }
 
 int topk_splits(int Q, int64_t n, int k, int bytes, int sm_count) {
