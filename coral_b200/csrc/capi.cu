@@ -30,18 +30,23 @@ namespace {
 
 thread_local std::string g_create_error;      // failures without a handle
 
-// A thread's last failure with a handle: another thread's on the same handle does not replace the text
-// that this one is about to ask for.
-struct LastError {
-    uint64_t handle = 0;
-    std::string text;
-};
-thread_local LastError t_error;
-
 // Handles are told apart by a number of their own: an address comes again after coral_index_destroy.
 std::atomic<uint64_t> g_handles;
-// Per handle, how many of its failed waits this thread has been told of.
-thread_local std::map<uint64_t, uint64_t> t_failures_told;
+
+// What a thread keeps of handles.
+struct OfThread {
+    // Its last failure with a handle: another thread's on the same handle does not replace the text that this
+    // one is about to ask for.
+    uint64_t failed_handle = 0;
+    std::string error;
+    std::string other_error;                  // a text that it asked for and that is not its own
+    std::map<uint64_t, uint64_t> told;        // per handle, how many of its failed waits it has been told of
+    ~OfThread();
+};
+thread_local bool t_over = false;             // its OfThread is gone, as for a handle that a static object destroys
+thread_local OfThread t_own;
+OfThread::~OfThread() { t_over = true; }
+OfThread* of_thread() { return t_over ? nullptr : &t_own; }
 
 // Control block shared with the kernel: word 0 = query counter | error flag, word 1 = hop
 // total, words 4..8 = record of the first failed index check (self-checking build only).
@@ -165,8 +170,10 @@ int fail(coral_index* h, int code, const std::string& msg) {
         std::lock_guard<std::mutex> lock(h->err_mu);
         h->err = msg;
     }
-    t_error.text = msg;
-    t_error.handle = h->number;
+    if (OfThread* t = of_thread()) {
+        t->error = msg;
+        t->failed_handle = h->number;
+    }
     return code;
 }
 
@@ -378,11 +385,12 @@ int coral_compiled_sm(void) { return 100; }
 
 const char* coral_last_error(coral_index_t* h) {
     if (!h) return g_create_error.c_str();
-    if (t_error.handle == h->number) return t_error.text.c_str();
-    thread_local std::string any;      // of another thread, or of a call before this thread's last failure elsewhere
+    OfThread* t = of_thread();
+    if (!t) return "";
+    if (t->failed_handle == h->number) return t->error.c_str();
     std::lock_guard<std::mutex> lock(h->err_mu);
-    any = h->err;
-    return any.c_str();
+    t->other_error = h->err;
+    return t->other_error.c_str();
 }
 
 int coral_index_create(coral_index_t** out, int device, int64_t n, int dim, int max_degree, int metric) {
@@ -406,7 +414,7 @@ int coral_index_create(coral_index_t** out, int device, int64_t n, int dim, int 
     }
     if (prop.major != 10) return fail(h, CORAL_ERR_NOGPU, "kernels are built for sm_100a only");
     h = new (std::nothrow) coral_index();
-    if (!h) return fail(nullptr, CORAL_ERR_CUDA, "out of host memory");
+    if (!h) return fail(nullptr, CORAL_ERR_CUDA, "no host memory for the thread's state");
     h->device = device;
     h->sm_count = prop.multiProcessorCount;
     h->smem_optin = (int)prop.sharedMemPerBlockOptin;
@@ -464,7 +472,7 @@ int coral_index_destroy(coral_index_t* h) {
     if (h->ev_t1) cudaEventDestroy(h->ev_t1);
     if (h->stream) cudaStreamDestroy(h->stream);
     cudaGetLastError();
-    t_failures_told.erase(h->number);
+    if (OfThread* t = of_thread()) t->told.erase(h->number);
     delete h;
     return CORAL_OK;
 }
@@ -1575,17 +1583,20 @@ bool meets(const void* p, int64_t bytes, const void* other, int64_t other_bytes)
 }
 
 // How many of the handle's failed waits this thread has been told of; for a thread that comes to the handle
-// with a call of its own (`with_call`), those found before it do not count.  Null: out of host memory.
+// with a call of its own (`with_call`), those found before it do not count.  Null: no memory, or the thread
+// is ending.
 uint64_t* failures_told(coral_index* h, bool with_call) {
-    const auto it = t_failures_told.find(h->number);
-    if (it != t_failures_told.end()) return &it->second;
+    OfThread* t = of_thread();
+    if (!t) return nullptr;
+    const auto it = t->told.find(h->number);
+    if (it != t->told.end()) return &it->second;
     uint64_t before = 0;
     if (with_call) {
         std::lock_guard<std::mutex> lock(h->failures_mu);
         before = h->failures;
     }
     try {
-        return &t_failures_told.emplace(h->number, before).first->second;
+        return &t->told.emplace(h->number, before).first->second;
     } catch (const std::bad_alloc&) {
         return nullptr;
     }
@@ -1668,7 +1679,7 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     a.ld = ld;
     a.err = h->h_scores_err;
     a.wait_clocks = h->opt.score_wait_us * kClocksPerUs;
-    if (!failures_told(h, true)) return fail(h, CORAL_ERR_LIMIT, "out of host memory");
+    if (!failures_told(h, true)) return fail(h, CORAL_ERR_LIMIT, "no host memory for the thread's state");
     CK(coral::launch_fp8_scores(a, h->sm_count, stream ? (cudaStream_t)stream : h->stream));
     h->score_launches += 1;
     return CORAL_OK;
@@ -1782,7 +1793,7 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
 int coral_scores_check(coral_index_t* h) {
     ARG(h, "null handle");
     uint64_t* told = failures_told(h, false);
-    if (!told) return fail(h, CORAL_ERR_LIMIT, "out of host memory");
+    if (!told) return fail(h, CORAL_ERR_LIMIT, "no host memory for the thread's state");
     uint64_t now;
     {
         std::lock_guard<std::mutex> lock(h->failures_mu);

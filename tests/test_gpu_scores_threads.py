@@ -97,3 +97,37 @@ def test_the_error_text_of_another_thread(ix):
             ix.set_option("mine", 1)
         in_a_thread(lambda: read(ix))
         assert read(ix).endswith(b"mine") and read(other).endswith(b"nor this") and read(ix).endswith(b"mine")
+
+
+def test_a_handle_that_outlives_its_thread(tmp_path):
+    """A C++ program whose static object destroys its handle: the main thread's own state is gone by then."""
+    import os
+    import subprocess
+    src, exe = tmp_path / "late.cpp", str(tmp_path / "late")
+    src.write_text("""
+#include <cstdio>
+#include "coral_b200.h"
+struct Holder {
+    coral_index_t* h = nullptr;
+    ~Holder() {
+        coral_set_option(h, "none", 1);
+        const bool text = coral_last_error(h) != nullptr;
+        std::printf("destroyed %d %d\\n", coral_index_destroy(h), text);
+        std::fflush(stdout);
+    }
+} holder;
+int main() {
+    if (coral_index_create(&holder.h, 0, 1, 4, 32, CORAL_IP) != CORAL_OK) return 2;
+    coral_index_t* more[8];
+    for (auto& h : more)
+        if (coral_index_create(&h, 0, 1, 4, 32, CORAL_IP) != CORAL_OK || coral_scores_check(h) != CORAL_OK) return 3;
+    return coral_scores_check(holder.h);
+}
+""")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.dirname(capi.lib_path())
+    subprocess.run(["g++", "-std=c++17", "-I" + os.path.join(root, "include"), str(src), "-o", exe, "-L" + lib, "-lcoral_b200",
+                    "-Wl,-rpath," + lib], check=True, capture_output=True, timeout=120)
+    # freed memory is overwritten, so that a use of it shows
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120, env=dict(os.environ, MALLOC_PERTURB_="165"))
+    assert r.returncode == 0 and r.stdout == "destroyed 0 1\n", (r.returncode, r.stdout, r.stderr)
