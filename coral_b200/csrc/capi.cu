@@ -387,7 +387,10 @@ const char* coral_last_error(coral_index_t* h) {
     if (!h) return g_create_error.c_str();
     OfThread* t = of_thread();
     if (!t) return "";
-    if (t->failed_handle == h->number) return t->error.c_str();
+    if (t->failed_handle == h->number) {      // once: later, another thread's failure may be what is asked for
+        t->failed_handle = 0;
+        return t->error.c_str();
+    }
     std::lock_guard<std::mutex> lock(h->err_mu);
     t->other_error = h->err;
     return t->other_error.c_str();

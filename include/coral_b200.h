@@ -472,9 +472,9 @@ int coral_topk_scores(coral_index_t* h, const void* d_scores, int type, int Q, i
  * Every thread is told: one thread's check takes nothing away from another's. */
 int coral_scores_check(coral_index_t* h);
 
-/* Last error text of the handle (or of handle creation when h is NULL): the calling thread's own if its
- * last failure was on this handle, else the last of any thread's.  The text stays until the calling
- * thread's next call. */
+/* Last error text of the handle (or of handle creation when h is NULL).  A thread that asks for the first
+ * time after a failure of its own gets that one's, whatever other threads did meanwhile; else it is the last
+ * of any thread's.  The text stays until the calling thread's next call. */
 const char* coral_last_error(coral_index_t* h);
 
 #ifdef __cplusplus

@@ -99,6 +99,15 @@ def test_the_error_text_of_another_thread(ix):
         assert read(ix).endswith(b"mine") and read(other).endswith(b"nor this") and read(ix).endswith(b"mine")
 
 
+def test_a_later_error_of_another_thread(ix):
+    """A thread that had its own failure, and asked for it, reads what another thread left since."""
+    with pytest.raises(capi.CoralError):
+        ix.set_option("mine", 1)
+    with pytest.raises(capi.CoralError):
+        in_a_thread(lambda: ix.set_option("theirs", 1))
+    assert ix._lib.coral_last_error(ix._h).endswith(b"theirs")
+
+
 def test_a_handle_that_outlives_its_thread(tmp_path):
     """A C++ program whose static object destroys its handle: the main thread's own state is gone by then."""
     import os
