@@ -417,7 +417,7 @@ int coral_index_create(coral_index_t** out, int device, int64_t n, int dim, int 
     }
     if (prop.major != 10) return fail(h, CORAL_ERR_NOGPU, "kernels are built for sm_100a only");
     h = new (std::nothrow) coral_index();
-    if (!h) return fail(nullptr, CORAL_ERR_CUDA, "no host memory for the thread's state");
+    if (!h) return fail(nullptr, CORAL_ERR_CUDA, "out of host memory");
     h->device = device;
     h->sm_count = prop.multiProcessorCount;
     h->smem_optin = (int)prop.sharedMemPerBlockOptin;
@@ -1654,8 +1654,8 @@ int coral_fp8_scores(coral_index_t* h, const uint8_t* d_q_codes, const uint8_t* 
     ARG(ld >= n && ld < (1ll << 31), "ld must be in [n, 2^31)");
     if (((int64_t)Q + 127) / 128 * ((n + 255) / 256) > 0x7fffffffll / 2)
         return fail(h, CORAL_ERR_LIMIT, "too many scores for one call");
-    if (!fits(Q, n, ld, 4)) return fail(h, CORAL_ERR_LIMIT, kTooFar);
     if (Q == 0 || n == 0) return CORAL_OK;
+    if (!fits(Q, n, ld, 4)) return fail(h, CORAL_ERR_LIMIT, kTooFar);
     ARG(d_q_codes && d_q_scales && d_codes && d_scales && d_out, "null argument");
     DeviceScope scope(h->device);
     if (!scope.ok) return fail(h, CORAL_ERR_CUDA, "cudaSetDevice failed");

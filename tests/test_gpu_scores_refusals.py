@@ -45,3 +45,14 @@ def test_types_that_are_none(ix):
         with pytest.raises(capi.CoralError) as e:
             ix.fp8_scores(q, q, 64, **kw)
         assert e.value.code == capi.ERR_ARG
+
+
+def test_empty_rows_may_be_far_apart(ix):
+    """No column, however many rows and whatever the distance between them: nothing to do, nothing to refuse."""
+    lib, h, far, OK = ix._lib, ix._h, (1 << 31) - 1, capi.OK
+    assert lib.coral_fp8_scores(h, None, None, far, None, None, 0, 64, 1.0, None, None, 0, far, 1) == OK
+    assert lib.coral_adjust_scores(h, None, 0, far, 0, far, None, 0, None, None, None, 0, None, 0, None, far, 1) == OK
+    assert lib.coral_fp8_quantize(h, None, 0, 0, 64, far, None, None, 1) == OK
+    pad = torch.zeros(2, 3, 2, dtype=torch.int32, device="cuda")
+    assert lib.coral_topk_scores(h, None, 0, 3, 0, far, 2, 0, pad[0].data_ptr(), pad[1].data_ptr(), None, 0, 1) == OK
+    assert bool((pad[0] == -1).all()) and bool((pad[1].view(torch.float32) == -3.4028234663852886e38).all())
