@@ -96,3 +96,22 @@ def test_every_thread_is_told_of_a_failed_wait(ix):
     assert [w(failed, ix) for w in (first, late, second, watcher)] == [True] * 4
     with capi.Index(1, 4, 32, "ip") as other:
         assert not first(failed, other) and not watcher(failed, other)
+
+
+@pytest.mark.parametrize("Q,n,dim,dtype,lead", CALLS + [(3, 40_000, 20_000, F32, 0), (128, 512, 65536, F32, 0), (200, 20_000, 5000, BF16, 0)])
+def test_a_wait_that_runs_out_on_the_way(ix, Q, n, dim, dtype, lead):
+    """Short limits, which some waits keep: the call ends whichever runs out, and the next one is right."""
+    q, base = rows8(ix, Q, dim, 1, 2), rows8(ix, n, dim, 2, 2)
+    out = torch.zeros(Q, n + 8, dtype=dtype, device="cuda")[:, lead:lead + n]
+    want = ix.fp8_scores(q, base, dim, 2.0 ** -9, dtype=dtype)
+    for limit in (1, 3, 10, 30):
+        for _ in range(3):
+            ix.set_option("score_wait_us", limit)
+            ix.fp8_scores(q, base, dim, 2.0 ** -9, out=out)
+            torch.cuda.synchronize()
+            if not failed(ix):
+                assert torch.equal(out, want)
+        ix.set_option("score_wait_us", 2_000_000)
+        ix.fp8_scores(q, base, dim, 2.0 ** -9, out=out)
+        torch.cuda.synchronize()
+        assert not failed(ix) and torch.equal(out, want)
